@@ -50,6 +50,49 @@ void* Context::optional_scratch(int slot, size_t bytes)
     return p;
 }
 
+void* Context::workspace(int slot, size_t bytes)
+{
+    if (slot < 0 || slot >= kScratchCount) return nullptr;
+    if (scratch_bytes[slot] >= bytes && scratch_ptr[slot] != nullptr) return scratch_ptr[slot];
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &st) != hipSuccess) {
+        (void)hipGetLastError();
+        error = "workspace: the stream's capture state is unknown";
+        return nullptr;
+    }
+    if (st != hipStreamCaptureStatusNone) {
+        error = "workspace too small under stream capture: make the call once before capturing it";
+        return nullptr;
+    }
+    retired.reserve(retired.size() + 1);
+    size_t grown = 2 * scratch_bytes[slot];
+    if (grown < bytes) grown = bytes;
+    void* p = nullptr;
+    // Another stream of the program may be captured meanwhile.
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) {
+        (void)hipGetLastError();
+        error = "workspace: the thread's capture mode could not be set";
+        return nullptr;
+    }
+    hipError_t e = hipMalloc(&p, grown);
+    if (e != hipSuccess && grown > bytes) {
+        (void)hipGetLastError();
+        grown = bytes;
+        e = hipMalloc(&p, grown);
+    }
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        error = "workspace allocation failed (" + std::to_string(bytes) + " bytes)";
+        return nullptr;
+    }
+    if (scratch_ptr[slot] != nullptr) retired.push_back(scratch_ptr[slot]);
+    scratch_ptr[slot] = p;
+    scratch_bytes[slot] = grown;
+    return p;
+}
+
 void Context::release(int slot)
 {
     if (scratch_ptr[slot] == nullptr || hipStreamSynchronize(stream) != hipSuccess) return;
@@ -101,6 +144,63 @@ int guarded(gofann_ctx* c, F&& f)
         return as_ctx(c)->fail(GOFANN_ERR_INVALID, e.what());
     }
 }
+
+// Checks of the key/value cache calls.  *empty: nothing to compute.
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+bool kv_rows(const gofann_kv_rows* r)
+{
+    return r != nullptr && r->data != nullptr && aligned(r->data, 2);
+}
+
+int kv_check(Context* ctx, const char* call, const gofann_kv_cache* c, const gofann_kv_batch* b, bool* empty)
+{
+    const std::string at = std::string(call) + ": ";
+    if (c == nullptr || b == nullptr) return ctx->fail(GOFANN_ERR_INVALID, at + "null cache or batch");
+    if (c->elem != GOFANN_ELEM_BF16 && c->elem != GOFANN_ELEM_F16)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "elem must be BF16 or F16");
+    if (c->dim != 64 && c->dim != 128 && c->dim != 256)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "dim must be 64, 128 or 256");
+    if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "page_size must be 32, 64, 128 or 256");
+    if (c->kv_heads == 0 || c->kv_heads > 4096)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "kv_heads must be in [1, 4096]");
+    // Tiles of 32 positions are counted in 32 bits.
+    if (c->pages > 0x7FFFFFFFu ||
+        static_cast<uint64_t>(c->pages) * c->kv_heads * (c->page_size / 32) > 0xFFFFFFFFull)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "too many pages");
+    if (c->k_codes == nullptr || c->k_scales == nullptr || c->v_codes == nullptr || c->v_scales == nullptr)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "a cache array is null");
+    if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->v_scales, 8) ||
+        !aligned(c->box, 16))
+        return ctx->fail(GOFANN_ERR_INVALID, at + "codes and boxes must be 16-byte aligned, v_scales 8-byte");
+    if ((c->box == nullptr) != (c->box_scale == nullptr))
+        return ctx->fail(GOFANN_ERR_INVALID, at + "box and box_scale come together");
+    if (b->sequences > 65535)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "at most 65535 sequences");
+    if (b->queries > 0x7FFFFFFFu || b->max_length > 0x7FFFFF00u || b->table_width > 0x7FFFFFu)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "queries, max_length or table_width too large");
+    *empty = b->sequences == 0 || b->queries == 0 ||
+             (b->query_offsets != nullptr && b->max_queries == 0);
+    if (*empty) return GOFANN_OK;
+    if (b->lengths == nullptr || (b->page_table == nullptr && b->table_width > 0))
+        return ctx->fail(GOFANN_ERR_INVALID, at + "page_table or lengths is null");
+    if (b->table_stride < b->table_width)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "table_stride below table_width");
+    if (b->query_offsets == nullptr && b->queries != b->sequences)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "without query_offsets there is one token a sequence");
+    if (b->query_offsets != nullptr && b->max_queries > b->queries)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "max_queries above queries");
+    return GOFANN_OK;
+}
+
+int kv_check_heads(Context* ctx, const char* call, const gofann_kv_cache* c, uint32_t heads)
+{
+    if (heads == 0 || heads % c->kv_heads != 0 || heads / c->kv_heads > 1024)
+        return ctx->fail(GOFANN_ERR_INVALID,
+                         std::string(call) + ": heads must be 1 to 1024 times kv_heads");
+    return GOFANN_OK;
+}
 }  // namespace
 
 extern "C" {
@@ -142,6 +242,7 @@ void gofann_destroy(gofann_ctx* c)
     gofann::destroy_blas(ctx);
     for (int i = 0; i < Context::kScratchCount; ++i)
         if (ctx->scratch_ptr[i]) (void)hipFree(ctx->scratch_ptr[i]);
+    for (void* p : ctx->retired) (void)hipFree(p);
     delete ctx;
 }
 
@@ -559,6 +660,62 @@ int gofann_build_reach(gofann_ctx* c, const uint32_t* graph, uint32_t n, uint32_
 {
     return guarded(c, [&](Context* ctx) {
         return gofann::build_reach(ctx, graph, n, degree, entry_row, reached, reached_count);
+    });
+}
+
+int gofann_kv_append(gofann_ctx* c, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                     const gofann_kv_rows* k, const gofann_kv_rows* v,
+                     const gofann_kv_rows* k_held, const gofann_kv_rows* v_held)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (int rc = kv_check(ctx, "kv_append", cache, batch, &empty)) return rc;
+        if (empty) return GOFANN_OK;
+        if (!kv_rows(k) || !kv_rows(v))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_append: k and v rows missing or misaligned");
+        if ((k_held && !kv_rows(k_held)) || (v_held && !kv_rows(v_held)))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_append: held rows misaligned");
+        return gofann::kv_append(ctx, cache, batch, k, v, k_held, v_held);
+    });
+}
+
+int gofann_kv_select(gofann_ctx* c, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                     const gofann_kv_rows* q, uint32_t heads, uint32_t width, uint32_t first,
+                     uint32_t last, int32_t* out_blocks)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (int rc = kv_check(ctx, "kv_select", cache, batch, &empty)) return rc;
+        if (cache->box == nullptr)
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_select: the cache keeps no boxes");
+        if (int rc = kv_check_heads(ctx, "kv_select", cache, heads)) return rc;
+        if (width == 0 || width > (1u << 24) || static_cast<uint64_t>(first) + last > width)
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_select: width must be in [max(1, first + last), 2^24]");
+        if (empty) return GOFANN_OK;
+        if (!kv_rows(q)) return ctx->fail(GOFANN_ERR_INVALID, "kv_select: q rows missing or misaligned");
+        if (out_blocks == nullptr || reinterpret_cast<uintptr_t>(out_blocks) % 4 != 0)
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_select: out_blocks missing or misaligned");
+        return gofann::kv_select(ctx, cache, batch, q, heads, width, first, last, out_blocks);
+    });
+}
+
+int gofann_kv_attention(gofann_ctx* c, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                        const gofann_kv_rows* q, uint32_t heads, float scale,
+                        const int32_t* blocks, uint32_t width, const gofann_kv_rows* out,
+                        float* out_lse)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (int rc = kv_check(ctx, "kv_attention", cache, batch, &empty)) return rc;
+        if (int rc = kv_check_heads(ctx, "kv_attention", cache, heads)) return rc;
+        if (!(scale > 0.0f) || !(scale <= 3.0e38f))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: scale must be positive and finite");
+        if (blocks != nullptr && (width == 0 || width > (1u << 24)))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: width of a block list must be in [1, 2^24]");
+        if (empty) return GOFANN_OK;
+        if (!kv_rows(q) || !kv_rows(out))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: q or out rows missing or misaligned");
+        return gofann::kv_attention(ctx, cache, batch, q, heads, scale, blocks, width, out, out_lse);
     });
 }
 

@@ -7,6 +7,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include "gofann_hip.h"
 
@@ -24,7 +25,8 @@ struct Context {
         kScratchBuild = 4,  // index construction (k-means, kNN, graph optimisation)
         kScratchLog = 5,    // admission logs of the set frontier
         kScratchScan = 6,   // the exact posting scan's lists per part before the merge
-        kScratchCount = 7
+        kScratchKv = 7,     // key/value cache calls: block keys, partial outputs (workspace())
+        kScratchCount = 8
     };
 
     int device = 0;
@@ -61,6 +63,13 @@ struct Context {
     // call may replace); another stream's capture is left intact, which an
     // allocation in the default capture mode would break.
     void* optional_scratch(int slot, size_t bytes);
+    // The same for a buffer whose address a captured graph may keep: where it
+    // must grow, the old one stays until gofann_destroy (sizes at least double,
+    // so all of them hold no more than twice the last).  nullptr, with the
+    // reason in `error`, on failure and where the stream is captured and the
+    // buffer too small.
+    void* workspace(int slot, size_t bytes);
+    std::vector<void*> retired;
     // Frees `slot`'s buffer, once the stream is done with it.
     void release(int slot);
 };
@@ -224,5 +233,14 @@ int build_reach(Context* ctx, const uint32_t* graph, uint32_t n, uint32_t degree
                 uint32_t* reached, uint32_t* out_count);
 int rabitq_prepare(Context* ctx, const gofann_rabitq_view* rq, const float* queries,
                    uint32_t count, const float* rotation, gofann_rabitq_queries* out);
+int kv_append(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+              const gofann_kv_rows* k, const gofann_kv_rows* v, const gofann_kv_rows* k_held,
+              const gofann_kv_rows* v_held);
+int kv_select(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+              const gofann_kv_rows* q, uint32_t heads, uint32_t width, uint32_t first,
+              uint32_t last, int32_t* out_blocks);
+int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                 const gofann_kv_rows* q, uint32_t heads, float scale, const int32_t* blocks,
+                 uint32_t width, const gofann_kv_rows* out, float* out_lse);
 
 }  // namespace gofann

@@ -1,0 +1,537 @@
+// kv_attention.hpp -- attention over the paged 4-bit key/value cache, and the
+// join of its partial results.
+#pragma once
+
+#include "kv_common.hpp"
+
+namespace gofann {
+namespace kv {
+
+struct AttendArgs {
+    Batch batch;
+    Rows q, out;
+    const uint8_t* k_codes;
+    const uint8_t* k_scales;
+    const uint8_t* v_codes;
+    const uint8_t* v_scales;
+    const int32_t* blocks;  // [queries][kv_heads][width] or NULL
+    float* lse;             // [queries][heads] or NULL
+    float* part_o;          // [item][split][rows][dim], splits > 1
+    float* part_ml;         // [item][split][rows][2]: running maximum, sum
+    float scale_log2;       // scale * log2(e)
+    int group;              // heads a key/value head
+    int width;
+    int row_tiles;          // row tiles of a sequence (listed: of a token times tokens)
+    int token_tiles;        // listed: row tiles of one token's heads
+    int splits;
+    int split_tiles;        // tiles of a split
+};
+
+// The rows of one row tile: rows [begin, end) of the sequence's flattened
+// (token, head of the group) rows, and the positions they reach.
+struct RowTile {
+    int begin, end;
+    int first_pos, last_pos;  // of the first and the last row's token
+    int token;                // listed: the one token
+};
+
+__device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int rows, int len, int n)
+{
+    RowTile t;
+    if (a.blocks != nullptr) {
+        t.token = index / a.token_tiles;
+        t.begin = t.token * a.group + (index % a.token_tiles) * rows;
+        t.end = (t.token + 1) * a.group;
+        if (t.token >= n) t.end = t.begin;
+    } else {
+        t.token = 0;
+        t.begin = index * rows;
+        t.end = n * a.group;
+    }
+    if (t.end > t.begin + rows) t.end = t.begin + rows;
+    t.first_pos = len - n + t.begin / a.group;
+    t.last_pos = len - n + (t.end - 1) / a.group;
+    return t;
+}
+
+// Tiles of 32 positions that a row tile reads.
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, const RowTile& t)
+{
+    if (t.end <= t.begin || t.last_pos < 0) return 0;
+    if (a.blocks != nullptr) return a.width << (a.batch.page_shift - 5);
+    return (t.last_pos >> 5) + 1;
+}
+
+// What a lane loads of one tile: keys of two positions, values of eight.
+template <int D>
+struct Raw {
+    static constexpr int kGroups = D == 256 ? 2 : 1;
+    uint32_t k[2][D / 32];
+    uint32_t ks[2][kGroups];
+    uint32_t v[D / 16];
+    uint32_t vs[2];
+};
+
+// One row tile of one key/value head over one split of its positions.
+//
+// A tile of 32 positions is two 16 x 16 score tiles S^T = K Q^T and D / 16
+// product tiles O^T += V^T P^T, all v_mfma_f32_16x16x32.  The order of the
+// contracted index is free as long as both operands agree, and is chosen so
+// that nothing crosses lanes: lane (r, g) = (lane % 16, lane / 16)
+//   * holds, as rows of S^T, keys 8 (r / 4) + r % 4 and that plus 4, whose
+//     channels [g dim/4, ..) are one or two 16-byte loads under one scale;
+//   * gets the scores of query r against the eight positions 8 g .. 8 g + 7,
+//     which are just the eight slots of P^T that lane (r, g) feeds;
+//   * holds, as rows of V^T, the dim / 16 channels of unit r at those eight
+//     positions, one run of dim / 4 bytes in the cache;
+//   * ends with the channels [g dim/4, (g+1) dim/4) of query r's output.
+// The 4-bit codes become 16-bit elements by the hardware's conversion, which
+// applies the group's power of two; both are exact.
+template <class E, int D, int NT, int WT>
+__global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
+{
+    using V8 = typename E::V8;
+    constexpr int kRows = 16 * NT;
+    constexpr int kUnit = D / 16;  // channels of a unit, tiles of O
+    constexpr float kSlack = 8.0f;
+    const Batch& t = a.batch;
+    const int lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int r16 = lane % 16, g4 = lane / 16;
+    const int h = blockIdx.x % t.kv_heads;
+    const int split = blockIdx.x / t.kv_heads;
+    const int index = gridDim.y - 1 - blockIdx.y;  // the longest rows first
+    const int b = blockIdx.z;
+    const int len = t.length(b);
+    const int q0 = t.first_query(b);
+    const int n = t.new_tokens(b, q0);
+    RowTile rt;
+    if constexpr (WT == 1)
+        rt = row_tile(a, index * 4 + wave, kRows, len, n);
+    else
+        rt = row_tile(a, index, kRows, len, n);
+    if (rt.end <= rt.begin) return;  // WT > 1: the whole workgroup; WT == 1: no barrier follows
+    const int tiles = tiles_of(a, rt);
+    const int tile_begin = split * a.split_tiles;
+    if (split > 0 && tile_begin >= tiles) return;
+    const int tile_end = tile_begin + a.split_tiles < tiles ? tile_begin + a.split_tiles : tiles;
+    const int hi_pos = rt.last_pos + 1;                         // positions of the last row
+    const int all_see = rt.first_pos + 1;                       // positions that every row sees
+
+    // The rows' queries and limits.
+    V8 q[NT][D / 32];
+    int limit[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = rt.begin + 16 * nt + r16;
+        const bool in = row < rt.end;
+        const int i = (in ? row : rt.begin) / a.group;
+        const int head = h * a.group + (in ? row : rt.begin) % a.group;
+        limit[nt] = in ? len - n + i + 1 : 0;
+        const uint16_t* const p = a.q.p + (q0 + i) * a.q.token_stride + head * a.q.head_stride;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            // Channels that the dword j of a lane's keys holds.
+            const int c = D == 64 ? 16 * g4 + 8 * j : 128 * (j / 4) + 32 * g4 + 8 * (j % 4);
+            q[nt][j] = __builtin_bit_cast(V8, load8(p + c, a.q.wide));
+        }
+    }
+
+    f32x4 o[NT][kUnit];
+    float m[NT], mu[NT], sum[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int c = 0; c < kUnit; ++c) o[nt][c] = f32x4{0, 0, 0, 0};
+        m[nt] = -__builtin_inff();
+        mu[nt] = 0.0f;
+        sum[nt] = 0.0f;
+    }
+
+    const auto load = [&](uint32_t at, Raw<D>& x) {
+        const uint8_t* const kc = a.k_codes + static_cast<uint64_t>(at) * (16 * D);
+        const uint8_t* const ks = a.k_scales + static_cast<uint64_t>(at) * D;
+        const uint8_t* const vc = a.v_codes + static_cast<uint64_t>(at) * (16 * D);
+        const uint8_t* const vs = a.v_scales + static_cast<uint64_t>(at) * D;
+        const uint32_t pos = 8 * (r16 / 4) + r16 % 4;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const uint32_t p = pos + 4 * s;
+            if constexpr (D == 64) {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(kc + p * (D / 2) + 8 * g4);
+                x.k[s][0] = v[0];
+                x.k[s][1] = v[1];
+                x.ks[s][0] = ks[p * (D / 32) + g4 / 2];
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 128; ++c) {
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(kc + p * (D / 2) + 64 * c + 16 * g4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x.k[s][4 * c + j] = v[j];
+                    x.ks[s][c] = ks[p * (D / 32) + 4 * c + g4];
+                }
+            }
+        }
+        const uint8_t* const vp = vc + (g4 * 16 + r16) * (D / 4);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(vp + 16 * c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.v[4 * c + j] = v[j];
+        }
+        const u32x2 s = *reinterpret_cast<const u32x2*>(vs + (g4 * (D / 32) + r16 * kUnit / 32) * 8);
+        x.vs[0] = s[0];
+        x.vs[1] = s[1];
+    };
+
+    const auto compute = [&](const Raw<D>& x, int t0, uint32_t word) {
+        // Scores.
+        f32x4 s[NT][2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][half] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const uint32_t sc = x.ks[half][D == 256 ? j / 4 : 0] << 23;
+                const uint32_t c = x.k[half][j];
+                const u32x4 e{E::template decode<0>(c, sc), E::template decode<1>(c, sc),
+                              E::template decode<2>(c, sc), E::template decode<3>(c, sc)};
+                const V8 k8 = __builtin_bit_cast(V8, e);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s[nt][half] = E::mfma(k8, q[nt][j], s[nt][half]);
+            }
+        }
+        uint32_t scale[8];  // of the eight positions' values, in bits 30:23
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            scale[4 * w] = x.vs[w] << 23;
+            scale[4 * w + 1] = x.vs[w] << 15;
+            scale[4 * w + 2] = x.vs[w] << 7;
+            scale[4 * w + 3] = x.vs[w] >> 1;
+        }
+        const bool masked = word != 0xFFFFFFFFu || t0 + kTile > all_see;
+        if (masked) {
+            const uint32_t mine = word >> (8 * g4);
+            // A position that no row sees may hold anything: its scale must
+            // not turn a weight of zero into a NaN.
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(mine >> e & 1u)) scale[e] = 127u << 23;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                int left = limit[nt] - t0 - 8 * g4;
+                left = left < 0 ? 0 : left > 8 ? 8 : left;
+                const uint32_t ok = mine & ((1u << left) - 1u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    s[nt][e / 4][e % 4] = (ok >> e & 1u) ? s[nt][e / 4][e % 4] : -__builtin_inff();
+            }
+        }
+        V8 p[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            // The running maximum is renewed only where a score passes it by
+            // more than kSlack (in powers of two): until then the weights are
+            // at most 2^kSlack, which costs 32-bit sums nothing.
+            float top = s[nt][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top = fmaxf(top, s[nt][e / 4][e % 4]);
+            top *= a.scale_log2;
+            if (__any(top > m[nt] + kSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float fresh = fmaxf(m[nt], top);
+                const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
+                const float f = __builtin_amdgcn_exp2f(m[nt] - keep);
+                sum[nt] *= f;
+#pragma unroll
+                for (int c = 0; c < kUnit; ++c) o[nt][c] *= f;
+                m[nt] = fresh;
+                mu[nt] = keep;
+            }
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][e / 4][e % 4], a.scale_log2, -mu[nt]));
+                sum[nt] += w[e];
+            }
+            // The weights enter the product in 16 bits, as the values do; their
+            // sum stays in 32.
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[nt][e] = static_cast<typename E::T>(w[e]);
+        }
+        // Values: two positions' bytes to pairs of channels, then to pairs of
+        // positions a channel.
+        each<kUnit / 2>([&](auto pair) {
+            constexpr int c = decltype(pair)::value;  // channels 2 c, 2 c + 1 of the unit
+            uint32_t d[8];
+            each<8>([&](auto pos) {
+                constexpr int e = decltype(pos)::value;
+                constexpr int byte = e * (D / 32) + c;
+                d[e] = E::template decode<byte % 4>(x.v[byte / 4], scale[e]);
+            });
+            u32x4 even, odd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                even[j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], 0x05040100u);
+                odd[j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], 0x07060302u);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                o[nt][2 * c] = E::mfma(__builtin_bit_cast(V8, even), p[nt], o[nt][2 * c]);
+                o[nt][2 * c + 1] = E::mfma(__builtin_bit_cast(V8, odd), p[nt], o[nt][2 * c + 1]);
+            }
+        });
+    };
+
+    // This wave's tiles, 64 at a time: lane l looks up the l-th one's page and
+    // filter word, so that only tiles with a visible position are visited and
+    // the next one's address is at hand while it is loaded.
+    const int step = WT;
+    const int first_tile = tile_begin + (WT == 1 ? 0 : wave);
+    const int page_tiles_shift = t.page_shift - 5;
+    for (int base = first_tile; base < tile_end; base += 64 * step) {
+        const int tile = base + lane * step;
+        uint32_t at = 0, word = 0;
+        int t0 = 0;
+        if (tile < tile_end) {
+            int block = tile >> page_tiles_shift;
+            const int within = tile & ((1 << page_tiles_shift) - 1);
+            if (a.blocks != nullptr)
+                block = a.blocks[(static_cast<int64_t>(q0 + rt.token) * t.kv_heads + h) * a.width + block];
+            const int page = t.page(b, block);
+            // A block of a list may lie anywhere: only positions below hi_pos count.
+            if (page >= 0 && block <= (rt.last_pos >> t.page_shift)) {
+                t0 = (block << t.page_shift) + kTile * within;
+                if (t0 < hi_pos) {
+                    word = t.word(b, t0 >> 5);
+                    if (hi_pos - t0 < 32) word &= (1u << (hi_pos - t0)) - 1u;
+                    at = ((static_cast<uint32_t>(page) * t.kv_heads + h) << page_tiles_shift) + within;
+                }
+            }
+        }
+        uint64_t live = __ballot(word != 0);
+        if (live == 0) continue;
+        Raw<D> cur, next;
+        int i = __builtin_ctzll(live);
+        live &= live - 1;
+        load(__builtin_amdgcn_readlane(at, i), cur);
+        while (true) {
+            const int now = i;
+            if (live != 0) {
+                i = __builtin_ctzll(live);
+                live &= live - 1;
+                load(__builtin_amdgcn_readlane(at, i), next);
+            } else {
+                i = -1;
+            }
+            compute(cur, __builtin_amdgcn_readlane(t0, now), __builtin_amdgcn_readlane(word, now));
+            if (i < 0) break;
+            cur = next;
+        }
+    }
+
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        sum[nt] += __shfl_xor(sum[nt], 16);
+        sum[nt] += __shfl_xor(sum[nt], 32);
+    }
+
+    if constexpr (WT > 1) {
+        // The four waves' maxima, sums and outputs joined; wave w then holds
+        // the output of O tiles [w kUnit/4, (w+1) kUnit/4).
+        constexpr int kQ = kUnit / 4;
+        __shared__ float wm[4][kRows], ws[4][kRows];
+        __shared__ f32x4 wo[3][NT][kQ][64];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            if (g4 == 0) {
+                wm[wave][16 * nt + r16] = m[nt];
+                ws[wave][16 * nt + r16] = sum[nt];
+            }
+        __syncthreads();
+        float factor[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = 16 * nt + r16;
+            float top = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+            const float keep = top == -__builtin_inff() ? 0.0f : top;
+            factor[nt] = __builtin_amdgcn_exp2f(m[nt] - keep);
+            float total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) total += ws[w][r] * __builtin_amdgcn_exp2f(wm[w][r] - keep);
+            m[nt] = top;
+            sum[nt] = total;
+        }
+        f32x4 mine[NT][kQ];
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+            // The three other waves' shares of wave `part`'s tiles, added in
+            // the order of the waves.
+            if (wave != part) {
+                const int slot = wave < part ? wave : wave - 1;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < kQ; ++c) wo[slot][nt][c][lane] = o[nt][part * kQ + c] * factor[nt];
+            }
+            __syncthreads();
+            if (wave == part) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < kQ; ++c)
+                        mine[nt][c] = o[nt][part * kQ + c] * factor[nt] + wo[0][nt][c][lane] +
+                                      wo[1][nt][c][lane] + wo[2][nt][c][lane];
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int row = rt.begin + 16 * nt + r16;
+            if (row >= rt.end) continue;
+            // Lane (r, g) holds, of units 4 g + i, the channels [wave kQ, ..).
+            if (a.splits > 1) {
+                const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
+                const int64_t at = (item * a.splits + split) * kRows + 16 * nt + r16;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < kQ; ++c)
+                        a.part_o[at * D + (4 * g4 + i) * kUnit + wave * kQ + c] = mine[nt][c][i];
+                if (g4 == 0 && wave == 0) {
+                    a.part_ml[2 * at] = m[nt];
+                    a.part_ml[2 * at + 1] = sum[nt];
+                }
+            } else {
+                const int i_tok = row / a.group, head = h * a.group + row % a.group;
+                uint16_t* const p = a.out.p + (q0 + i_tok) * a.out.token_stride + head * a.out.head_stride;
+                const float inv = sum[nt] != 0.0f ? 1.0f / sum[nt] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < kQ; ++c)
+                        p[(4 * g4 + i) * kUnit + wave * kQ + c] = __builtin_bit_cast(
+                            uint16_t, static_cast<typename E::T>(mine[nt][c][i] * inv));
+                if (a.lse != nullptr && g4 == 0 && wave == 0)
+                    a.lse[static_cast<int64_t>(q0 + i_tok) * t.kv_heads * a.group + head] =
+                        (m[nt] + __builtin_log2f(sum[nt])) * 0.69314718055994531f;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int row = rt.begin + 16 * nt + r16;
+            if (row >= rt.end) continue;
+            const int i_tok = row / a.group, head = h * a.group + row % a.group;
+            uint16_t* const p = a.out.p + (q0 + i_tok) * a.out.token_stride + head * a.out.head_stride;
+            const float inv = sum[nt] != 0.0f ? 1.0f / sum[nt] : 0.0f;
+            // Channels [g dim/4, (g+1) dim/4) in order: unit 4 g + i, tile c.
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+                u32x4 v;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int ch = 8 * x + 2 * y;
+                    typename E::V2 e;
+                    e[0] = static_cast<typename E::T>(o[nt][ch % kUnit][ch / kUnit] * inv);
+                    e[1] = static_cast<typename E::T>(o[nt][(ch + 1) % kUnit][ch / kUnit] * inv);
+                    v[y] = __builtin_bit_cast(uint32_t, e);
+                }
+                store8(p + (D / 4) * g4 + 8 * x, v, a.out.wide);
+            }
+            if (a.lse != nullptr && g4 == 0)
+                a.lse[static_cast<int64_t>(q0 + i_tok) * t.kv_heads * a.group + head] =
+                    (m[nt] + __builtin_log2f(sum[nt])) * 0.69314718055994531f;
+        }
+    }
+}
+
+// Joins the splits' partial results of one row: one wave a row, dim / 64
+// channels a lane.
+template <class E, int D, int NT>
+__global__ __launch_bounds__(64) void kv_join_kernel(AttendArgs a)
+{
+    constexpr int kRows = 16 * NT;
+    constexpr int kC = D / 64;
+    const Batch& t = a.batch;
+    const int lane = threadIdx.x;
+    const int h = blockIdx.x % t.kv_heads;
+    const int r = blockIdx.x / t.kv_heads;
+    const int index = blockIdx.y, b = blockIdx.z;
+    const int len = t.length(b);
+    const int q0 = t.first_query(b);
+    const int n = t.new_tokens(b, q0);
+    const RowTile rt = row_tile(a, index, kRows, len, n);
+    const int row = rt.begin + r;
+    if (row >= rt.end) return;
+    const int tiles = tiles_of(a, rt);
+    int splits = (tiles + a.split_tiles - 1) / a.split_tiles;
+    splits = splits < 1 ? 1 : splits;
+    const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
+    const float* const ml = a.part_ml + (item * a.splits * kRows + r) * 2;
+    const float* const po = a.part_o + (item * a.splits * kRows + r) * D + lane * kC;
+    float top = -__builtin_inff();
+    for (int s = lane; s < splits; s += 64) top = fmaxf(top, ml[static_cast<int64_t>(s) * kRows * 2]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float keep = top == -__builtin_inff() ? 0.0f : top;
+    float acc[kC] = {};
+    float sum = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+        const float f = __builtin_amdgcn_exp2f(ml[static_cast<int64_t>(s) * kRows * 2] - keep);
+        sum += f * ml[static_cast<int64_t>(s) * kRows * 2 + 1];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) acc[c] += f * po[static_cast<int64_t>(s) * kRows * D + c];
+    }
+    const int i_tok = row / a.group, head = h * a.group + row % a.group;
+    uint16_t* const p = a.out.p + (q0 + i_tok) * a.out.token_stride + head * a.out.head_stride;
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+        p[lane * kC + c] = __builtin_bit_cast(uint16_t, static_cast<typename E::T>(acc[c] * inv));
+    if (a.lse != nullptr && lane == 0)
+        a.lse[static_cast<int64_t>(q0 + i_tok) * t.kv_heads * a.group + head] =
+            (top + __builtin_log2f(sum)) * 0.69314718055994531f;
+}
+
+// How a call is cut up, chosen on the host.
+struct AttendPlan {
+    int nt;      // 16-row tiles a wave holds
+    int wt;      // waves that share a row tile's positions (4), or 1: a row tile each
+    dim3 grid, join;
+};
+
+// One launch each; defined per element type and dim.
+template <class E, int D>
+void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
+{
+    if (p.wt == 1) {
+        if constexpr (D == 256)
+            kv_attention_kernel<E, D, 2, 1><<<p.grid, 256, 0, stream>>>(a);
+        else
+            kv_attention_kernel<E, D, 4, 1><<<p.grid, 256, 0, stream>>>(a);
+        return;
+    }
+    if (p.nt == 1)
+        kv_attention_kernel<E, D, 1, 4><<<p.grid, 256, 0, stream>>>(a);
+    else
+        kv_attention_kernel<E, D, 2, 4><<<p.grid, 256, 0, stream>>>(a);
+    if (a.splits > 1) {
+        if (p.nt == 1)
+            kv_join_kernel<E, D, 1><<<p.join, 64, 0, stream>>>(a);
+        else
+            kv_join_kernel<E, D, 2><<<p.join, 64, 0, stream>>>(a);
+    }
+}
+
+extern template void attend_launch<Bf16, 64>(const AttendArgs&, const AttendPlan&, hipStream_t);
+extern template void attend_launch<Bf16, 128>(const AttendArgs&, const AttendPlan&, hipStream_t);
+extern template void attend_launch<Bf16, 256>(const AttendArgs&, const AttendPlan&, hipStream_t);
+extern template void attend_launch<F16, 64>(const AttendArgs&, const AttendPlan&, hipStream_t);
+extern template void attend_launch<F16, 128>(const AttendArgs&, const AttendPlan&, hipStream_t);
+extern template void attend_launch<F16, 256>(const AttendArgs&, const AttendPlan&, hipStream_t);
+
+}  // namespace kv
+}  // namespace gofann

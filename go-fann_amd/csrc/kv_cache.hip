@@ -1,0 +1,87 @@
+// kv_cache.hip -- host side of the attention over the 4-bit key/value cache:
+// how a call is cut into row tiles and splits, and its launches.
+#include "kv_attention.hpp"
+
+namespace gofann {
+
+int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                 const gofann_kv_rows* q, uint32_t heads, float scale, const int32_t* blocks,
+                 uint32_t width, const gofann_kv_rows* out, float* out_lse)
+{
+    using namespace kv;
+    AttendArgs a{};
+    a.batch = batch_of(cache, batch);
+    a.q = rows_of(q);
+    a.out = rows_of(out);
+    a.k_codes = cache->k_codes;
+    a.k_scales = cache->k_scales;
+    a.v_codes = cache->v_codes;
+    a.v_scales = cache->v_scales;
+    a.blocks = blocks;
+    a.lse = out_lse;
+    a.scale_log2 = scale * 1.44269504088896341f;
+    a.group = static_cast<int>(heads / cache->kv_heads);
+    a.width = static_cast<int>(width);
+    const uint32_t dim = cache->dim;
+    const uint32_t tokens = batch->query_offsets == nullptr ? 1 : batch->max_queries;
+    const uint64_t rows = blocks != nullptr ? static_cast<uint64_t>(a.group)
+                                            : static_cast<uint64_t>(tokens) * a.group;
+    const uint32_t most_tiles =
+        blocks != nullptr ? width * (cache->page_size / kTile)
+                          : (static_cast<uint32_t>(a.batch.max_positions) + kTile - 1) / kTile;
+    AttendPlan p{};
+    const int wide_rows = dim == 256 ? 32 : 64;  // rows of a wave where a row tile has one wave
+    const uint64_t wide_items = (rows + 4 * wide_rows - 1) / (4 * wide_rows) * cache->kv_heads *
+                                batch->sequences;
+    if (blocks == nullptr && wide_items >= static_cast<uint64_t>(ctx->compute_units)) {
+        p.wt = 1;
+        p.nt = wide_rows / 16;
+        a.splits = 1;
+        a.split_tiles = static_cast<int>(most_tiles);
+        a.row_tiles = static_cast<int>((rows + 4 * wide_rows - 1) / (4 * wide_rows));
+        p.grid = dim3(cache->kv_heads, static_cast<uint32_t>(a.row_tiles), batch->sequences);
+    } else {
+        p.wt = 4;
+        p.nt = rows <= 16 ? 1 : 2;
+        const uint32_t per = 16 * p.nt;
+        a.token_tiles = static_cast<int>((a.group + per - 1) / per);
+        a.row_tiles = static_cast<int>(blocks != nullptr
+                                           ? static_cast<uint64_t>(tokens) * a.token_tiles
+                                           : (rows + per - 1) / per);
+        // Splits: enough workgroups to fill the chip, of at least two tiles a wave.
+        const uint64_t items = static_cast<uint64_t>(a.row_tiles) * cache->kv_heads * batch->sequences;
+        const uint64_t aim = 3ull * static_cast<uint64_t>(ctx->compute_units);
+        uint64_t splits = (aim + items - 1) / items;
+        const uint64_t cap = most_tiles / 8 > 1 ? most_tiles / 8 : 1;
+        if (splits > cap) splits = cap;
+        if (splits < 1) splits = 1;
+        uint32_t per_split = static_cast<uint32_t>((most_tiles + splits - 1) / splits);
+        if (per_split < 1) per_split = 1;
+        a.split_tiles = static_cast<int>(per_split);
+        a.splits = most_tiles > 0 ? static_cast<int>((most_tiles + per_split - 1) / per_split) : 1;
+        if (a.splits > 1) {
+            const uint64_t parts = items * static_cast<uint64_t>(a.splits) * per;
+            const size_t o_bytes = parts * dim * sizeof(float);
+            char* const w = static_cast<char*>(
+                ctx->workspace(Context::kScratchKv, o_bytes + parts * 2 * sizeof(float)));
+            if (w == nullptr) return GOFANN_ERR_NOMEM;
+            a.part_o = reinterpret_cast<float*>(w);
+            a.part_ml = reinterpret_cast<float*>(w + o_bytes);
+        }
+        p.grid = dim3(cache->kv_heads * static_cast<uint32_t>(a.splits),
+                      static_cast<uint32_t>(a.row_tiles), batch->sequences);
+        p.join = dim3(cache->kv_heads * per, static_cast<uint32_t>(a.row_tiles), batch->sequences);
+    }
+    if (a.row_tiles > 65535)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, "kv_attention: too many tokens a sequence for one call");
+    const bool bf = cache->elem == GOFANN_ELEM_BF16;
+    switch (dim) {
+        case 64: (bf ? attend_launch<Bf16, 64> : attend_launch<F16, 64>)(a, p, ctx->stream); break;
+        case 128: (bf ? attend_launch<Bf16, 128> : attend_launch<F16, 128>)(a, p, ctx->stream); break;
+        default: (bf ? attend_launch<Bf16, 256> : attend_launch<F16, 256>)(a, p, ctx->stream); break;
+    }
+    if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_attention: launch");
+    return GOFANN_OK;
+}
+
+}  // namespace gofann

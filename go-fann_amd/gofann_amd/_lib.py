@@ -18,7 +18,7 @@ LIB_PATH = Path(os.environ.get("GOFANN_HIP_LIB", str(_HERE.parent / "libgofann_h
 GOFANN_OK = 0
 OK, ERR_INVALID, ERR_HIP, ERR_UNSUPPORTED, ERR_NOMEM = 0, -1, -2, -3, -4
 EARLY_STOP_FIXED, EARLY_STOP_OFF, EARLY_STOP_ADAPTIVE = 0, 1, 2
-ELEM_U8, ELEM_F32, ELEM_F16 = 0, 1, 2
+ELEM_U8, ELEM_F32, ELEM_F16, ELEM_BF16 = 0, 1, 2, 3
 EXACT_ORDER_SERIAL, EXACT_ORDER_WARP = 0, 1
 PLACE_AUTO, PLACE_LDS, PLACE_GLOBAL, PLACE_SPILL = 0, 1, 2, 3
 
@@ -125,6 +125,22 @@ class BuildLinkInputs(C.Structure):
 class BuildLinkParams(C.Structure):
     _fields_ = [("degree", U32), ("local", U32), ("near_links", U32), ("rep_local", U32),
                 ("rep_near", U32), ("entry_row", U32), ("seed", U64)]
+
+
+class KvCacheView(C.Structure):
+    _fields_ = [(n, P) for n in ("k_codes", "k_scales", "v_codes", "v_scales", "box",
+                                 "box_scale")] + [
+        ("pages", U32), ("kv_heads", U32), ("page_size", U32), ("dim", U32), ("elem", C.c_int)]
+
+
+class KvBatchView(C.Structure):
+    _fields_ = [(n, P) for n in ("page_table", "lengths", "query_offsets", "visible")] + [
+        (n, U32) for n in ("sequences", "table_width", "table_stride", "visible_stride",
+                           "queries", "max_queries", "max_length")]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("data", P), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
 class GraphFileHeader(C.Structure):
@@ -271,6 +287,14 @@ SIGNATURES = {
                                      P]),
     "gofann_build_cagra_optimize": (C.c_int, [P, P, U32, U32, U32, P, P]),
     "gofann_build_reach": (C.c_int, [P, P, U32, U32, U32, P, C.POINTER(U32)]),
+    "gofann_kv_append": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView),
+                                   C.POINTER(KvRows), C.POINTER(KvRows), C.POINTER(KvRows),
+                                   C.POINTER(KvRows)]),
+    "gofann_kv_select": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView),
+                                   C.POINTER(KvRows), U32, U32, U32, U32, P]),
+    "gofann_kv_attention": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView),
+                                      C.POINTER(KvRows), U32, C.c_float, P, U32,
+                                      C.POINTER(KvRows), P]),
 }
 
 _lib = None
@@ -320,6 +344,7 @@ class Context:
 
     def bind_stream(self, stream) -> None:
         self.check(self.lib.gofann_set_stream(self.handle, P(stream.cuda_stream)))
+        self.stream = stream.cuda_stream
 
     def check(self, rc: int) -> None:
         if rc != GOFANN_OK:

@@ -51,6 +51,7 @@ extern "C" {
 #define GOFANN_ELEM_U8 0
 #define GOFANN_ELEM_F32 1
 #define GOFANN_ELEM_F16 2
+#define GOFANN_ELEM_BF16 3 /* key/value cache calls only */
 
 #define GOFANN_PLACE_AUTO 0
 #define GOFANN_PLACE_LDS 1
@@ -945,6 +946,100 @@ int gofann_build_cagra_optimize(gofann_ctx* ctx, const uint32_t* knn, uint32_t n
  * guarantee_connectivity (graph_builder.cu:1295). */
 int gofann_build_reach(gofann_ctx* ctx, const uint32_t* graph, uint32_t n, uint32_t degree,
                        uint32_t entry_row, uint32_t* reached, uint32_t* reached_count);
+
+/* ---- 4-bit key/value cache (no counterpart in the reference) --------------
+ * The keys and values of one attention layer, searched by its queries as an
+ * index is: few-bit codes, a cheap integer score that picks blocks of them,
+ * a filter in bits evaluated before any product, and exact work on what is
+ * left.  The cache is paged; a page holds page_size positions of one
+ * sequence, for every key/value head.  All arrays are the caller's.
+ *
+ * A row of `dim` channels is held in groups of 32: group exponent e = the
+ * least with max|x| <= 6 * 2^e, clamped to [-125, 125] (BF16) or [-23, 13]
+ * (F16); code = the nearest of {0, .5, 1, 1.5, 2, 3, 4, 6} to |x| / 2^e,
+ * halfway to the even code, in bits 2:0, the sign of x in bit 3.  A NaN is
+ * held as zero, an infinity (left out of max|x|) as the group's largest. */
+typedef struct {
+    uint8_t* k_codes;  /* [pages][kv_heads][page_size][dim/2], low nibble: even channel */
+    uint8_t* k_scales; /* [pages][kv_heads][page_size][dim/32], e + 127 */
+    uint8_t* v_codes;  /* [pages][kv_heads][page_size/8][16][8][dim/32]: unit u of 16 holds
+                          channels [u dim/16, (u+1) dim/16) of eight tokens in turn */
+    uint8_t* v_scales; /* [pages][kv_heads][page_size/8][dim/32][8] */
+    /* Box of a page's keys, for gofann_kv_select (both NULL: none): the most
+     * and the least of every channel over the page's positions, rounded
+     * outwards to whole multiples of 2^(box_scale - 127), the least power of
+     * two with all of them within [-127, 127]. */
+    int8_t* box;        /* [pages][kv_heads][2][dim] */
+    uint8_t* box_scale; /* [pages][kv_heads] */
+    uint32_t pages;
+    uint32_t kv_heads;
+    uint32_t page_size; /* 32, 64, 128 or 256 */
+    uint32_t dim;       /* 64, 128 or 256 */
+    int elem;           /* GOFANN_ELEM_BF16 or GOFANN_ELEM_F16: of every row below */
+} gofann_kv_cache;
+
+/* The sequences of one call.  Sequence b holds lengths[b] positions, the last
+ * query_offsets[b+1] - query_offsets[b] of which are this call's tokens (rows
+ * query_offsets[b] ..).  A page id outside [0, pages) is a hole: its
+ * positions are neither written nor read. */
+typedef struct {
+    const int32_t* page_table;    /* [sequences][table_stride], table_width used */
+    const int32_t* lengths;       /* [sequences] */
+    const int32_t* query_offsets; /* [sequences + 1]; NULL: one token each */
+    const uint32_t* visible;      /* [sequences][visible_stride] bits, bit t % 32 of word t / 32:
+                                     position t may be attended to; NULL: all.  Positions
+                                     past the words may not. */
+    uint32_t sequences;
+    uint32_t table_width;
+    uint32_t table_stride;
+    uint32_t visible_stride;
+    uint32_t queries;     /* rows of the call in all */
+    uint32_t max_queries; /* at least the tokens of any sequence */
+    uint32_t max_length;  /* at least any length; only so many positions are read */
+} gofann_kv_batch;
+
+/* Rows [token][head][dim] of the cache's element type; strides in elements,
+ * channels contiguous. */
+typedef struct {
+    void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+} gofann_kv_rows;
+
+/* Quantizes the tokens' keys and values [queries][kv_heads][dim] into their
+ * pages and renews the box of every page they fall in.  k_held, v_held
+ * (optional): the values that the cache then holds. */
+int gofann_kv_append(gofann_ctx* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                     const gofann_kv_rows* k, const gofann_kv_rows* v,
+                     const gofann_kv_rows* k_held, const gofann_kv_rows* v_held);
+
+/* Blocks (indexes into a sequence's page table) to be read for each token and
+ * key/value head: out_blocks [queries][kv_heads][width], ascending, -1 past
+ * the last.  Candidates are the blocks with a visible position up to the
+ * token's own.  The first `first` and the last `last` blocks up to the
+ * token's come first, then those of the highest score, ties to the lowest
+ * block, up to `width` in all (width >= first + last).
+ *   score = max over the heads h of the group of
+ *           (sum_c max(q8[h][c] * most[c], q8[h][c] * least[c])) * 2^(eq[h] + eb)
+ * with eq[h] = x - 7 for 2^(x-1) <= max|q[h]| < 2^x, clamped to [-125, 125],
+ * q8 = q / 2^eq rounded to nearest even and clamped to [-127, 127] (NaN: 0;
+ * infinities left out of the maximum): whole numbers, so no order of
+ * summation changes the choice. */
+int gofann_kv_select(gofann_ctx* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                     const gofann_kv_rows* q, uint32_t heads, uint32_t width, uint32_t first,
+                     uint32_t last, int32_t* out_blocks);
+
+/* out [queries][heads][dim] = softmax(scale * q . k) v over the positions up
+ * to the token's own whose filter bit is set, and with `blocks`
+ * [queries][kv_heads][width] only those in the listed blocks (distinct, in
+ * any order; negative: none).  Head h reads key/value head
+ * h / (heads / kv_heads).  A row with no position left gives zeros.
+ * out_lse (optional) [queries][heads]: the natural log of the sum of
+ * exponentials, -inf for such a row. */
+int gofann_kv_attention(gofann_ctx* ctx, const gofann_kv_cache* cache,
+                        const gofann_kv_batch* batch, const gofann_kv_rows* q, uint32_t heads,
+                        float scale, const int32_t* blocks, uint32_t width,
+                        const gofann_kv_rows* out, float* out_lse);
 
 #ifdef __cplusplus
 }
