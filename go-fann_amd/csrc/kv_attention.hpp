@@ -88,7 +88,7 @@ struct Raw {
 // The 4-bit codes become 16-bit elements by the hardware's conversion, which
 // applies the group's power of two; both are exact.
 template <class E, int D, int NT, int WT>
-__global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttendArgs a)
 {
     using V8 = typename E::V8;
     constexpr int kRows = 16 * NT;
@@ -148,11 +148,13 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
         sum[nt] = 0.0f;
     }
 
-    const auto load = [&](uint32_t at, Raw<D>& x) {
+    // Keys and values of tile `at`, loaded apart: a tile's keys are requested
+    // once the last tile's scores are formed, its values once the last tile's
+    // product is, each into the registers just freed.
+    Raw<D> x;
+    const auto load_keys = [&](uint32_t at) {
         const uint8_t* const kc = a.k_codes + static_cast<uint64_t>(at) * (16 * D);
         const uint8_t* const ks = a.k_scales + static_cast<uint64_t>(at) * D;
-        const uint8_t* const vc = a.v_codes + static_cast<uint64_t>(at) * (16 * D);
-        const uint8_t* const vs = a.v_scales + static_cast<uint64_t>(at) * D;
         const uint32_t pos = 8 * (r16 / 4) + r16 % 4;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -172,6 +174,10 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
                 }
             }
         }
+    };
+    const auto load_values = [&](uint32_t at) {
+        const uint8_t* const vc = a.v_codes + static_cast<uint64_t>(at) * (16 * D);
+        const uint8_t* const vs = a.v_scales + static_cast<uint64_t>(at) * D;
         const uint8_t* const vp = vc + (g4 * 16 + r16) * (D / 4);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
@@ -184,9 +190,8 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
         x.vs[1] = s[1];
     };
 
-    const auto compute = [&](const Raw<D>& x, int t0, uint32_t word) {
-        // Scores.
-        f32x4 s[NT][2];
+    f32x4 s[NT][2];
+    const auto scores = [&]() {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -202,33 +207,9 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
                 for (int nt = 0; nt < NT; ++nt) s[nt][half] = E::mfma(k8, q[nt][j], s[nt][half]);
             }
         }
-        uint32_t scale[8];  // of the eight positions' values, in bits 30:23
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            scale[4 * w] = x.vs[w] << 23;
-            scale[4 * w + 1] = x.vs[w] << 15;
-            scale[4 * w + 2] = x.vs[w] << 7;
-            scale[4 * w + 3] = x.vs[w] >> 1;
-        }
-        const bool masked = word != 0xFFFFFFFFu || t0 + kTile > all_see;
-        if (masked) {
-            const uint32_t mine = word >> (8 * g4);
-            // A position that no row sees may hold anything: its scale must
-            // not turn a weight of zero into a NaN.
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!(mine >> e & 1u)) scale[e] = 127u << 23;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                int left = limit[nt] - t0 - 8 * g4;
-                left = left < 0 ? 0 : left > 8 ? 8 : left;
-                const uint32_t ok = mine & ((1u << left) - 1u);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    s[nt][e / 4][e % 4] = (ok >> e & 1u) ? s[nt][e / 4][e % 4] : -__builtin_inff();
-            }
-        }
-        V8 p[NT];
+    };
+    V8 p[NT];
+    const auto weights = [&]() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             // The running maximum is renewed only where a score passes it by
@@ -261,8 +242,20 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[nt][e] = static_cast<typename E::T>(w[e]);
         }
-        // Values: two positions' bytes to pairs of channels, then to pairs of
-        // positions a channel.
+    };
+    uint32_t scale[8];  // of the eight positions' values, in bits 30:23
+    const auto value_scales = [&]() {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            scale[4 * w] = x.vs[w] << 23;
+            scale[4 * w + 1] = x.vs[w] << 15;
+            scale[4 * w + 2] = x.vs[w] << 7;
+            scale[4 * w + 3] = x.vs[w] >> 1;
+        }
+    };
+    // Two positions' bytes to pairs of channels, then to pairs of positions a
+    // channel.
+    const auto product = [&]() {
         each<kUnit / 2>([&](auto pair) {
             constexpr int c = decltype(pair)::value;  // channels 2 c, 2 c + 1 of the unit
             uint32_t d[8];
@@ -311,24 +304,51 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttendArgs a)
                 }
             }
         }
-        uint64_t live = __ballot(word != 0);
-        if (live == 0) continue;
-        Raw<D> cur, next;
-        int i = __builtin_ctzll(live);
-        live &= live - 1;
-        load(__builtin_amdgcn_readlane(at, i), cur);
-        while (true) {
-            const int now = i;
-            if (live != 0) {
-                i = __builtin_ctzll(live);
-                live &= live - 1;
-                load(__builtin_amdgcn_readlane(at, i), next);
-            } else {
-                i = -1;
+        // Tiles that every row sees whole, then the others.
+        uint64_t whole = __ballot(word == 0xFFFFFFFFu && t0 + kTile <= all_see);
+        uint64_t part = __ballot(word != 0) & ~whole;
+        if (whole != 0) {
+            uint32_t now = __builtin_amdgcn_readlane(at, __builtin_ctzll(whole));
+            load_keys(now);
+            load_values(now);
+            while (true) {
+                whole &= whole - 1;
+                const bool more = whole != 0;
+                if (more) now = __builtin_amdgcn_readlane(at, __builtin_ctzll(whole));
+                scores();
+                if (more) load_keys(now);
+                weights();
+                value_scales();
+                product();
+                if (!more) break;
+                load_values(now);
             }
-            compute(cur, __builtin_amdgcn_readlane(t0, now), __builtin_amdgcn_readlane(word, now));
-            if (i < 0) break;
-            cur = next;
+        }
+        for (; part != 0; part &= part - 1) {
+            const int i = __builtin_ctzll(part);
+            const uint32_t now = __builtin_amdgcn_readlane(at, i);
+            load_keys(now);
+            load_values(now);
+            const int from = __builtin_amdgcn_readlane(t0, i) + 8 * g4;
+            const uint32_t mine = static_cast<uint32_t>(__builtin_amdgcn_readlane(word, i)) >> (8 * g4);
+            scores();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                int left = limit[nt] - from;
+                left = left < 0 ? 0 : left > 8 ? 8 : left;
+                const uint32_t ok = mine & ((1u << left) - 1u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    s[nt][e / 4][e % 4] = (ok >> e & 1u) ? s[nt][e / 4][e % 4] : -__builtin_inff();
+            }
+            weights();
+            // A position that no row sees may hold anything: its scale must
+            // not turn a weight of zero into a NaN.
+            value_scales();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(mine >> e & 1u)) scale[e] = 127u << 23;
+            product();
         }
     }
 
@@ -503,15 +523,16 @@ struct AttendPlan {
     dim3 grid, join;
 };
 
+// 16-row tiles of a wave that has a row tile to itself.
+template <int D>
+constexpr int kWideTiles = D == 256 ? 1 : 2;
+
 // One launch each; defined per element type and dim.
 template <class E, int D>
 void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
 {
     if (p.wt == 1) {
-        if constexpr (D == 256)
-            kv_attention_kernel<E, D, 2, 1><<<p.grid, 256, 0, stream>>>(a);
-        else
-            kv_attention_kernel<E, D, 4, 1><<<p.grid, 256, 0, stream>>>(a);
+        kv_attention_kernel<E, D, kWideTiles<D>, 1><<<p.grid, 256, 0, stream>>>(a);
         return;
     }
     if (p.nt == 1)

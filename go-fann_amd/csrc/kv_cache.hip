@@ -30,10 +30,10 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         blocks != nullptr ? width * (cache->page_size / kTile)
                           : (static_cast<uint32_t>(a.batch.max_positions) + kTile - 1) / kTile;
     AttendPlan p{};
-    const int wide_rows = dim == 256 ? 32 : 64;  // rows of a wave where a row tile has one wave
+    const int wide_rows = 16 * (dim == 256 ? kWideTiles<256> : kWideTiles<128>);
     const uint64_t wide_items = (rows + 4 * wide_rows - 1) / (4 * wide_rows) * cache->kv_heads *
                                 batch->sequences;
-    if (blocks == nullptr && wide_items >= static_cast<uint64_t>(ctx->compute_units)) {
+    if (blocks == nullptr && rows > 64 && wide_items >= static_cast<uint64_t>(ctx->compute_units)) {
         p.wt = 1;
         p.nt = wide_rows / 16;
         a.splits = 1;
