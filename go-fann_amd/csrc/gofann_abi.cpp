@@ -93,6 +93,22 @@ void* Context::workspace(int slot, size_t bytes)
     return p;
 }
 
+void* Context::zeroed(int slot, size_t bytes)
+{
+    const void* const old = scratch_ptr[slot];
+    void* const p = workspace(slot, bytes);
+    // A buffer that has just grown: the stream is not captured then.
+    if (p != nullptr && p != old && hipMemsetAsync(p, 0, scratch_bytes[slot], stream) != hipSuccess) {
+        (void)hipGetLastError();
+        error = "workspace: clearing failed";
+        retired.push_back(p);
+        scratch_ptr[slot] = nullptr;
+        scratch_bytes[slot] = 0;
+        return nullptr;
+    }
+    return p;
+}
+
 void Context::release(int slot)
 {
     if (scratch_ptr[slot] == nullptr || hipStreamSynchronize(stream) != hipSuccess) return;

@@ -26,7 +26,8 @@ struct Context {
         kScratchLog = 5,    // admission logs of the set frontier
         kScratchScan = 6,   // the exact posting scan's lists per part before the merge
         kScratchKv = 7,     // key/value cache calls: block keys, partial outputs (workspace())
-        kScratchCount = 8
+        kScratchKvArrived = 8,  // its splits' arrival counters (zeroed())
+        kScratchCount = 9
     };
 
     int device = 0;
@@ -69,6 +70,8 @@ struct Context {
     // reason in `error`, on failure and where the stream is captured and the
     // buffer too small.
     void* workspace(int slot, size_t bytes);
+    // The same, zero when it is first handed out; its users leave it zero.
+    void* zeroed(int slot, size_t bytes);
     std::vector<void*> retired;
     // Frees `slot`'s buffer, once the stream is done with it.
     void release(int slot);

@@ -18,6 +18,7 @@ struct AttendArgs {
     float* lse;             // [queries][heads] or NULL
     float* part_o;          // [item][split][rows][dim], splits > 1
     float* part_ml;         // [item][split][rows][2]: running maximum, sum
+    uint32_t* arrived;      // [item], zero between calls: splits done; NULL: kv_join_kernel joins
     float scale_log2;       // scale * log2(e)
     int group;              // heads a key/value head
     int width;
@@ -54,12 +55,61 @@ __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int 
     return t;
 }
 
+// Splits up to which the last workgroup of an item to finish joins them
+// itself; past it the partial results are too many for one workgroup.
+constexpr int kJoinSplits = 16;
+
+// Partial results go between workgroups of one launch as accesses of device
+// scope, eight bytes at a time.
+__device__ __forceinline__ void put2(float* p, float x, float y)
+{
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, float2{x, y}),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p)
+{
+    return __builtin_bit_cast(
+        float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                  __HIP_MEMORY_SCOPE_AGENT));
+}
+
 // Tiles of 32 positions that a row tile reads.
 __device__ __forceinline__ int tiles_of(const AttendArgs& a, const RowTile& t)
 {
     if (t.end <= t.begin || t.last_pos < 0) return 0;
     if (a.blocks != nullptr) return a.width << (a.batch.page_shift - 5);
     return (t.last_pos >> 5) + 1;
+}
+
+// Four channels of a row's output, from the weighted values and the weights'
+// sum in units of 2^top.
+template <class E>
+__device__ __forceinline__ void finish(const AttendArgs& a, const Batch& t, int q0, int h, int row,
+                                       int ch, f32x4 acc, float top, float total)
+{
+    const int token = q0 + row / a.group, head = h * a.group + row % a.group;
+    uint16_t* const to = a.out.p + token * a.out.token_stride + head * a.out.head_stride + ch;
+    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+    typename E::V2 lo, hi;
+    lo[0] = static_cast<typename E::T>(acc[0] * inv);
+    lo[1] = static_cast<typename E::T>(acc[1] * inv);
+    hi[0] = static_cast<typename E::T>(acc[2] * inv);
+    hi[1] = static_cast<typename E::T>(acc[3] * inv);
+    u32x2 v{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    // One rounding for both ways of storing: moved into the branches, one of
+    // them would become a product and conversion in a single instruction.
+    asm("" : "+v"(v));
+    if (a.out.wide) {
+        *reinterpret_cast<u32x2*>(to) = v;
+    } else {
+        to[0] = static_cast<uint16_t>(v[0]);
+        to[1] = static_cast<uint16_t>(v[0] >> 16);
+        to[2] = static_cast<uint16_t>(v[1]);
+        to[3] = static_cast<uint16_t>(v[1] >> 16);
+    }
+    if (a.lse != nullptr && ch == 0)
+        a.lse[static_cast<int64_t>(token) * t.kv_heads * a.group + head] =
+            (top + __builtin_log2f(total)) * 0.69314718055994531f;
 }
 
 // What a lane loads of one tile: keys of two positions, values of eight.
@@ -359,85 +409,107 @@ __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttendArgs a)
     }
 
     if constexpr (WT > 1) {
-        // The four waves' maxima, sums and outputs joined; wave w then holds
-        // the output of O tiles [w kUnit/4, (w+1) kUnit/4).
-        constexpr int kQ = kUnit / 4;
+        // The four waves' maxima, sums and outputs joined through LDS, sixteen
+        // rows at a time: thread x then has four channels of row x / (D / 4)
+        // and of every 256 / (D / 4)-th after it.
+        constexpr int kLanes = D / 4, kStep = 256 / kLanes;
+        constexpr int kPad = D + 4;  // rows start on other banks
         __shared__ float wm[4][kRows], ws[4][kRows];
-        __shared__ f32x4 wo[3][NT][kQ][64];
+        __shared__ __attribute__((aligned(16))) float wo[4][16][kPad];
+        const int active = (tiles + a.split_tiles - 1) / a.split_tiles;
+        const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
+        float* const po = a.part_o + item * a.splits * kRows * D;
+        float* const pm = a.part_ml + item * a.splits * kRows * 2;
+        const int my_ch = 4 * (threadIdx.x % kLanes);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
             if (g4 == 0) {
                 wm[wave][16 * nt + r16] = m[nt];
                 ws[wave][16 * nt + r16] = sum[nt];
             }
-        __syncthreads();
-        float factor[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = 16 * nt + r16;
-            float top = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-            const float keep = top == -__builtin_inff() ? 0.0f : top;
-            factor[nt] = __builtin_amdgcn_exp2f(m[nt] - keep);
-            float total = 0.0f;
+            for (int x = 0; x < kUnit; ++x) {
+                // Channels [g dim/4, ..) in order: unit 4 g + i, tile c.
+                f32x4 v;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) total += ws[w][r] * __builtin_amdgcn_exp2f(wm[w][r] - keep);
-            m[nt] = top;
-            sum[nt] = total;
-        }
-        f32x4 mine[NT][kQ];
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-            // The three other waves' shares of wave `part`'s tiles, added in
-            // the order of the waves.
-            if (wave != part) {
-                const int slot = wave < part ? wave : wave - 1;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < kQ; ++c) wo[slot][nt][c][lane] = o[nt][part * kQ + c] * factor[nt];
+                for (int y = 0; y < 4; ++y) v[y] = o[nt][(4 * x + y) % kUnit][(4 * x + y) / kUnit];
+                *reinterpret_cast<f32x4*>(&wo[wave][r16][(D / 4) * g4 + 4 * x]) = v;
             }
             __syncthreads();
-            if (wave == part) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int r = threadIdx.x / kLanes; r < 16; r += kStep) {
+                const int row = rt.begin + 16 * nt + r;
+                if (row >= rt.end) break;
+                float top = wm[0][16 * nt + r];
 #pragma unroll
-                    for (int c = 0; c < kQ; ++c)
-                        mine[nt][c] = o[nt][part * kQ + c] * factor[nt] + wo[0][nt][c][lane] +
-                                      wo[1][nt][c][lane] + wo[2][nt][c][lane];
-            }
-            __syncthreads();
-        }
+                for (int w = 1; w < 4; ++w) top = fmaxf(top, wm[w][16 * nt + r]);
+                const float keep = top == -__builtin_inff() ? 0.0f : top;
+                float total = 0.0f;
+                f32x4 acc{0, 0, 0, 0};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int row = rt.begin + 16 * nt + r16;
-            if (row >= rt.end) continue;
-            // Lane (r, g) holds, of units 4 g + i, the channels [wave kQ, ..).
-            if (a.splits > 1) {
-                const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
-                const int64_t at = (item * a.splits + split) * kRows + 16 * nt + r16;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int c = 0; c < kQ; ++c)
-                        a.part_o[at * D + (4 * g4 + i) * kUnit + wave * kQ + c] = mine[nt][c][i];
-                if (g4 == 0 && wave == 0) {
-                    a.part_ml[2 * at] = m[nt];
-                    a.part_ml[2 * at + 1] = sum[nt];
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(wm[w][16 * nt + r] - keep);
+                    total += f * ws[w][16 * nt + r];
+                    acc += f * *reinterpret_cast<const f32x4*>(&wo[w][r][my_ch]);
                 }
-            } else {
-                const int i_tok = row / a.group, head = h * a.group + row % a.group;
-                uint16_t* const p = a.out.p + (q0 + i_tok) * a.out.token_stride + head * a.out.head_stride;
-                const float inv = sum[nt] != 0.0f ? 1.0f / sum[nt] : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int c = 0; c < kQ; ++c)
-                        p[(4 * g4 + i) * kUnit + wave * kQ + c] = __builtin_bit_cast(
-                            uint16_t, static_cast<typename E::T>(mine[nt][c][i] * inv));
-                if (a.lse != nullptr && g4 == 0 && wave == 0)
-                    a.lse[static_cast<int64_t>(q0 + i_tok) * t.kv_heads * a.group + head] =
-                        (m[nt] + __builtin_log2f(sum[nt])) * 0.69314718055994531f;
+                if (active <= 1) {
+                    finish<E>(a, t, q0, h, row, my_ch, acc, top, total);
+                } else {
+                    const int at = split * kRows + 16 * nt + r;
+                    float* const to = po + static_cast<int64_t>(at) * D + my_ch;
+                    if (a.arrived != nullptr) {
+                        put2(to, acc[0], acc[1]);
+                        put2(to + 2, acc[2], acc[3]);
+                        if (my_ch == 0) put2(pm + 2 * at, top, total);
+                    } else {
+                        *reinterpret_cast<f32x4*>(to) = acc;
+                        if (my_ch == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{top, total};
+                    }
+                }
             }
+            if (nt + 1 < NT) __syncthreads();
+        }
+        if (active <= 1) return;
+        if (a.arrived == nullptr) return;
+        // The workgroup that arrives last joins the splits, in their order
+        // whichever that is.  Every access to the partial results is an atomic
+        // of the whole device (put, get), which no XCD's cache holds back, so
+        // their completion is all that the count has to wait for; a fence of
+        // the device would write back the XCD's cache and take 5 us a call.
+        __shared__ int last;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const uint32_t before =
+                __hip_atomic_fetch_add(a.arrived + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = before + 1 == static_cast<uint32_t>(active);
+            if (last) __hip_atomic_store(a.arrived + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last) return;
+        __shared__ float jm[kJoinSplits][kRows], js[kJoinSplits][kRows];
+        for (int x = threadIdx.x; x < active * kRows; x += 256) {
+            const bool in = rt.begin + x % kRows < rt.end;
+            const float2 v = in ? get2(pm + 2 * x) : float2{0.0f, 0.0f};
+            jm[x / kRows][x % kRows] = v.x;
+            js[x / kRows][x % kRows] = v.y;
+        }
+        __syncthreads();
+        for (int r = threadIdx.x / kLanes; rt.begin + r < rt.end; r += kStep) {
+            float top = -__builtin_inff();
+            for (int w = 0; w < active; ++w) top = fmaxf(top, jm[w][r]);
+            const float keep = top == -__builtin_inff() ? 0.0f : top;
+            float total = 0.0f;
+            f32x4 acc{0, 0, 0, 0};
+#pragma unroll 4
+            for (int w = 0; w < active; ++w) {
+                const float f = __builtin_amdgcn_exp2f(jm[w][r] - keep);
+                total += f * js[w][r];
+                const float* const from = po + (static_cast<int64_t>(w) * kRows + r) * D + my_ch;
+                const float2 lo = get2(from), hi = get2(from + 2);
+                acc += f * f32x4{lo.x, lo.y, hi.x, hi.y};
+            }
+            finish<E>(a, t, q0, h, rt.begin + r, my_ch, acc, top, total);
         }
     } else {
 #pragma unroll
@@ -459,6 +531,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttendArgs a)
                     e[1] = static_cast<typename E::T>(o[nt][(ch + 1) % kUnit][ch / kUnit] * inv);
                     v[y] = __builtin_bit_cast(uint32_t, e);
                 }
+                asm("" : "+v"(v));
                 store8(p + (D / 4) * g4 + 8 * x, v, a.out.wide);
             }
             if (a.lse != nullptr && g4 == 0)
@@ -468,15 +541,17 @@ __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttendArgs a)
     }
 }
 
-// Joins the splits' partial results of one row: one wave a row, dim / 64
-// channels a lane.
+// Joins the splits' partial results of one row: four waves a row, wave w the
+// splits w, w + 4, .., each lane D / 64 channels.
 template <class E, int D, int NT>
-__global__ __launch_bounds__(64) void kv_join_kernel(AttendArgs a)
+__global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
 {
     constexpr int kRows = 16 * NT;
     constexpr int kC = D / 64;
+    __shared__ float wo[4][D], wm[4], ws[4];
     const Batch& t = a.batch;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int h = blockIdx.x % t.kv_heads;
     const int r = blockIdx.x / t.kv_heads;
     const int index = blockIdx.y, b = blockIdx.z;
@@ -486,34 +561,65 @@ __global__ __launch_bounds__(64) void kv_join_kernel(AttendArgs a)
     const RowTile rt = row_tile(a, index, kRows, len, n);
     const int row = rt.begin + r;
     if (row >= rt.end) return;
-    const int tiles = tiles_of(a, rt);
-    int splits = (tiles + a.split_tiles - 1) / a.split_tiles;
-    splits = splits < 1 ? 1 : splits;
+    const int active = (tiles_of(a, rt) + a.split_tiles - 1) / a.split_tiles;
+    if (active <= 1) return;  // written already
     const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
     const float* const ml = a.part_ml + (item * a.splits * kRows + r) * 2;
     const float* const po = a.part_o + (item * a.splits * kRows + r) * D + lane * kC;
-    float top = -__builtin_inff();
-    for (int s = lane; s < splits; s += 64) top = fmaxf(top, ml[static_cast<int64_t>(s) * kRows * 2]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float keep = top == -__builtin_inff() ? 0.0f : top;
+    float top = -__builtin_inff(), total = 0.0f;
     float acc[kC] = {};
-    float sum = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(ml[static_cast<int64_t>(s) * kRows * 2] - keep);
-        sum += f * ml[static_cast<int64_t>(s) * kRows * 2 + 1];
+    for (int base = wave; base < active; base += 256) {
+        // Lane l has split base + 4 l.
+        const int s = base + 4 * lane;
+        const float m = s < active ? ml[static_cast<int64_t>(s) * kRows * 2] : -__builtin_inff();
+        const float z = s < active ? ml[static_cast<int64_t>(s) * kRows * 2 + 1] : 0.0f;
+        float fresh = m;
 #pragma unroll
-        for (int c = 0; c < kC; ++c) acc[c] += f * po[static_cast<int64_t>(s) * kRows * D + c];
+        for (int d = 1; d < 64; d <<= 1) fresh = fmaxf(fresh, __shfl_xor(fresh, d));
+        fresh = fmaxf(fresh, top);
+        const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
+        const float old = __builtin_amdgcn_exp2f(top - keep);
+        top = fresh;
+        const float f = __builtin_amdgcn_exp2f(m - keep);
+        total = total * old + f * z;  // a lane's own splits
+#pragma unroll
+        for (int c = 0; c < kC; ++c) acc[c] *= old;
+        int count = (active - base + 3) / 4;
+        count = count < 64 ? count : 64;
+        for (int k = 0; k < count; ++k) {
+            const float fk = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k));
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+                acc[c] += fk * po[static_cast<int64_t>(base + 4 * k) * kRows * D + c];
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) wo[wave][lane * kC + c] = acc[c];
+    if (lane == 0) {
+        wm[wave] = top;
+        ws[wave] = total;
+    }
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) >= D) return;
+    const float all = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    const float keep = all == -__builtin_inff() ? 0.0f : all;
+    float sum = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(wm[w] - keep);
+        sum += f * ws[w];
+        o += f * wo[w][threadIdx.x];
     }
     const int i_tok = row / a.group, head = h * a.group + row % a.group;
     uint16_t* const p = a.out.p + (q0 + i_tok) * a.out.token_stride + head * a.out.head_stride;
     const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int c = 0; c < kC; ++c)
-        p[lane * kC + c] = __builtin_bit_cast(uint16_t, static_cast<typename E::T>(acc[c] * inv));
-    if (a.lse != nullptr && lane == 0)
+    p[threadIdx.x] = __builtin_bit_cast(uint16_t, static_cast<typename E::T>(o * inv));
+    if (a.lse != nullptr && threadIdx.x == 0)
         a.lse[static_cast<int64_t>(q0 + i_tok) * t.kv_heads * a.group + head] =
-            (top + __builtin_log2f(sum)) * 0.69314718055994531f;
+            (all + __builtin_log2f(sum)) * 0.69314718055994531f;
 }
 
 // How a call is cut up, chosen on the host.
@@ -539,11 +645,11 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
         kv_attention_kernel<E, D, 1, 4><<<p.grid, 256, 0, stream>>>(a);
     else
         kv_attention_kernel<E, D, 2, 4><<<p.grid, 256, 0, stream>>>(a);
-    if (a.splits > 1) {
+    if (a.splits > 1 && a.arrived == nullptr) {
         if (p.nt == 1)
-            kv_join_kernel<E, D, 1><<<p.join, 64, 0, stream>>>(a);
+            kv_join_kernel<E, D, 1><<<p.join, 256, 0, stream>>>(a);
         else
-            kv_join_kernel<E, D, 2><<<p.join, 64, 0, stream>>>(a);
+            kv_join_kernel<E, D, 2><<<p.join, 256, 0, stream>>>(a);
     }
 }
 

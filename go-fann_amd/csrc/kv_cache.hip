@@ -3,6 +3,23 @@
 #include "kv_attention.hpp"
 
 namespace gofann {
+namespace {
+
+// Tiles of a split of `items` row tiles of at most `most` tiles: enough
+// workgroups that all of them are resident at once, at least one tile a wave,
+// and where sequences may differ in length at most 64, so that a long one does
+// not outlast the others.
+int split_tiles(const Context* ctx, uint64_t items, uint64_t most, bool ragged)
+{
+    const uint64_t resident = 3ull * static_cast<uint64_t>(ctx->compute_units);
+    uint64_t n = (items * most + resident - 1) / resident;
+    n = (n + 3) / 4 * 4;
+    if (n < 4) n = 4;
+    if (ragged && n > 64) n = 64;
+    return static_cast<int>(n);
+}
+
+}  // namespace
 
 int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
                  const gofann_kv_rows* q, uint32_t heads, float scale, const int32_t* blocks,
@@ -48,23 +65,19 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         a.row_tiles = static_cast<int>(blocks != nullptr
                                            ? static_cast<uint64_t>(tokens) * a.token_tiles
                                            : (rows + per - 1) / per);
-        // Splits: enough workgroups to fill the chip, of at least two tiles a wave.
         const uint64_t items = static_cast<uint64_t>(a.row_tiles) * cache->kv_heads * batch->sequences;
-        const uint64_t aim = 3ull * static_cast<uint64_t>(ctx->compute_units);
-        uint64_t splits = (aim + items - 1) / items;
-        const uint64_t cap = most_tiles / 8 > 1 ? most_tiles / 8 : 1;
-        if (splits > cap) splits = cap;
-        if (splits < 1) splits = 1;
-        uint32_t per_split = static_cast<uint32_t>((most_tiles + splits - 1) / splits);
-        if (per_split < 1) per_split = 1;
-        a.split_tiles = static_cast<int>(per_split);
-        a.splits = most_tiles > 0 ? static_cast<int>((most_tiles + per_split - 1) / per_split) : 1;
+        a.split_tiles = split_tiles(ctx, items, most_tiles, batch->sequences > 1);
+        a.splits = most_tiles > 0 ? static_cast<int>((most_tiles + a.split_tiles - 1) / a.split_tiles) : 1;
         if (a.splits > 1) {
             const uint64_t parts = items * static_cast<uint64_t>(a.splits) * per;
             const size_t o_bytes = parts * dim * sizeof(float);
             char* const w = static_cast<char*>(
                 ctx->workspace(Context::kScratchKv, o_bytes + parts * 2 * sizeof(float)));
             if (w == nullptr) return GOFANN_ERR_NOMEM;
+            if (a.splits <= kJoinSplits) {
+                a.arrived = static_cast<uint32_t*>(ctx->zeroed(Context::kScratchKvArrived, items * 4));
+                if (a.arrived == nullptr) return GOFANN_ERR_NOMEM;
+            }
             a.part_o = reinterpret_cast<float*>(w);
             a.part_ml = reinterpret_cast<float*>(w + o_bytes);
         }

@@ -28,6 +28,9 @@ import torch
 from . import _lib
 
 _ELEM = {torch.bfloat16: _lib.ELEM_BF16, torch.float16: _lib.ELEM_F16}
+# The handle of torch's current stream, as torch.cuda.current_stream(i).cuda_stream.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda i: torch.cuda.current_stream(i).cuda_stream)
 DIMS = (64, 128, 256)
 PAGE_SIZES = (32, 64, 128, 256)
 
@@ -173,7 +176,7 @@ class KvCache:
     def _ready(self, batch: KvBatch) -> None:
         if batch.device != self.device:
             raise ValueError("the batch is on another device")
-        if torch.cuda.current_stream(self.device).cuda_stream != self.ctx.stream:
+        if _raw_stream(self.device.index or 0) != self.ctx.stream:
             raise _lib.GofannError("the context is bound to another stream than torch's current "
                                    "one: call ctx.bind_stream")
 
@@ -222,8 +225,10 @@ class KvCache:
         rq = self._rows("q", q, batch.queries, None)
         heads = q.shape[1]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ro = self._rows("out", out, batch.queries, heads, True)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            ro = _lib.KvRows(out.data_ptr(), heads * self.dim, self.dim)
+        else:
+            ro = self._rows("out", out, batch.queries, heads, True)
         width = 0
         if blocks is not None:
             if blocks.dim() != 3 or blocks.shape[:2] != (batch.queries, self.kv_heads) or \
