@@ -1,14 +1,15 @@
 // kv_select.hip -- the blocks of the paged 4-bit key/value cache that each
 // token and key/value head reads: integer scores of the queries against the
 // pages' boxes, then the highest `width` of them in ascending order.
+#include "device_common.hpp"
 #include "kv_common.hpp"
 
 namespace gofann {
 namespace kv {
 namespace {
 
-constexpr int kChunkTiles = 16;               // 16-block tiles a workgroup scores
-constexpr int kChunk = 16 * kChunkTiles;      // blocks of them
+constexpr int kChunk = 256;                   // blocks that a workgroup scores: 16 tiles of 16
+constexpr int kBins = 2048;
 constexpr uint32_t kForced = 0xFFFFFFFFu;     // above every score's key
 constexpr uint32_t kIneligible = 0;           // below every score's key
 
@@ -17,17 +18,25 @@ struct SelectArgs {
     Rows q;
     const int8_t* box;
     const uint8_t* box_scale;
-    uint32_t* keys;  // [queries][kv_heads][key_stride]
+    uint32_t* keys;     // [queries][kv_heads][key_stride], where a row has several chunks
     int64_t key_stride;
+    uint32_t* arrived;  // [item], zero between calls: chunks scored
     int32_t* out;
     int group;        // heads a key/value head
     int group_shift;  // log2 of the rows a token's heads take of a 16-row tile
+    int tokens;       // tokens of a tile, a power of two
+    int token_tiles;  // tiles of a sequence
     int head_tiles;   // 16-row tiles of one token's heads, where they are more than 16
     int width, first, last;
 };
 
 // Position of token i of sequence b, and the blocks up to it; none below 0.
 __device__ __forceinline__ int position(int len, int n, int i) { return len - n + i; }
+
+__device__ __forceinline__ int blocks_to(const Batch& t, int pos)
+{
+    return pos < 0 ? 0 : (pos >> t.page_shift) + 1;
+}
 
 // Whether block j (page_size positions) has a visible position up to pos.
 __device__ __forceinline__ bool any_visible(const Batch& t, int b, int j, int pos)
@@ -44,64 +53,293 @@ __device__ __forceinline__ bool any_visible(const Batch& t, int b, int j, int po
     return any != 0;
 }
 
-// Scores.  The rows of an i8 product are a token's heads (each token padded
-// to a power of two of rows by repeating its last head, which changes no
-// maximum), the columns blocks: a lane then holds four heads of one block,
+// Keys pass between workgroups of one launch as accesses of device scope.
+__device__ __forceinline__ void put(uint32_t* p, uint32_t x)
+{
+    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint32_t get(const uint32_t* p)
+{
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x)
+{
+    const auto shifted = [](uint32_t v, auto ctrl, auto rows) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+            0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xF, true));
+    };
+    using std::integral_constant;
+    x += shifted(x, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr 1
+    x += shifted(x, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+    x += shifted(x, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+    x += shifted(x, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+    x += shifted(x, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // lane 15 on
+    x += shifted(x, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // lane 31 on
+    return x;
+}
+
+struct PickShared {
+    __attribute__((aligned(16))) uint32_t hist[kBins];
+    uint32_t part[4][4];
+    uint32_t found[3];
+};
+
+// The `width` highest of a row's keys, their blocks written in ascending
+// order.  The range of the keys is cut into 2048 bins, the bin that the last
+// taken key falls into becomes the range, until the number wanted of it is all
+// of it or one key is left, of which the lowest blocks are taken: two rounds
+// for keys that differ, at most three.  Wave w has the w-th quarter of the
+// blocks, N keys a lane in registers where they all fit.  load(j): the j-th key.
+template <int N, class L>
+__device__ void pick(const SelectArgs& a, PickShared& sh, int blocks, int32_t* out, L&& load)
+{
+    const int tid = threadIdx.x, lane = tid % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int span = (blocks + 255) / 256 * 64;
+    const int begin = wave * span;
+    const int end = begin + span < blocks ? begin + span : blocks;
+    const bool held = span <= 64 * N;
+    uint32_t k[N];
+    const auto fetch = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = from + 64 * i + lane;
+            k[i] = j < end ? load(j) : kIneligible;
+        }
+    };
+    // f(key, block) for every block of the wave, all lanes together.
+    const auto visit = [&](auto&& f) {
+        if (held) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f(k[i], begin + 64 * i + lane);
+        } else {
+            for (int from = begin; from < end; from += 64 * N) {
+                fetch(from);
+#pragma unroll
+                for (int i = 0; i < N; ++i) f(k[i], from + 64 * i + lane);
+            }
+        }
+    };
+    if (held) fetch(begin);
+
+    uint32_t forced = 0, open = 0, least = 0xFFFFFFFFu, most = 0;
+    visit([&](uint32_t key, int) {
+        const bool is_open = key != kForced && key != kIneligible;
+        forced += __popcll(__ballot(key == kForced));
+        open += __popcll(__ballot(is_open));
+        const uint32_t l = is_open ? key : 0xFFFFFFFFu, m = is_open ? key : 0u;
+        least = l < least ? l : least;
+        most = m > most ? m : most;
+    });
+    least = wave_min_u32(least);
+    most = wave_max_u32(most);
+#pragma unroll
+    for (int x = tid; x < kBins / 4; x += 256) reinterpret_cast<u32x4*>(sh.hist)[x] = u32x4{0, 0, 0, 0};
+    if (lane == 0) *reinterpret_cast<u32x4*>(sh.part[wave]) = u32x4{forced, open, least, most};
+    __syncthreads();
+    forced = open = most = 0;
+    least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(sh.part[w]);
+        forced += v[0];
+        open += v[1];
+        least = v[2] < least ? v[2] : least;
+        most = v[3] > most ? v[3] : most;
+    }
+    uint32_t want = static_cast<uint32_t>(a.width) - forced;
+    // Taken: keys above `limit`, and the first `want` that equal it.
+    uint32_t limit;
+    if (open <= want) {
+        limit = 0;
+        want = 0;
+    } else if (want == 0) {
+        limit = kForced - 1;
+    } else {
+        while (true) {
+            limit = least;
+            if (least == most) break;
+            const int bits = 32 - __builtin_clz(most - least);
+            const int shift = bits > 11 ? bits - 11 : 0;
+            visit([&](uint32_t key, int) {
+                if (key >= least && key <= most) atomicAdd(&sh.hist[(key - least) >> shift], 1u);
+            });
+            __syncthreads();
+            // Thread x has eight bins, the highest first; they are cleared for
+            // the next round as they are read.
+            constexpr int kOwn = kBins / 256;
+            const int low = kBins - kOwn * (tid + 1);
+            uint32_t c[kOwn], sum = 0;
+#pragma unroll
+            for (int m = 0; m < kOwn; m += 4) {
+                u32x4* const at = reinterpret_cast<u32x4*>(sh.hist + low + m);
+                const u32x4 v = *at;
+                *at = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    c[m + y] = v[y];
+                    sum += v[y];
+                }
+            }
+            uint32_t upto = wave_scan(sum);
+            if (lane == 63) sh.part[wave][0] = upto;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) upto += sh.part[w][0];
+            uint32_t above = upto - sum;
+            if (above < want && upto >= want) {
+#pragma unroll
+                for (int m = kOwn - 1; m >= 0; --m) {
+                    if (above < want && above + c[m] >= want) {
+                        sh.found[0] = static_cast<uint32_t>(low + m);
+                        sh.found[1] = above;
+                        sh.found[2] = c[m];
+                    }
+                    above += c[m];
+                }
+            }
+            __syncthreads();
+            want -= sh.found[1];
+            least += sh.found[0] << shift;
+            if (sh.found[2] == want) {  // all of the bin
+                limit = least - 1;
+                want = 0;
+                break;
+            }
+            const uint32_t last = least + ((1u << shift) - 1u);
+            most = last < most ? last : most;
+        }
+    }
+    // Every wave writes behind what the waves before it take.
+    uint32_t above = 0, equal = 0;
+    visit([&](uint32_t key, int) {
+        above += __popcll(__ballot(key > limit));
+        equal += __popcll(__ballot(key == limit && key != kIneligible));
+    });
+    __syncthreads();
+    if (lane == 0) *reinterpret_cast<u32x2*>(sh.part[wave]) = u32x2{above, equal};
+    __syncthreads();
+    uint32_t at = 0, seen = 0, total = 0, ties = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(sh.part[w]);
+        if (w < wave) {
+            at += v[0];
+            seen += v[1];
+        }
+        total += v[0];
+        ties += v[1];
+    }
+    total += ties < want ? ties : want;
+    at += seen < want ? seen : want;
+    const uint64_t below = (1ull << lane) - 1ull;
+    visit([&](uint32_t key, int j) {
+        const bool is_tie = key == limit && key != kIneligible;
+        const uint64_t eq = __ballot(is_tie);
+        const uint64_t take = __ballot(key > limit || (is_tie && seen + __popcll(eq & below) < want));
+        if (take >> lane & 1ull) out[at + __popcll(take & below)] = j;
+        at += __popcll(take);
+        seen += __popcll(eq);
+    });
+    for (uint32_t j = total + tid; j < static_cast<uint32_t>(a.width); j += 256) out[j] = -1;
+}
+
+// Scores of 256 blocks for a tile of tokens; the last workgroup of a tile to
+// finish picks.  The rows of an i8 product are a token's heads (each token
+// padded to a power of two of rows by repeating its last head, which changes
+// no maximum), the columns blocks: a lane then holds four heads of one block,
 // and the maximum over a token's heads stays in the lane and its neighbours
 // 16 and 32 lanes away.  sum_c max(q most, q least) is one product of length
 // 2 dim, of the positive part of q with `most` and the negative with `least`.
-template <class E, int D>
-__global__ __launch_bounds__(256) void kv_score_kernel(SelectArgs a)
+// kQuads: a token has at least four rows, so a lane's four are one token's.
+template <class E, int D, bool kQuads>
+__global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(SelectArgs a)
 {
-    constexpr int K = D / 64;  // products of 64 channels
+    constexpr int K = D / 64;               // products of 64 channels
+    constexpr int kBatch = D == 256 ? 2 : 4;  // 16-block tiles requested at once
+    __shared__ uint32_t stage[4 * kChunk];  // the keys of up to four tokens, where one chunk is all
+    __shared__ PickShared sh;
+    __shared__ int is_last;
     const Batch& t = a.batch;
     const int h = blockIdx.x % t.kv_heads;
     const int chunk = blockIdx.x / t.kv_heads;
     const int b = blockIdx.z;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int r16 = lane % 16, g4 = lane / 16;
+    // Pages are looked up beside the sequence's length, which may rule them out.
+    int early[kBatch];
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) early[x] = t.page(b, chunk * kChunk + 16 * (wave + 4 * x) + r16);
     const int len = t.length(b);
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
-    const int rows_shift = a.group_shift;             // rows a token takes: 1 << rows_shift
-    const int tokens = 16 >> rows_shift;
-    const int i0 = blockIdx.y * tokens;
+    const int rows_shift = a.group_shift;  // rows a token takes: 1 << rows_shift
+    const int i0 = blockIdx.y * a.tokens;
     if (i0 >= n) return;
-    const int i_last = (i0 + tokens < n ? i0 + tokens : n) - 1;
-    const int last_pos = position(len, n, i_last);
-    if (last_pos < 0) return;
-    const int blocks = (last_pos >> t.page_shift) + 1;
-    if (chunk * kChunk >= blocks) return;
-
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int r16 = lane % 16, g4 = lane / 16;
+    const int i_end = i0 + a.tokens < n ? i0 + a.tokens : n;
+    const int blocks = blocks_to(t, position(len, n, i_end - 1));
+    const int chunks = (blocks + kChunk - 1) / kChunk;
+    if (chunk > 0 && chunk >= chunks) return;
 
     // Positive and negative part of the quantized queries, 16 channels a lane
     // and product; the rows' powers of two.
-    const auto load_queries = [&](int ht, i32x4 (&pos)[K], i32x4 (&neg)[K], float (&unit)[4]) {
-        const int i = i0 + (r16 >> rows_shift);
+    i32x4 qp[K], qn[K];
+    float unit[4];
+    uint32_t raw[K][8];
+    const auto request_queries = [&](int ht) {
+        int i = i0 + (r16 >> rows_shift);
+        i = i < i_end ? i : i_end - 1;
         int head = 16 * ht + (r16 & ((1 << rows_shift) - 1));
         head = head < a.group ? head : a.group - 1;
-        const int token = i < n ? i : n - 1;
-        const uint16_t* const row = a.q.p + (q0 + token) * a.q.token_stride +
+        const uint16_t* const row = a.q.p + (q0 + i) * a.q.token_stride +
                                     (static_cast<int64_t>(h) * a.group + head) * a.q.head_stride;
-        float x[K][16];
-        float amax = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const u32x4 v = load8(row + 64 * k + 16 * g4 + 8 * half, a.q.wide);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float f = static_cast<float>(
-                        __builtin_bit_cast(typename E::V2, static_cast<uint32_t>(v[j / 2]))[j % 2]);
-                    f = f != f ? 0.0f : f;
-                    const float m = __builtin_fabsf(f);
-                    amax = m > amax && m < __builtin_inff() ? m : amax;
-                    x[k][8 * half + j] = f;
-                }
+                for (int j = 0; j < 4; ++j) raw[k][4 * half + j] = v[j];
             }
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
+    };
+    const auto quantize_queries = [&]() {
+        // Magnitudes compare as the integers of their bits, two to a word.
+        constexpr uint32_t kInf = std::is_same_v<E, Bf16> ? 0x7F80u : 0x7C00u;
+        using U2 = uint16_t __attribute__((ext_vector_type(2)));
+        const auto largest = [&]() {
+            U2 m = {0, 0};
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    m = __builtin_elementwise_max(m, __builtin_bit_cast(U2, raw[k][j] & 0x7FFF7FFFu));
+            uint32_t top = m[0] > m[1] ? m[0] : m[1];
+            uint32_t other = __shfl_xor(top, 16);
+            top = other > top ? other : top;
+            other = __shfl_xor(top, 32);
+            return other > top ? other : top;
+        };
+        uint32_t top = largest();
+        if (__any(top >= kInf)) {
+            // Infinities stay out of the maximum and saturate, a NaN is zero.
+            uint32_t kept[K][8];
+            for (int k = 0; k < K; ++k)
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t w = raw[k][j], fin = w;
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t m = w >> (16 * half) & 0x7FFFu, mask = 0xFFFFu << (16 * half);
+                        if (m > kInf) w &= ~mask;
+                        if (m >= kInf) fin &= ~mask;
+                    }
+                    kept[k][j] = w;
+                    raw[k][j] = fin;
+                }
+            top = largest();
+            for (int k = 0; k < K; ++k)
+                for (int j = 0; j < 8; ++j) raw[k][j] = kept[k][j];
+        }
+        const float amax = static_cast<float>(__builtin_bit_cast(typename E::V2, top)[0]);
         int e = amax > 0.0f ? __builtin_amdgcn_frexp_expf(amax) - 7 : -125;
         e = e < -125 ? -125 : e > 125 ? 125 : e;
         const float inv = __builtin_bit_cast(float, static_cast<uint32_t>(127 - e) << 23);
@@ -109,215 +347,162 @@ __global__ __launch_bounds__(256) void kv_score_kernel(SelectArgs a)
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                uint32_t p = 0, m = 0;
+                uint32_t v[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float f = __builtin_rintf(x[k][4 * w + j] * inv);
-                    f = f > 127.0f ? 127.0f : f < -127.0f ? -127.0f : f;
-                    const int v = static_cast<int>(f);
-                    p |= static_cast<uint32_t>(v > 0 ? v : 0) << (8 * j);
-                    m |= static_cast<uint32_t>((v < 0 ? v : 0) & 255) << (8 * j);
+                    float f = static_cast<float>(
+                        __builtin_bit_cast(typename E::V2, raw[k][2 * w + j / 2])[j % 2]);
+                    // Rounded to nearest even in the low bits of a number of
+                    // ulp 1; clamping to a whole number may come before it.
+                    f = __builtin_amdgcn_fmed3f(f * inv, -127.0f, 127.0f) + 12582912.0f;
+                    v[j] = __builtin_bit_cast(uint32_t, f);
                 }
-                pos[k][w] = static_cast<int>(p);
-                neg[k][w] = static_cast<int>(m);
+                const uint32_t x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], 0x0C0C0400u),
+                                                         __builtin_amdgcn_perm(v[1], v[0], 0x0C0C0400u),
+                                                         0x05040100u);
+                const uint32_t sign = x >> 7 & 0x01010101u;
+                const uint32_t mask = (sign << 8) - sign;  // 255 in every negative byte
+                qp[k][w] = static_cast<int>(x & ~mask);
+                qn[k][w] = static_cast<int>(x & mask);
             }
         const float mine = __builtin_bit_cast(float, static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) unit[i4] = __shfl(mine, 4 * g4 + i4);
     };
 
-    i32x4 qp[K], qn[K];
-    float unit[4];
-    load_queries(0, qp, qn, unit);
-
-    for (int tile = wave; tile < kChunkTiles; tile += 4) {
-        const int block = chunk * kChunk + 16 * tile + r16;
-        if (chunk * kChunk + 16 * tile >= blocks) break;
-        const int page = block < blocks ? t.page(b, block) : -1;
-        i32x4 hi[K] = {}, lo[K] = {};
-        float eb = 0.0f;
-        if (page >= 0) {
-            const int64_t ph = static_cast<int64_t>(page) * t.kv_heads + h;
+    const int64_t row0 = static_cast<int64_t>(q0) * t.kv_heads + h;  // row of token i: + i kv_heads
+    // Tiles of the chunk: wave w has w, w + 4, w + 8, w + 12.
+    for (int batch = 0; batch < 4 / kBatch; ++batch) {
+        int page[kBatch];
+        float eb[kBatch];
+        i32x4 hi[kBatch][K], lo[kBatch][K];
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int block = chunk * kChunk + 16 * (wave + 4 * (batch * kBatch + x)) + r16;
+            page[x] = batch == 0 ? early[x] : t.page(b, block);
+            if (block >= blocks) page[x] = -1;
+        }
+        // The queries are requested between the pages and the boxes, so that
+        // they are quantized while the boxes are on their way.
+        if (batch == 0) request_queries(0);
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int64_t ph = static_cast<int64_t>(page[x] < 0 ? 0 : page[x]) * t.kv_heads + h;
             const int8_t* const p = a.box + ph * 2 * D + 16 * g4;
+            const bool in = page[x] >= 0;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                hi[k] = *reinterpret_cast<const i32x4*>(p + 64 * k);
-                lo[k] = *reinterpret_cast<const i32x4*>(p + D + 64 * k);
+                hi[x][k] = in ? *reinterpret_cast<const i32x4*>(p + 64 * k) : i32x4{0, 0, 0, 0};
+                lo[x][k] = in ? *reinterpret_cast<const i32x4*>(p + D + 64 * k) : i32x4{0, 0, 0, 0};
             }
-            eb = __builtin_bit_cast(float, static_cast<uint32_t>(a.box_scale[ph]) << 23);
+            eb[x] = in ? __builtin_bit_cast(float, static_cast<uint32_t>(a.box_scale[ph]) << 23) : 0.0f;
         }
-        float s[4];
+        float s[kBatch][4];
         for (int ht = 0; ht < a.head_tiles; ++ht) {
-            if (a.head_tiles > 1) load_queries(ht, qp, qn, unit);
-            i32x4 acc = {0, 0, 0, 0};
+            if (ht > 0 || (batch > 0 && a.head_tiles > 1)) request_queries(ht);
+            if (batch == 0 || a.head_tiles > 1) quantize_queries();
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qp[k], hi[k], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qn[k], lo[k], acc, 0, 0, 0);
-            }
-            // |acc| < 2^23, so the conversion and both products are exact
-            // wherever the result is a normal number.
+            for (int x = 0; x < kBatch; ++x) {
+                i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float f = static_cast<float>(acc[i]) * unit[i] * eb;
-                s[i] = ht == 0 ? f : fmaxf(s[i], f);
-            }
-        }
-        // Maximum over a token's rows.
-        if (rows_shift >= 1) {
-            s[0] = s[1] = fmaxf(s[0], s[1]);
-            s[2] = s[3] = fmaxf(s[2], s[3]);
-        }
-        if (rows_shift >= 2) s[0] = s[1] = s[2] = s[3] = fmaxf(s[0], s[2]);
-        if (rows_shift >= 3) s[0] = fmaxf(s[0], __shfl_xor(s[0], 16));
-        if (rows_shift >= 4) s[0] = fmaxf(s[0], __shfl_xor(s[0], 32));
-        const int step = rows_shift >= 2 ? 4 : 1 << rows_shift;  // rows of this lane a token
-        if (rows_shift >= 3 && (4 * g4 & ((1 << rows_shift) - 1)) != 0) continue;
-        for (int i = 0; i < 4; i += step) {
-            const int token = i0 + ((4 * g4 + i) >> rows_shift);
-            if (token >= n) break;
-            const int pos = position(len, n, token);
-            const int mine = pos < 0 ? 0 : (pos >> t.page_shift) + 1;
-            if (block >= mine) continue;
-            uint32_t key = kIneligible;
-            if (page >= 0 && any_visible(t, b, block, pos)) {
-                const uint32_t u = __builtin_bit_cast(uint32_t, s[i] + 0.0f);  // -0 as 0
-                key = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-                if (block < a.first || block >= mine - a.last) key = kForced;
-            }
-            a.keys[(static_cast<int64_t>(q0 + token) * t.kv_heads + h) * a.key_stride + block] = key;
-        }
-    }
-}
-
-// Sum over the lanes up to and with this one.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v)
-{
-    const int lane = threadIdx.x % 64;
+                for (int k = 0; k < K; ++k) {
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qp[k], hi[x][k], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qn[k], lo[x][k], acc, 0, 0, 0);
+                }
+                // |acc| < 2^23, so the conversion and both products are exact
+                // wherever the result is a normal number.
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
-// The `width` highest keys of a token and head, written in ascending order of
-// their blocks: a radix descent finds the least key taken and how many of the
-// blocks that have it are, then every thread places its own run of blocks.
-__global__ __launch_bounds__(256) void kv_pick_kernel(SelectArgs a)
-{
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t found[2];
-    __shared__ uint32_t part[2][4];
-    const Batch& t = a.batch;
-    const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
-    const int len = t.length(b);
-    const int q0 = t.first_query(b);
-    const int n = t.new_tokens(b, q0);
-    if (i >= n) return;
-    const int pos = position(len, n, i);
-    const int blocks = pos < 0 ? 0 : (pos >> t.page_shift) + 1;
-    const int64_t row = static_cast<int64_t>(q0 + i) * t.kv_heads + h;
-    const uint32_t* const keys = a.keys + row * a.key_stride;
-    int32_t* const out = a.out + row * a.width;
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-
-    uint32_t prefix = 0, mask = 0;
-    uint32_t want = a.width;  // still to be taken among keys that match the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < blocks; j += 256) {
-            const uint32_t k = keys[j];
-            if (k != kIneligible && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {
-            // Lane l takes the bins 255 - 4 l .. 252 - 4 l, highest first.
-            uint32_t c[4], sum = 0;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                c[m] = hist[255 - 4 * lane - m];
-                sum += c[m];
-            }
-            const uint32_t incl = wave_scan(sum);
-            uint32_t above = incl - sum;
-            if (lane == 63 && incl < want) {  // fewer than wanted: all of them
-                found[0] = 256;
-                found[1] = 0;
-            }
-            if (above < want && incl >= want) {
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    if (above < want && above + c[m] >= want) {
-                        found[0] = 255 - 4 * lane - m;
-                        found[1] = want - above;
-                    }
-                    above += c[m];
+                for (int i = 0; i < 4; ++i) {
+                    const float f = static_cast<float>(acc[i]) * unit[i] * eb[x];
+                    s[x][i] = ht == 0 ? f : fmaxf(s[x][i], f);
                 }
             }
         }
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            // Maximum over a token's rows.
+            const int block = chunk * kChunk + 16 * (wave + 4 * (batch * kBatch + x)) + r16;
+            const auto write = [&](int first_row, float score) {
+                const int token = i0 + (first_row >> rows_shift);
+                if (token >= i_end) return;
+                const int pos = position(len, n, token);
+                const int mine = blocks_to(t, pos);
+                uint32_t key = kIneligible;
+                if (block < mine && page[x] >= 0 && any_visible(t, b, block, pos)) {
+                    const uint32_t u = __builtin_bit_cast(uint32_t, score + 0.0f);  // -0 as 0
+                    key = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+                    if (block < a.first || block >= mine - a.last) key = kForced;
+                }
+                if (chunks <= 1)
+                    stage[(token - i0) * kChunk + block] = key;
+                else if (block < mine)
+                    put(a.keys + (row0 + static_cast<int64_t>(token) * t.kv_heads) * a.key_stride + block,
+                        key);
+            };
+            if constexpr (kQuads) {
+                float m = fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3]));
+                if (rows_shift >= 3) m = fmaxf(m, __shfl_xor(m, 16));
+                if (rows_shift >= 4) m = fmaxf(m, __shfl_xor(m, 32));
+                if ((4 * g4 & ((1 << rows_shift) - 1)) == 0) write(4 * g4, m);
+            } else if (rows_shift == 1) {
+                write(4 * g4, fmaxf(s[x][0], s[x][1]));
+                write(4 * g4 + 2, fmaxf(s[x][2], s[x][3]));
+            } else {
+                for (int i = 0; i < 4; ++i) write(4 * g4 + i, s[x][i]);
+            }
+        }
+    }
+    if (chunks > 1) {
+        // The keys are atomics of the whole device, so that their completion
+        // is all that the count has to wait for.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (found[0] == 256) {  // every eligible block (only at the first digit)
-            prefix = 1;
-            want = 0;
-            mask = 0;
-            break;
+        if (threadIdx.x == 0) {
+            uint32_t* const count =
+                a.arrived + (static_cast<int64_t>(b) * a.token_tiles + blockIdx.y) * t.kv_heads + h;
+            const uint32_t before =
+                __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            is_last = before + 1 == static_cast<uint32_t>(chunks);
+            if (is_last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        prefix |= found[0] << shift;
-        mask |= 255u << shift;
-        want = found[1];
+        __syncthreads();
+        if (!is_last) return;
+    } else {
+        __syncthreads();
     }
-    // Taken: keys above `prefix`, and the first `want` that equal it.  Where
-    // all are taken: keys of at least 1.
-    const bool all = mask == 0;
-    const int each_thread = (blocks + 255) / 256;
-    const int begin = tid * each_thread;
-    const int end = begin + each_thread < blocks ? begin + each_thread : blocks;
-    uint32_t above = 0, equal = 0;
-    for (int j = begin; j < end; ++j) {
-        const uint32_t k = keys[j];
-        above += all ? k >= prefix : k > prefix;
-        equal += !all && k == prefix;
-    }
-    const uint32_t sa = wave_scan(above), se = wave_scan(equal);
-    if (lane == 63) {
-        part[0][wave] = sa;
-        part[1][wave] = se;
-    }
-    __syncthreads();
-    uint32_t before_a = sa - above, before_e = se - equal, total_a = 0, total_e = 0;
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) {
-            before_a += part[0][w];
-            before_e += part[1][w];
+    for (int token = i0; token < i_end; ++token) {
+        const int64_t row = row0 + static_cast<int64_t>(token) * t.kv_heads;
+        const int mine = blocks_to(t, position(len, n, token));
+        int32_t* const out = a.out + row * a.width;
+        if (token > i0) __syncthreads();
+        if (chunks <= 1) {
+            const uint32_t* const keys = stage + (token - i0) * kChunk;
+            pick<1>(a, sh, mine, out, [&](int j) { return keys[j]; });
+        } else {
+            const uint32_t* const keys = a.keys + row * a.key_stride;
+            if (mine <= 2048)
+                pick<8>(a, sh, mine, out, [&](int j) { return get(keys + j); });
+            else
+                pick<16>(a, sh, mine, out, [&](int j) { return get(keys + j); });
         }
-        total_a += part[0][w];
-        total_e += part[1][w];
     }
-    uint32_t at = before_a + (before_e < want ? before_e : want);
-    for (int j = begin; j < end; ++j) {
-        const uint32_t k = keys[j];
-        bool take = all ? k >= prefix : k > prefix;
-        if (!all && k == prefix) {
-            take = before_e < want;
-            ++before_e;
-        }
-        if (take) out[at++] = j;
-    }
-    const uint32_t total = total_a + (total_e < want ? total_e : want);
-    for (uint32_t j = total + tid; j < static_cast<uint32_t>(a.width); j += 256) out[j] = -1;
 }
 
 template <class E>
-void launch_score(const SelectArgs& a, uint32_t dim, dim3 grid, hipStream_t stream)
+void launch(const SelectArgs& a, uint32_t dim, dim3 grid, hipStream_t stream)
 {
-    switch (dim) {
-        case 64: kv_score_kernel<E, 64><<<grid, 256, 0, stream>>>(a); break;
-        case 128: kv_score_kernel<E, 128><<<grid, 256, 0, stream>>>(a); break;
-        default: kv_score_kernel<E, 256><<<grid, 256, 0, stream>>>(a); break;
-    }
+    const auto run = [&](auto quads) {
+        constexpr bool kQuads = decltype(quads)::value;
+        switch (dim) {
+            case 64: kv_select_kernel<E, 64, kQuads><<<grid, 256, 0, stream>>>(a); break;
+            case 128: kv_select_kernel<E, 128, kQuads><<<grid, 256, 0, stream>>>(a); break;
+            default: kv_select_kernel<E, 256, kQuads><<<grid, 256, 0, stream>>>(a); break;
+        }
+    };
+    if (a.group_shift >= 2)
+        run(std::true_type{});
+    else
+        run(std::false_type{});
 }
 
 }  // namespace
@@ -337,30 +522,35 @@ int kv_select(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch*
     a.group = static_cast<int>(heads / cache->kv_heads);
     while ((1 << a.group_shift) < a.group && a.group_shift < 4) ++a.group_shift;
     a.head_tiles = (a.group + 15) / 16;
+    // At most four tokens a tile: its last workgroup picks for them in turn.
+    a.tokens = 16 >> a.group_shift;
+    if (a.tokens > 4) a.tokens = 4;
     a.width = static_cast<int>(width);
     a.first = static_cast<int>(first);
     a.last = static_cast<int>(last);
     const uint32_t tokens = batch->query_offsets == nullptr ? 1 : batch->max_queries;
-    if (tokens > 65535)
-        return ctx->fail(GOFANN_ERR_UNSUPPORTED, "kv_select: at most 65535 tokens a sequence");
+    a.token_tiles = static_cast<int>((tokens + a.tokens - 1) / a.tokens);
+    if (a.token_tiles > 65535)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, "kv_select: too many tokens a sequence for one call");
     const uint32_t most = static_cast<uint32_t>(a.batch.max_positions);
     const uint32_t blocks = (most + cache->page_size - 1) / cache->page_size;
-    a.key_stride = blocks;
-    const size_t bytes = static_cast<size_t>(batch->queries) * cache->kv_heads * blocks * 4;
-    if (bytes > 0) {
-        a.keys = static_cast<uint32_t*>(ctx->workspace(Context::kScratchKv, bytes));
+    const uint32_t chunks = blocks > 0 ? (blocks + kChunk - 1) / kChunk : 1;
+    if (chunks > 1) {
+        a.key_stride = blocks;
+        a.keys = static_cast<uint32_t*>(
+            ctx->workspace(Context::kScratchKv,
+                           static_cast<size_t>(batch->queries) * cache->kv_heads * a.key_stride * 4));
         if (a.keys == nullptr) return GOFANN_ERR_NOMEM;
+        a.arrived = static_cast<uint32_t*>(
+            ctx->zeroed(Context::kScratchKvArrived, static_cast<size_t>(batch->sequences) *
+                                                        a.token_tiles * cache->kv_heads * 4));
+        if (a.arrived == nullptr) return GOFANN_ERR_NOMEM;
     }
-    if (blocks > 0) {
-        const uint32_t per = 16u >> a.group_shift;
-        const dim3 grid((blocks + kChunk - 1) / kChunk * cache->kv_heads, (tokens + per - 1) / per,
-                        batch->sequences);
-        if (cache->elem == GOFANN_ELEM_BF16)
-            launch_score<Bf16>(a, cache->dim, grid, ctx->stream);
-        else
-            launch_score<F16>(a, cache->dim, grid, ctx->stream);
-    }
-    kv_pick_kernel<<<dim3(cache->kv_heads, tokens, batch->sequences), 256, 0, ctx->stream>>>(a);
+    const dim3 grid(chunks * cache->kv_heads, static_cast<uint32_t>(a.token_tiles), batch->sequences);
+    if (cache->elem == GOFANN_ELEM_BF16)
+        launch<Bf16>(a, cache->dim, grid, ctx->stream);
+    else
+        launch<F16>(a, cache->dim, grid, ctx->stream);
     if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_select: launch");
     return GOFANN_OK;
 }

@@ -533,16 +533,16 @@ def test_workspace_too_small_under_capture_is_an_error(gpu_ctx):
     with torch.cuda.stream(side):
         own.bind_stream(side)
         d, db, (k, v, q) = _step_world(own)
-        blocks = torch.empty((3, 2, 4), dtype=torch.int32, device="cuda")
+        out = torch.empty_like(q)
         side.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
             d.append(db, k, v)  # needs none
             with pytest.raises(_lib.GofannError, match="before capturing"):
-                d.select(db, q, 4, out=blocks)
+                d.attend(db, q, out=out)  # 700 positions in splits
         graph.replay()
         side.synchronize()
-        d.select(db, q, 4, out=blocks)
+        d.attend(db, q, out=out)
         side.synchronize()
     own.close()
 
