@@ -138,7 +138,7 @@ struct Raw {
 // The 4-bit codes become 16-bit elements by the hardware's conversion, which
 // applies the group's power of two; both are exact.
 template <class E, int D, int NT, int WT>
-__global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention_kernel(AttendArgs a)
 {
     using V8 = typename E::V8;
     constexpr int kRows = 16 * NT;
@@ -357,49 +357,50 @@ __global__ __launch_bounds__(256, 2) void kv_attention_kernel(AttendArgs a)
         // Tiles that every row sees whole, then the others.
         uint64_t whole = __ballot(word == 0xFFFFFFFFu && t0 + kTile <= all_see);
         uint64_t part = __ballot(word != 0) & ~whole;
-        if (whole != 0) {
-            uint32_t now = __builtin_amdgcn_readlane(at, __builtin_ctzll(whole));
-            load_keys(now);
-            load_values(now);
+        const auto run = [&](auto kind, uint64_t live) {
+            constexpr bool kMasked = decltype(kind)::value;
+            if (live == 0) return;
+            int i = __builtin_ctzll(live);
+            load_keys(__builtin_amdgcn_readlane(at, i));
+            load_values(__builtin_amdgcn_readlane(at, i));
             while (true) {
-                whole &= whole - 1;
-                const bool more = whole != 0;
-                if (more) now = __builtin_amdgcn_readlane(at, __builtin_ctzll(whole));
+                live &= live - 1;
+                const bool more = live != 0;
+                const int next = more ? __builtin_ctzll(live) : i;
+                const uint32_t ahead = __builtin_amdgcn_readlane(at, next);
                 scores();
-                if (more) load_keys(now);
+                if (more) load_keys(ahead);
+                uint32_t mine = 0;
+                if constexpr (kMasked) {
+                    const int from = __builtin_amdgcn_readlane(t0, i) + 8 * g4;
+                    mine = static_cast<uint32_t>(__builtin_amdgcn_readlane(word, i)) >> (8 * g4);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        int left = limit[nt] - from;
+                        left = left < 0 ? 0 : left > 8 ? 8 : left;
+                        const uint32_t ok = mine & ((1u << left) - 1u);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            s[nt][e / 4][e % 4] = (ok >> e & 1u) ? s[nt][e / 4][e % 4] : -__builtin_inff();
+                    }
+                }
                 weights();
                 value_scales();
+                if constexpr (kMasked) {
+                    // A position that no row sees may hold anything: its scale
+                    // must not turn a weight of zero into a NaN.
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!(mine >> e & 1u)) scale[e] = 127u << 23;
+                }
                 product();
                 if (!more) break;
-                load_values(now);
+                load_values(ahead);
+                i = next;
             }
-        }
-        for (; part != 0; part &= part - 1) {
-            const int i = __builtin_ctzll(part);
-            const uint32_t now = __builtin_amdgcn_readlane(at, i);
-            load_keys(now);
-            load_values(now);
-            const int from = __builtin_amdgcn_readlane(t0, i) + 8 * g4;
-            const uint32_t mine = static_cast<uint32_t>(__builtin_amdgcn_readlane(word, i)) >> (8 * g4);
-            scores();
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                int left = limit[nt] - from;
-                left = left < 0 ? 0 : left > 8 ? 8 : left;
-                const uint32_t ok = mine & ((1u << left) - 1u);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    s[nt][e / 4][e % 4] = (ok >> e & 1u) ? s[nt][e / 4][e % 4] : -__builtin_inff();
-            }
-            weights();
-            // A position that no row sees may hold anything: its scale must
-            // not turn a weight of zero into a NaN.
-            value_scales();
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!(mine >> e & 1u)) scale[e] = 127u << 23;
-            product();
-        }
+        };
+        run(std::false_type{}, whole);
+        run(std::true_type{}, part);
     }
 
 #pragma unroll

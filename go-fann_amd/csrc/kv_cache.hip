@@ -15,6 +15,10 @@ int split_tiles(const Context* ctx, uint64_t items, uint64_t most, bool ragged)
     uint64_t n = (items * most + resident - 1) / resident;
     n = (n + 3) / 4 * 4;
     if (n < 4) n = 4;
+    // Few enough for the last workgroup to join, where that costs a wave at
+    // most two tiles.
+    const uint64_t few = (most + kv::kJoinSplits - 1) / kv::kJoinSplits;
+    if (n < few && few <= 8) n = few;
     if (ragged && n > 64) n = 64;
     return static_cast<int>(n);
 }

@@ -158,18 +158,18 @@ class KvCache:
     # -- checks ----------------------------------------------------------
     def _rows(self, name: str, t: torch.Tensor, queries: int, heads: int | None,
               written: bool = False) -> _lib.KvRows:
-        if t.dim() != 3 or t.shape[0] != queries or t.shape[2] != self.dim or \
-                (heads is not None and t.shape[1] != heads):
+        shape, (st, sh, sd) = t.shape, t.stride() if t.dim() == 3 else (0, 0, 0)
+        if len(shape) != 3 or shape[0] != queries or shape[2] != self.dim or \
+                (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [{queries}][{heads if heads is not None else 'heads'}]"
-                             f"[{self.dim}], got {tuple(t.shape)}")
+                             f"[{self.dim}], got {tuple(shape)}")
         if t.dtype != self.dtype or t.device != self.device:
             raise ValueError(f"{name} must be {self.dtype} on {self.device}")
-        st, sh, sd = t.stride()
         if sd != 1:
             raise ValueError(f"{name} must be contiguous along its channels")
-        if written and ((t.shape[0] > 1 and st < self.dim) or (t.shape[1] > 1 and sh < self.dim)
-                        or (t.shape[0] > 1 and t.shape[1] > 1 and st < sh * t.shape[1]
-                            and sh < st * t.shape[0])):
+        if written and ((shape[0] > 1 and st < self.dim) or (shape[1] > 1 and sh < self.dim)
+                        or (shape[0] > 1 and shape[1] > 1 and st < sh * shape[1]
+                            and sh < st * shape[0])):
             raise ValueError(f"rows of {name} overlap")
         return _lib.KvRows(t.data_ptr(), st, sh)
 
