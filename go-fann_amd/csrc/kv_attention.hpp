@@ -55,6 +55,10 @@ __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int 
     return t;
 }
 
+// How far, in powers of two, a score may pass the running maximum before that
+// is renewed.
+constexpr float kSlack = 8.0f;
+
 // Splits up to which the last workgroup of an item to finish joins them
 // itself; past it the partial results are too many for one workgroup.
 constexpr int kJoinSplits = 16;
@@ -112,6 +116,54 @@ __device__ __forceinline__ void finish(const AttendArgs& a, const Batch& t, int 
             (top + __builtin_log2f(total)) * 0.69314718055994531f;
 }
 
+// Scores of a lane's eight positions, -inf where the row may not look: bit e
+// of `mine` is position e's, and only the first `left` are before the row's end.
+__device__ __forceinline__ void mask_scores(f32x4 (&s)[2], uint32_t mine, int left)
+{
+    left = left < 0 ? 0 : left > 8 ? 8 : left;
+    const uint32_t ok = mine & ((1u << left) - 1u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e / 4][e % 4] = (ok >> e & 1u) ? s[e / 4][e % 4] : -__builtin_inff();
+}
+
+// Weights 2^(score - m) of a row's scores, the row's running maximum m, sum of
+// weights and weighted values o brought along; mu is m, or 0 while there is
+// none.  The maximum is renewed only where a score passes it by more than
+// kSlack (in powers of two): until then the weights are at most 2^kSlack, which
+// costs 32-bit sums nothing.  The weights enter the product in 16 bits, as the
+// values do; their sum stays in 32.
+template <class E, int kUnit>
+__device__ __forceinline__ typename E::V8 weigh(const f32x4 (&s)[2], float scale_log2, float& m,
+                                                float& mu, float& sum, f32x4 (&o)[kUnit])
+{
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e / 4][e % 4]);
+    top *= scale_log2;
+    if (__any(top > m + kSlack)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float fresh = fmaxf(m, top);
+        const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
+        const float f = __builtin_amdgcn_exp2f(m - keep);
+        sum *= f;
+#pragma unroll
+        for (int c = 0; c < kUnit; ++c) o[c] *= f;
+        m = fresh;
+        mu = keep;
+    }
+    typename E::V8 p;
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], scale_log2, -mu));
+        sum += w[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = static_cast<typename E::T>(w[e]);
+    return p;
+}
+
 // What a lane loads of one tile: keys of two positions, values of eight.
 template <int D>
 struct Raw {
@@ -137,13 +189,12 @@ struct Raw {
 //   * ends with the channels [g dim/4, (g+1) dim/4) of query r's output.
 // The 4-bit codes become 16-bit elements by the hardware's conversion, which
 // applies the group's power of two; both are exact.
-template <class E, int D, int NT, int WT>
+template <class E, int D, int NT>
 __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention_kernel(AttendArgs a)
 {
     using V8 = typename E::V8;
     constexpr int kRows = 16 * NT;
     constexpr int kUnit = D / 16;  // channels of a unit, tiles of O
-    constexpr float kSlack = 8.0f;
     const Batch& t = a.batch;
     const int lane = threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -155,12 +206,8 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
     const int len = t.length(b);
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
-    RowTile rt;
-    if constexpr (WT == 1)
-        rt = row_tile(a, index * 4 + wave, kRows, len, n);
-    else
-        rt = row_tile(a, index, kRows, len, n);
-    if (rt.end <= rt.begin) return;  // WT > 1: the whole workgroup; WT == 1: no barrier follows
+    const RowTile rt = row_tile(a, index, kRows, len, n);
+    if (rt.end <= rt.begin) return;
     const int tiles = tiles_of(a, rt);
     const int tile_begin = split * a.split_tiles;
     if (split > 0 && tile_begin >= tiles) return;
@@ -259,40 +306,6 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
         }
     };
     V8 p[NT];
-    const auto weights = [&]() {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            // The running maximum is renewed only where a score passes it by
-            // more than kSlack (in powers of two): until then the weights are
-            // at most 2^kSlack, which costs 32-bit sums nothing.
-            float top = s[nt][0][0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top = fmaxf(top, s[nt][e / 4][e % 4]);
-            top *= a.scale_log2;
-            if (__any(top > m[nt] + kSlack)) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float fresh = fmaxf(m[nt], top);
-                const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
-                const float f = __builtin_amdgcn_exp2f(m[nt] - keep);
-                sum[nt] *= f;
-#pragma unroll
-                for (int c = 0; c < kUnit; ++c) o[nt][c] *= f;
-                m[nt] = fresh;
-                mu[nt] = keep;
-            }
-            float w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][e / 4][e % 4], a.scale_log2, -mu[nt]));
-                sum[nt] += w[e];
-            }
-            // The weights enter the product in 16 bits, as the values do; their
-            // sum stays in 32.
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[nt][e] = static_cast<typename E::T>(w[e]);
-        }
-    };
     uint32_t scale[8];  // of the eight positions' values, in bits 30:23
     const auto value_scales = [&]() {
 #pragma unroll
@@ -331,11 +344,9 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
     // This wave's tiles, 64 at a time: lane l looks up the l-th one's page and
     // filter word, so that only tiles with a visible position are visited and
     // the next one's address is at hand while it is loaded.
-    const int step = WT;
-    const int first_tile = tile_begin + (WT == 1 ? 0 : wave);
     const int page_tiles_shift = t.page_shift - 5;
-    for (int base = first_tile; base < tile_end; base += 64 * step) {
-        const int tile = base + lane * step;
+    for (int base = tile_begin + wave; base < tile_end; base += 64 * 4) {
+        const int tile = base + lane * 4;
         uint32_t at = 0, word = 0;
         int t0 = 0;
         if (tile < tile_end) {
@@ -375,16 +386,11 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
                     const int from = __builtin_amdgcn_readlane(t0, i) + 8 * g4;
                     mine = static_cast<uint32_t>(__builtin_amdgcn_readlane(word, i)) >> (8 * g4);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        int left = limit[nt] - from;
-                        left = left < 0 ? 0 : left > 8 ? 8 : left;
-                        const uint32_t ok = mine & ((1u << left) - 1u);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            s[nt][e / 4][e % 4] = (ok >> e & 1u) ? s[nt][e / 4][e % 4] : -__builtin_inff();
-                    }
+                    for (int nt = 0; nt < NT; ++nt) mask_scores(s[nt], mine, limit[nt] - from);
                 }
-                weights();
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    p[nt] = weigh<E, kUnit>(s[nt], a.scale_log2, m[nt], mu[nt], sum[nt], o[nt]);
                 value_scales();
                 if constexpr (kMasked) {
                     // A position that no row sees may hold anything: its scale
@@ -409,137 +415,456 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
         sum[nt] += __shfl_xor(sum[nt], 32);
     }
 
-    if constexpr (WT > 1) {
-        // The four waves' maxima, sums and outputs joined through LDS, sixteen
-        // rows at a time: thread x then has four channels of row x / (D / 4)
-        // and of every 256 / (D / 4)-th after it.
-        constexpr int kLanes = D / 4, kStep = 256 / kLanes;
-        constexpr int kPad = D + 4;  // rows start on other banks
-        __shared__ float wm[4][kRows], ws[4][kRows];
-        __shared__ __attribute__((aligned(16))) float wo[4][16][kPad];
-        const int active = (tiles + a.split_tiles - 1) / a.split_tiles;
-        const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
-        float* const po = a.part_o + item * a.splits * kRows * D;
-        float* const pm = a.part_ml + item * a.splits * kRows * 2;
-        const int my_ch = 4 * (threadIdx.x % kLanes);
+    // The four waves' maxima, sums and outputs joined through LDS, sixteen
+    // rows at a time: thread x then has four channels of row x / (D / 4)
+    // and of every 256 / (D / 4)-th after it.
+    constexpr int kLanes = D / 4, kStep = 256 / kLanes;
+    constexpr int kPad = D + 4;  // rows start on other banks
+    __shared__ float wm[4][kRows], ws[4][kRows];
+    __shared__ __attribute__((aligned(16))) float wo[4][16][kPad];
+    const int active = (tiles + a.split_tiles - 1) / a.split_tiles;
+    const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
+    float* const po = a.part_o + item * a.splits * kRows * D;
+    float* const pm = a.part_ml + item * a.splits * kRows * 2;
+    const int my_ch = 4 * (threadIdx.x % kLanes);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (g4 == 0) {
-                wm[wave][16 * nt + r16] = m[nt];
-                ws[wave][16 * nt + r16] = sum[nt];
-            }
-#pragma unroll
-            for (int x = 0; x < kUnit; ++x) {
-                // Channels [g dim/4, ..) in order: unit 4 g + i, tile c.
-                f32x4 v;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) v[y] = o[nt][(4 * x + y) % kUnit][(4 * x + y) / kUnit];
-                *reinterpret_cast<f32x4*>(&wo[wave][r16][(D / 4) * g4 + 4 * x]) = v;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = threadIdx.x / kLanes; r < 16; r += kStep) {
-                const int row = rt.begin + 16 * nt + r;
-                if (row >= rt.end) break;
-                float top = wm[0][16 * nt + r];
-#pragma unroll
-                for (int w = 1; w < 4; ++w) top = fmaxf(top, wm[w][16 * nt + r]);
-                const float keep = top == -__builtin_inff() ? 0.0f : top;
-                float total = 0.0f;
-                f32x4 acc{0, 0, 0, 0};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(wm[w][16 * nt + r] - keep);
-                    total += f * ws[w][16 * nt + r];
-                    acc += f * *reinterpret_cast<const f32x4*>(&wo[w][r][my_ch]);
-                }
-                if (active <= 1) {
-                    finish<E>(a, t, q0, h, row, my_ch, acc, top, total);
-                } else {
-                    const int at = split * kRows + 16 * nt + r;
-                    float* const to = po + static_cast<int64_t>(at) * D + my_ch;
-                    if (a.arrived != nullptr) {
-                        put2(to, acc[0], acc[1]);
-                        put2(to + 2, acc[2], acc[3]);
-                        if (my_ch == 0) put2(pm + 2 * at, top, total);
-                    } else {
-                        *reinterpret_cast<f32x4*>(to) = acc;
-                        if (my_ch == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{top, total};
-                    }
-                }
-            }
-            if (nt + 1 < NT) __syncthreads();
+    for (int nt = 0; nt < NT; ++nt) {
+        if (g4 == 0) {
+            wm[wave][16 * nt + r16] = m[nt];
+            ws[wave][16 * nt + r16] = sum[nt];
         }
-        if (active <= 1) return;
-        if (a.arrived == nullptr) return;
-        // The workgroup that arrives last joins the splits, in their order
-        // whichever that is.  Every access to the partial results is an atomic
-        // of the whole device (put, get), which no XCD's cache holds back, so
-        // their completion is all that the count has to wait for; a fence of
-        // the device would write back the XCD's cache and take 5 us a call.
-        __shared__ int last;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const uint32_t before =
-                __hip_atomic_fetch_add(a.arrived + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            last = before + 1 == static_cast<uint32_t>(active);
-            if (last) __hip_atomic_store(a.arrived + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int x = 0; x < kUnit; ++x) {
+            // Channels [g dim/4, ..) in order: unit 4 g + i, tile c.
+            f32x4 v;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[y] = o[nt][(4 * x + y) % kUnit][(4 * x + y) / kUnit];
+            *reinterpret_cast<f32x4*>(&wo[wave][r16][(D / 4) * g4 + 4 * x]) = v;
         }
         __syncthreads();
-        if (!last) return;
-        __shared__ float jm[kJoinSplits][kRows], js[kJoinSplits][kRows];
-        for (int x = threadIdx.x; x < active * kRows; x += 256) {
-            const bool in = rt.begin + x % kRows < rt.end;
-            const float2 v = in ? get2(pm + 2 * x) : float2{0.0f, 0.0f};
-            jm[x / kRows][x % kRows] = v.x;
-            js[x / kRows][x % kRows] = v.y;
-        }
-        __syncthreads();
-        for (int r = threadIdx.x / kLanes; rt.begin + r < rt.end; r += kStep) {
-            float top = -__builtin_inff();
-            for (int w = 0; w < active; ++w) top = fmaxf(top, jm[w][r]);
+#pragma unroll
+        for (int r = threadIdx.x / kLanes; r < 16; r += kStep) {
+            const int row = rt.begin + 16 * nt + r;
+            if (row >= rt.end) break;
+            float top = wm[0][16 * nt + r];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) top = fmaxf(top, wm[w][16 * nt + r]);
             const float keep = top == -__builtin_inff() ? 0.0f : top;
             float total = 0.0f;
             f32x4 acc{0, 0, 0, 0};
-#pragma unroll 4
-            for (int w = 0; w < active; ++w) {
-                const float f = __builtin_amdgcn_exp2f(jm[w][r] - keep);
-                total += f * js[w][r];
-                const float* const from = po + (static_cast<int64_t>(w) * kRows + r) * D + my_ch;
-                const float2 lo = get2(from), hi = get2(from + 2);
-                acc += f * f32x4{lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(wm[w][16 * nt + r] - keep);
+                total += f * ws[w][16 * nt + r];
+                acc += f * *reinterpret_cast<const f32x4*>(&wo[w][r][my_ch]);
             }
-            finish<E>(a, t, q0, h, rt.begin + r, my_ch, acc, top, total);
-        }
-    } else {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int row = rt.begin + 16 * nt + r16;
-            if (row >= rt.end) continue;
-            const int i_tok = row / a.group, head = h * a.group + row % a.group;
-            uint16_t* const p = a.out.p + (q0 + i_tok) * a.out.token_stride + head * a.out.head_stride;
-            const float inv = sum[nt] != 0.0f ? 1.0f / sum[nt] : 0.0f;
-            // Channels [g dim/4, (g+1) dim/4) in order: unit 4 g + i, tile c.
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                u32x4 v;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int ch = 8 * x + 2 * y;
-                    typename E::V2 e;
-                    e[0] = static_cast<typename E::T>(o[nt][ch % kUnit][ch / kUnit] * inv);
-                    e[1] = static_cast<typename E::T>(o[nt][(ch + 1) % kUnit][ch / kUnit] * inv);
-                    v[y] = __builtin_bit_cast(uint32_t, e);
+            if (active <= 1) {
+                finish<E>(a, t, q0, h, row, my_ch, acc, top, total);
+            } else {
+                const int at = split * kRows + 16 * nt + r;
+                float* const to = po + static_cast<int64_t>(at) * D + my_ch;
+                if (a.arrived != nullptr) {
+                    put2(to, acc[0], acc[1]);
+                    put2(to + 2, acc[2], acc[3]);
+                    if (my_ch == 0) put2(pm + 2 * at, top, total);
+                } else {
+                    *reinterpret_cast<f32x4*>(to) = acc;
+                    if (my_ch == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{top, total};
                 }
-                asm("" : "+v"(v));
-                store8(p + (D / 4) * g4 + 8 * x, v, a.out.wide);
             }
-            if (a.lse != nullptr && g4 == 0)
-                a.lse[static_cast<int64_t>(q0 + i_tok) * t.kv_heads * a.group + head] =
-                    (m[nt] + __builtin_log2f(sum[nt])) * 0.69314718055994531f;
         }
+        if (nt + 1 < NT) __syncthreads();
     }
+    if (active <= 1) return;
+    if (a.arrived == nullptr) return;
+    // The workgroup that arrives last joins the splits, in their order
+    // whichever that is.  Every access to the partial results is an atomic
+    // of the whole device (put, get), which no XCD's cache holds back, so
+    // their completion is all that the count has to wait for; a fence of
+    // the device would write back the XCD's cache and take 5 us a call.
+    __shared__ int last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t before =
+            __hip_atomic_fetch_add(a.arrived + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = before + 1 == static_cast<uint32_t>(active);
+        if (last) __hip_atomic_store(a.arrived + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    __shared__ float jm[kJoinSplits][kRows], js[kJoinSplits][kRows];
+    for (int x = threadIdx.x; x < active * kRows; x += 256) {
+        const bool in = rt.begin + x % kRows < rt.end;
+        const float2 v = in ? get2(pm + 2 * x) : float2{0.0f, 0.0f};
+        jm[x / kRows][x % kRows] = v.x;
+        js[x / kRows][x % kRows] = v.y;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x / kLanes; rt.begin + r < rt.end; r += kStep) {
+        float top = -__builtin_inff();
+        for (int w = 0; w < active; ++w) top = fmaxf(top, jm[w][r]);
+        const float keep = top == -__builtin_inff() ? 0.0f : top;
+        float total = 0.0f;
+        f32x4 acc{0, 0, 0, 0};
+#pragma unroll 4
+        for (int w = 0; w < active; ++w) {
+            const float f = __builtin_amdgcn_exp2f(jm[w][r] - keep);
+            total += f * js[w][r];
+            const float* const from = po + (static_cast<int64_t>(w) * kRows + r) * D + my_ch;
+            const float2 lo = get2(from), hi = get2(from + 2);
+            acc += f * f32x4{lo.x, lo.y, hi.x, hi.y};
+        }
+        finish<E>(a, t, q0, h, rt.begin + r, my_ch, acc, top, total);
+    }
+}
+
+// Long chunks: four waves of 32 rows each read the same positions.
+//
+// A tile of 32 positions is D / 16 products S^T += K Q^T and D / 16 products
+// O^T += V^T P^T, all v_mfma_f32_32x32x16: beside them the vector unit keeps
+// working (three of its instructions in the time of 16 matrix cycles cost 8%
+// more time; beside the 16 x 16 x 32 products, 20%).  The order of the
+// contracted index is chosen so that a lane's scores are its weights: lane
+// (r, g) = (lane % 32, lane / 32)
+//   * gets the scores of query r against positions 16 u + 8 g + e, e < 8, for
+//     u = 0 and 1, which are the slots of P^T that it feeds to product u;
+//   * feeds, as row r of V^T, channels [r dim/32, (r+1) dim/32), one a tile.
+// Converting a tile's codes in every wave would take more vector instructions
+// than the softmax.  So each wave converts a quarter of the keys and values
+// into LDS, in the order in which lanes feed them to the products (16 bytes a
+// lane, no bank conflicts), and all four read them from there.  A turn takes
+// two tiles (one at 256 channels): while they are multiplied the next two are
+// converted and two more requested; one barrier a turn.
+//
+// 2,048 tokens of 32 heads over 16,390 positions, 516 GFLOP: 0.63 ms, 820
+// TFLOP/s, 0.60 of what a large matrix product of the library reaches.  The
+// chip's power bounds it: half of the workgroups on half of the CUs run 1.65
+// times as fast each, and one or two tiles a turn, or scores formed a turn
+// ahead of their softmax, end within 3% of each other.  Without LDS, each wave
+// converting for itself (16 x 16 products): 0.69 ms.
+template <class E, int D>
+__global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
+{
+    using V8 = typename E::V8;
+    constexpr int kRows = 32;
+    constexpr int kKeys = D / 16;     // fragments of a tile's keys
+    constexpr int kMine = kKeys / 4;  // of them a wave's
+    constexpr int kTiles = D / 32;    // tiles of O
+    constexpr int kPer = D == 256 ? 1 : 2;  // tiles a turn
+    __shared__ u32x4 keys[2][kPer][kKeys][64];
+    __shared__ u32x4 values[2][kPer][kTiles][2][64];
+    const Batch& t = a.batch;
+    const int lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int r32 = lane % 32, g2 = lane / 32;
+    const int h = blockIdx.x;
+    const int index = gridDim.y - 1 - blockIdx.y;  // the longest rows first
+    const int b = blockIdx.z;
+    const int len = t.length(b);
+    const int q0 = t.first_query(b);
+    const int n = t.new_tokens(b, q0);
+    const RowTile all = row_tile(a, index, 4 * kRows, len, n);
+    if (all.end <= all.begin) return;
+    const int tiles = tiles_of(a, all);
+    const int hi_pos = all.last_pos + 1;
+    const int first_see = all.first_pos + 1;  // positions that every row of the workgroup sees
+    // This wave's rows; at a chunk's end maybe none, and it only converts.
+    const int begin = all.begin + wave * kRows;
+    const int end = begin + kRows < all.end ? begin + kRows : all.end;
+
+    // Fragment j of the keys is of wave j / kMine: channels 16 kMine w + 8 kMine
+    // g + 8 i + e, so that a lane's share of a tile is one load.
+    V8 q[kKeys];
+    const int row = begin + r32;
+    const bool in = row < end;
+    const int token = (in ? row : all.begin) / a.group;
+    const int head = h * a.group + (in ? row : all.begin) % a.group;
+    const int limit = in ? len - n + token + 1 : 0;
+    {
+        const uint16_t* const p = a.q.p + (q0 + token) * a.q.token_stride + head * a.q.head_stride;
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+            q[j] = __builtin_bit_cast(
+                V8, load8(p + 16 * kMine * (j / kMine) + 8 * kMine * g2 + 8 * (j % kMine), a.q.wide));
+    }
+    f32x16 o[kTiles];
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
+    float m = -__builtin_inff(), mu = 0.0f, sum = 0.0f;
+
+    // This wave's share of a tile as it is in the cache: the key of one
+    // position a lane (row r of S^T is position 16 u + 8 g + 4 a + b for
+    // r = 16 u + 8 a + 4 g + b), and the values of eight, of product `half`.
+    uint32_t kr[kPer][kMine], ks[kPer], vr[kPer][D == 64 ? 4 : 8], vs[kPer][2];
+    const int half = wave / 2;
+    const uint32_t my_key = 16 * (r32 / 16) + 8 * (r32 / 4 % 2) + 4 * (r32 / 8 % 2) + r32 % 4;
+    const int my_block = 2 * half + g2;  // of eight positions
+    const uint32_t key_at = my_key * (D / 2) + 8 * kMine * wave + 4 * kMine * g2;
+    const uint32_t key_scale_at = my_key * (D / 32) + (16 * kMine * wave + 8 * kMine * g2) / 32;
+    const uint32_t value_at = (my_block * 16 + r32 / 2) * (D / 4);
+    const uint32_t value_scale_at = (my_block * (D / 32) + r32 * D / 1024) * 8;
+    const auto request = [&](int x, uint32_t at) {
+        const uint64_t tile = at;
+        const uint8_t* const kc = a.k_codes + tile * (16 * D) + key_at;
+        if constexpr (kMine == 1) {
+            kr[x][0] = *reinterpret_cast<const uint32_t*>(kc);
+        } else if constexpr (kMine == 2) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(kc);
+            kr[x][0] = v[0];
+            kr[x][1] = v[1];
+        } else {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(kc);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kr[x][j] = v[j];
+        }
+        ks[x] = (a.k_scales + tile * D)[key_scale_at];
+        const uint8_t* const vp = a.v_codes + tile * (16 * D) + value_at;
+        if constexpr (D == 256) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                vr[x][e] = *reinterpret_cast<const uint32_t*>(vp + 8 * e + 4 * (r32 % 2));
+        } else {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(vp + 16 * c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) vr[x][4 * c + j] = v[j];
+            }
+        }
+        const u32x2 s = *reinterpret_cast<const u32x2*>(a.v_scales + tile * D + value_scale_at);
+        vs[x][0] = s[0];
+        vs[x][1] = s[1];
+    };
+    // .. and as elements in LDS.  word: the tile's filter; the scale of a
+    // position that no row sees, which may be anything, becomes 1.
+    const auto convert = [&](auto kind, int x, int buf, uint32_t word) {
+        const uint32_t sc = ks[x] << 23;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            keys[buf][x][wave * kMine + i][lane] =
+                u32x4{E::template decode<0>(kr[x][i], sc), E::template decode<1>(kr[x][i], sc),
+                      E::template decode<2>(kr[x][i], sc), E::template decode<3>(kr[x][i], sc)};
+        if (D == 64 && wave % 2 != 0) return;  // one byte a position: two waves convert
+        uint32_t scale[8];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            scale[4 * w] = vs[x][w] << 23;
+            scale[4 * w + 1] = vs[x][w] << 15;
+            scale[4 * w + 2] = vs[x][w] << 7;
+            scale[4 * w + 3] = vs[x][w] >> 1;
+        }
+        if constexpr (decltype(kind)::value) {
+            const uint32_t mine = word >> (16 * half + 8 * g2);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(mine >> e & 1u)) scale[e] = 127u << 23;
+        }
+        // Bytes of a lane's that this wave converts: D = 128: byte w % 2 of two,
+        // D = 256: bytes 2 (w % 2) and that plus 1 of four.
+        constexpr int kOwn = D == 256 ? 2 : 1;
+#pragma unroll
+        for (int y = 0; y < kOwn; ++y) {
+            const int byte = D == 64 ? 0 : D == 128 ? wave % 2 : 2 * (wave % 2) + y;
+            uint32_t g[2];  // the byte of four positions each
+            if constexpr (D == 64) {
+                const uint32_t pick = 0x06040200u + 0x01010101u * (r32 % 2);
+                g[0] = __builtin_amdgcn_perm(vr[x][1], vr[x][0], pick);
+                g[1] = __builtin_amdgcn_perm(vr[x][3], vr[x][2], pick);
+            } else {
+                const uint32_t at = D == 128 ? 2 * (r32 % 2) + byte : byte;
+                const uint32_t low = 0x0C0C0400u + 0x0101u * at, high = 0x04000C0Cu + 0x01010000u * at;
+                g[0] = __builtin_amdgcn_perm(vr[x][1], vr[x][0], low) | __builtin_amdgcn_perm(vr[x][3], vr[x][2], high);
+                g[1] = __builtin_amdgcn_perm(vr[x][5], vr[x][4], low) | __builtin_amdgcn_perm(vr[x][7], vr[x][6], high);
+            }
+            const uint32_t d[8] = {
+                E::template decode<0>(g[0], scale[0]), E::template decode<1>(g[0], scale[1]),
+                E::template decode<2>(g[0], scale[2]), E::template decode<3>(g[0], scale[3]),
+                E::template decode<0>(g[1], scale[4]), E::template decode<1>(g[1], scale[5]),
+                E::template decode<2>(g[1], scale[6]), E::template decode<3>(g[1], scale[7])};
+            u32x4 even, odd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                even[j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], 0x05040100u);
+                odd[j] = __builtin_amdgcn_perm(d[2 * j + 1], d[2 * j], 0x07060302u);
+            }
+            values[buf][x][2 * byte][half][lane] = even;
+            values[buf][x][2 * byte + 1][half][lane] = odd;
+        }
+    };
+    // Fragments are read from LDS kAhead at a time, before their products.
+    constexpr int kAhead = D == 128 ? 8 : 4;
+    const auto multiply = [&](auto kind, int buf, const int (&from)[kPer], const uint32_t (&mine)[kPer]) {
+        f32x16 s[kPer];
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+#pragma unroll
+            for (int lead = 0; lead < kKeys; lead += kAhead) {
+                u32x4 f[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) f[j] = keys[buf][x][lead + j][lane];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    s[x] = E::mfma(__builtin_bit_cast(V8, f[j]), q[lead + j], s[x]);
+            }
+            if constexpr (decltype(kind)::value) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    int left = limit - from[x] - 16 * u - 8 * g2;
+                    left = left < 0 ? 0 : left > 8 ? 8 : left;
+                    const uint32_t ok = mine[x] >> (16 * u + 8 * g2) & ((1u << left) - 1u);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        s[x][8 * u + e] = (ok >> e & 1u) ? s[x][8 * u + e] : -__builtin_inff();
+                }
+            }
+        }
+        // As weigh(), for 16 scores a tile and lane and two lanes a row.
+        float top = s[0][0];
+#pragma unroll
+        for (int x = 0; x < kPer; ++x)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
+        top *= a.scale_log2;
+        if (__any(top > m + kSlack)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float fresh = fmaxf(m, top);
+            const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
+            const float f = __builtin_amdgcn_exp2f(m - keep);
+            sum *= f;
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) o[c] *= f;
+            m = fresh;
+            mu = keep;
+        }
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+            V8 p[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][8 * u + e], a.scale_log2, -mu));
+                    sum += w[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[u][e] = static_cast<typename E::T>(w[e]);
+            }
+#pragma unroll
+            for (int lead = 0; lead < 2 * kTiles; lead += kAhead) {
+                u32x4 f[kAhead];
+#pragma unroll
+                for (int y = 0; y < kAhead; ++y) f[y] = values[buf][x][(lead + y) / 2][y % 2][lane];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int y = u; y < kAhead; y += 2)
+                        o[(lead + y) / 2] = E::mfma(__builtin_bit_cast(V8, f[y]), p[u], o[(lead + y) / 2]);
+            }
+        }
+    };
+
+    const int page_tiles_shift = t.page_shift - 5;
+    for (int base = 0; base < tiles; base += 64) {
+        const int tile = base + lane;
+        uint32_t at = 0, word = 0;
+        const int t0 = tile * kTile;
+        if (tile < tiles) {
+            const int page = t.page(b, tile >> page_tiles_shift);
+            if (page >= 0) {
+                word = t.word(b, tile);
+                if (hi_pos - t0 < 32) word &= (1u << (hi_pos - t0)) - 1u;
+                at = ((static_cast<uint32_t>(page) * t.kv_heads + h) << page_tiles_shift) +
+                     (tile & ((1 << page_tiles_shift) - 1));
+            }
+        }
+        // The same in every wave: tiles that every row sees whole, kPer a turn,
+        // then the others.
+        uint64_t whole = __ballot(word == 0xFFFFFFFFu && t0 + kTile <= first_see);
+        if (kPer == 2 && __popcll(whole) % 2 != 0) whole &= whole - 1;
+        const uint64_t part = __ballot(word != 0) & ~whole;
+        const auto run = [&](auto kind, uint64_t live) {
+            if (live == 0) return;
+            int i[kPer], next[kPer];
+            uint32_t mine[kPer], ahead[kPer];
+            // The next kPer tiles; past the last one it stands in, masked.
+            const auto take = [&](int (&to)[kPer], uint32_t (&filter)[kPer], int last) {
+#pragma unroll
+                for (int x = 0; x < kPer; ++x) {
+                    const bool some = live != 0;
+                    to[x] = some ? __builtin_ctzll(live) : last;
+                    live &= live - 1;
+                    last = to[x];
+                    filter[x] = some ? static_cast<uint32_t>(__builtin_amdgcn_readlane(word, to[x])) : 0u;
+                    request(x, __builtin_amdgcn_readlane(at, to[x]));
+                }
+            };
+            take(i, mine, 0);
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) convert(kind, x, 0, mine[x]);
+            bool more = live != 0;
+            if (more) take(next, ahead, i[kPer - 1]);
+            __syncthreads();
+            int buf = 0;
+            while (true) {
+                int from[kPer];
+                uint32_t now[kPer];
+#pragma unroll
+                for (int x = 0; x < kPer; ++x) {
+                    from[x] = __builtin_amdgcn_readlane(t0, i[x]);
+                    now[x] = mine[x];
+                }
+                const bool turn = more;
+                if (turn) {
+#pragma unroll
+                    for (int x = 0; x < kPer; ++x) {
+                        convert(kind, x, buf ^ 1, ahead[x]);
+                        i[x] = next[x];
+                        mine[x] = ahead[x];
+                    }
+                    more = live != 0;
+                    if (more) take(next, ahead, i[kPer - 1]);
+                }
+                multiply(kind, buf, from, now);
+                __syncthreads();
+                if (!turn) break;
+                buf ^= 1;
+            }
+        };
+        run(std::false_type{}, whole);
+        run(std::true_type{}, part);
+    }
+
+    sum += __shfl_xor(sum, 32);
+    if (!in) return;
+    uint16_t* const p = a.out.p + (q0 + token) * a.out.token_stride + head * a.out.head_stride;
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    // Rows 8 x + 4 g + y of O^T, y < 4, hold channels dim/32 (8 x + 4 g) ..
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int z = 0; z < kTiles / 2; ++z) {
+            u32x4 v;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int ch = 8 * z + 2 * y;
+                typename E::V2 e;
+                e[0] = static_cast<typename E::T>(o[ch % kTiles][4 * x + ch / kTiles] * inv);
+                e[1] = static_cast<typename E::T>(o[(ch + 1) % kTiles][4 * x + ch / kTiles] * inv);
+                v[y] = __builtin_bit_cast(uint32_t, e);
+            }
+            asm("" : "+v"(v));
+            store8(p + kTiles * (8 * x + 4 * g2) + 8 * z, v, a.out.wide);
+        }
+    if (a.lse != nullptr && g2 == 0)
+        a.lse[static_cast<int64_t>(q0 + token) * t.kv_heads * a.group + head] =
+            (m + __builtin_log2f(sum)) * 0.69314718055994531f;
 }
 
 // Joins the splits' partial results of one row: four waves a row, wave w the
@@ -626,32 +951,31 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
 // How a call is cut up, chosen on the host.
 struct AttendPlan {
     int nt;      // 16-row tiles a wave holds
-    int wt;      // waves that share a row tile's positions (4), or 1: a row tile each
+    bool wide;   // four row tiles a workgroup over the same positions
     dim3 grid, join;
 };
 
-// 16-row tiles of a wave that has a row tile to itself.
-template <int D>
-constexpr int kWideTiles = D == 256 ? 1 : 2;
+// Rows of a workgroup of kv_attention_wide_kernel.
+constexpr int kWideRows = 128;
 
 // One launch each; defined per element type and dim.
 template <class E, int D>
 void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
 {
-    if (p.wt == 1) {
-        kv_attention_kernel<E, D, kWideTiles<D>, 1><<<p.grid, 256, 0, stream>>>(a);
+    if (p.wide) {
+        kv_attention_wide_kernel<E, D><<<p.grid, 256, 0, stream>>>(a);
         return;
     }
-    if (p.nt == 1)
-        kv_attention_kernel<E, D, 1, 4><<<p.grid, 256, 0, stream>>>(a);
-    else
-        kv_attention_kernel<E, D, 2, 4><<<p.grid, 256, 0, stream>>>(a);
-    if (a.splits > 1 && a.arrived == nullptr) {
-        if (p.nt == 1)
-            kv_join_kernel<E, D, 1><<<p.join, 256, 0, stream>>>(a);
-        else
-            kv_join_kernel<E, D, 2><<<p.join, 256, 0, stream>>>(a);
+    const auto run = [&](auto nt) {
+        constexpr int kNt = decltype(nt)::value;
+        kv_attention_kernel<E, D, kNt><<<p.grid, 256, 0, stream>>>(a);
+        if (a.splits > 1 && a.arrived == nullptr)
+            kv_join_kernel<E, D, kNt><<<p.join, 256, 0, stream>>>(a);
+    };
+    if constexpr (D < 256) {
+        if (p.nt == 2) return run(std::integral_constant<int, 2>{});
     }
+    run(std::integral_constant<int, 1>{});
 }
 
 extern template void attend_launch<Bf16, 64>(const AttendArgs&, const AttendPlan&, hipStream_t);

@@ -51,19 +51,20 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         blocks != nullptr ? width * (cache->page_size / kTile)
                           : (static_cast<uint32_t>(a.batch.max_positions) + kTile - 1) / kTile;
     AttendPlan p{};
-    const int wide_rows = 16 * (dim == 256 ? kWideTiles<256> : kWideTiles<128>);
-    const uint64_t wide_items = (rows + 4 * wide_rows - 1) / (4 * wide_rows) * cache->kv_heads *
-                                batch->sequences;
-    if (blocks == nullptr && rows > 64 && wide_items >= static_cast<uint64_t>(ctx->compute_units)) {
-        p.wt = 1;
-        p.nt = wide_rows / 16;
+    const uint64_t wide_tiles = (rows + kWideRows - 1) / kWideRows;
+    if (blocks == nullptr && rows > 64 &&
+        wide_tiles * cache->kv_heads * batch->sequences >= static_cast<uint64_t>(ctx->compute_units)) {
+        p.wide = true;
         a.splits = 1;
         a.split_tiles = static_cast<int>(most_tiles);
-        a.row_tiles = static_cast<int>((rows + 4 * wide_rows - 1) / (4 * wide_rows));
+        a.row_tiles = static_cast<int>(wide_tiles > 0x7FFFFFFF ? 0x7FFFFFFF : wide_tiles);
         p.grid = dim3(cache->kv_heads, static_cast<uint32_t>(a.row_tiles), batch->sequences);
     } else {
-        p.wt = 4;
-        p.nt = rows <= 16 ? 1 : 2;
+        // Two 16-row tiles a wave past 16 rows: 32 rows of 128 channels over 8 x
+        // 30,000 positions, two heads, take 31.6 us, and 48 rows 39.  At 256
+        // channels they do not fit the registers: 119 us with spills, 65 as two
+        // tiles of 16.
+        p.nt = rows <= 16 || dim == 256 ? 1 : 2;
         const uint32_t per = 16 * p.nt;
         a.token_tiles = static_cast<int>((a.group + per - 1) / per);
         a.row_tiles = static_cast<int>(blocks != nullptr

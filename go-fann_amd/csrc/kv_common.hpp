@@ -15,6 +15,7 @@ namespace gofann {
 namespace kv {
 
 using f32x4 = float __attribute__((ext_vector_type(4)));
+using f32x16 = float __attribute__((ext_vector_type(16)));
 using i32x4 = int __attribute__((ext_vector_type(4)));
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
@@ -32,6 +33,10 @@ struct Bf16 {
     static __device__ f32x4 mfma(V8 a, V8 b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ f32x16 mfma(V8 a, V8 b, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
     // Byte SEL of `codes` as two elements times the power of two in bits 30:23
     // of `scale` (the conversion reads no other bit of it; exact).
@@ -51,6 +56,10 @@ struct F16 {
     static __device__ f32x4 mfma(V8 a, V8 b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ f32x16 mfma(V8 a, V8 b, f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
     template <int SEL>
     static __device__ uint32_t decode(uint32_t codes, uint32_t scale)
