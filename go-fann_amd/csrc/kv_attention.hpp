@@ -26,6 +26,8 @@ struct AttendArgs {
     int token_tiles;        // listed: row tiles of one token's heads
     int splits;
     int split_tiles;        // tiles of a split
+    int rows_over;          // sequences of at most so many rows are not this launch's,
+    int rows_upto;          // nor those of more than so many
 };
 
 // The rows of one row tile: rows [begin, end) of the sequence's flattened
@@ -49,6 +51,7 @@ __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int 
         t.begin = index * rows;
         t.end = n * a.group;
     }
+    if (n * a.group <= a.rows_over || n * a.group > a.rows_upto) t.end = t.begin;
     if (t.end > t.begin + rows) t.end = t.begin + rows;
     t.first_pos = len - n + t.begin / a.group;
     t.last_pos = len - n + (t.end - 1) / a.group;

@@ -5,6 +5,9 @@
 namespace gofann {
 namespace {
 
+// Rows up to which a sequence of a long-chunk launch is left to the other kernel.
+constexpr int kFewRows = 64;
+
 // Tiles of a split of `items` row tiles of at most `most` tiles: enough
 // workgroups that all of them are resident at once, at least one tile a wave,
 // and where sequences may differ in length at most 64, so that a long one does
@@ -45,59 +48,79 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
     a.width = static_cast<int>(width);
     const uint32_t dim = cache->dim;
     const uint32_t tokens = batch->query_offsets == nullptr ? 1 : batch->max_queries;
-    const uint64_t rows = blocks != nullptr ? static_cast<uint64_t>(a.group)
-                                            : static_cast<uint64_t>(tokens) * a.group;
     const uint32_t most_tiles =
         blocks != nullptr ? width * (cache->page_size / kTile)
                           : (static_cast<uint32_t>(a.batch.max_positions) + kTile - 1) / kTile;
-    AttendPlan p{};
-    const uint64_t wide_tiles = (rows + kWideRows - 1) / kWideRows;
-    if (blocks == nullptr && rows > 64 &&
-        wide_tiles * cache->kv_heads * batch->sequences >= static_cast<uint64_t>(ctx->compute_units)) {
+    const auto launch = [&](const AttendArgs& x, const AttendPlan& p) {
+        const bool bf = cache->elem == GOFANN_ELEM_BF16;
+        switch (dim) {
+            case 64: (bf ? attend_launch<Bf16, 64> : attend_launch<F16, 64>)(x, p, ctx->stream); break;
+            case 128: (bf ? attend_launch<Bf16, 128> : attend_launch<F16, 128>)(x, p, ctx->stream); break;
+            default: (bf ? attend_launch<Bf16, 256> : attend_launch<F16, 256>)(x, p, ctx->stream); break;
+        }
+    };
+    const char* const too_many = "kv_attention: too many tokens a sequence for one call";
+    uint64_t rows = blocks != nullptr ? static_cast<uint64_t>(a.group)
+                                      : static_cast<uint64_t>(tokens) * a.group;
+    a.rows_upto = 0x7FFFFFFF;
+
+    // Long chunks, where they fill the chip: by the rows that there are, not by
+    // sequences times the longest.  Sequences of few rows among them, such as
+    // the decoding ones of a mixed batch, would each keep a workgroup busy with
+    // all of their positions; they are left to the other kernel.
+    const uint64_t all_rows = static_cast<uint64_t>(batch->queries) * a.group;
+    if (blocks == nullptr && rows > kFewRows &&
+        all_rows / kWideRows * cache->kv_heads >= static_cast<uint64_t>(ctx->compute_units)) {
+        AttendPlan p{};
         p.wide = true;
+        const uint64_t row_tiles = (rows + kWideRows - 1) / kWideRows;
+        if (row_tiles > 65535) return ctx->fail(GOFANN_ERR_UNSUPPORTED, too_many);
         a.splits = 1;
         a.split_tiles = static_cast<int>(most_tiles);
-        a.row_tiles = static_cast<int>(wide_tiles > 0x7FFFFFFF ? 0x7FFFFFFF : wide_tiles);
-        p.grid = dim3(cache->kv_heads, static_cast<uint32_t>(a.row_tiles), batch->sequences);
-    } else {
-        // Two 16-row tiles a wave past 16 rows: 32 rows of 128 channels over 8 x
-        // 30,000 positions, two heads, take 31.6 us, and 48 rows 39.  At 256
-        // channels they do not fit the registers: 119 us with spills, 65 as two
-        // tiles of 16.
-        p.nt = rows <= 16 || dim == 256 ? 1 : 2;
-        const uint32_t per = 16 * p.nt;
-        a.token_tiles = static_cast<int>((a.group + per - 1) / per);
-        a.row_tiles = static_cast<int>(blocks != nullptr
-                                           ? static_cast<uint64_t>(tokens) * a.token_tiles
-                                           : (rows + per - 1) / per);
-        const uint64_t items = static_cast<uint64_t>(a.row_tiles) * cache->kv_heads * batch->sequences;
-        a.split_tiles = split_tiles(ctx, items, most_tiles, batch->sequences > 1);
-        a.splits = most_tiles > 0 ? static_cast<int>((most_tiles + a.split_tiles - 1) / a.split_tiles) : 1;
-        if (a.splits > 1) {
-            const uint64_t parts = items * static_cast<uint64_t>(a.splits) * per;
-            const size_t o_bytes = parts * dim * sizeof(float);
-            char* const w = static_cast<char*>(
-                ctx->workspace(Context::kScratchKv, o_bytes + parts * 2 * sizeof(float)));
-            if (w == nullptr) return GOFANN_ERR_NOMEM;
-            if (a.splits <= kJoinSplits) {
-                a.arrived = static_cast<uint32_t*>(ctx->zeroed(Context::kScratchKvArrived, items * 4));
-                if (a.arrived == nullptr) return GOFANN_ERR_NOMEM;
-            }
-            a.part_o = reinterpret_cast<float*>(w);
-            a.part_ml = reinterpret_cast<float*>(w + o_bytes);
+        a.row_tiles = static_cast<int>(row_tiles);
+        const bool mixed = static_cast<uint64_t>(batch->sequences) * tokens > batch->queries;
+        a.rows_over = mixed ? kFewRows : 0;
+        p.grid = dim3(cache->kv_heads, static_cast<uint32_t>(row_tiles), batch->sequences);
+        launch(a, p);
+        if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_attention: launch");
+        if (!mixed) return GOFANN_OK;
+        a.rows_over = 0;
+        a.rows_upto = kFewRows;
+        rows = kFewRows;
+    }
+
+    // Two 16-row tiles a wave past 16 rows: 32 rows of 128 channels over 8 x
+    // 30,000 positions, two heads, take 31.6 us, and 48 rows 39.  At 256
+    // channels they do not fit the registers: 119 us with spills, 65 as two
+    // tiles of 16.
+    AttendPlan p{};
+    p.nt = rows <= 16 || dim == 256 ? 1 : 2;
+    const uint32_t per = 16 * p.nt;
+    a.token_tiles = static_cast<int>((a.group + per - 1) / per);
+    const uint64_t row_tiles =
+        blocks != nullptr ? static_cast<uint64_t>(tokens) * a.token_tiles : (rows + per - 1) / per;
+    if (row_tiles > 65535) return ctx->fail(GOFANN_ERR_UNSUPPORTED, too_many);
+    a.row_tiles = static_cast<int>(row_tiles);
+    const uint64_t items = row_tiles * cache->kv_heads * batch->sequences;
+    a.split_tiles = split_tiles(ctx, items, most_tiles, batch->sequences > 1);
+    a.splits = most_tiles > 0 ? static_cast<int>((most_tiles + a.split_tiles - 1) / a.split_tiles) : 1;
+    if (a.splits > 1) {
+        const uint64_t parts = items * static_cast<uint64_t>(a.splits) * per;
+        const size_t o_bytes = parts * dim * sizeof(float);
+        char* const w = static_cast<char*>(
+            ctx->workspace(Context::kScratchKv, o_bytes + parts * 2 * sizeof(float)));
+        if (w == nullptr) return GOFANN_ERR_NOMEM;
+        if (a.splits <= kJoinSplits) {
+            a.arrived = static_cast<uint32_t*>(ctx->zeroed(Context::kScratchKvArrived, items * 4));
+            if (a.arrived == nullptr) return GOFANN_ERR_NOMEM;
         }
-        p.grid = dim3(cache->kv_heads * static_cast<uint32_t>(a.splits),
-                      static_cast<uint32_t>(a.row_tiles), batch->sequences);
-        p.join = dim3(cache->kv_heads * per, static_cast<uint32_t>(a.row_tiles), batch->sequences);
+        a.part_o = reinterpret_cast<float*>(w);
+        a.part_ml = reinterpret_cast<float*>(w + o_bytes);
     }
-    if (a.row_tiles > 65535)
-        return ctx->fail(GOFANN_ERR_UNSUPPORTED, "kv_attention: too many tokens a sequence for one call");
-    const bool bf = cache->elem == GOFANN_ELEM_BF16;
-    switch (dim) {
-        case 64: (bf ? attend_launch<Bf16, 64> : attend_launch<F16, 64>)(a, p, ctx->stream); break;
-        case 128: (bf ? attend_launch<Bf16, 128> : attend_launch<F16, 128>)(a, p, ctx->stream); break;
-        default: (bf ? attend_launch<Bf16, 256> : attend_launch<F16, 256>)(a, p, ctx->stream); break;
-    }
+    p.grid = dim3(cache->kv_heads * static_cast<uint32_t>(a.splits), static_cast<uint32_t>(row_tiles),
+                  batch->sequences);
+    p.join = dim3(cache->kv_heads * per, static_cast<uint32_t>(row_tiles), batch->sequences);
+    launch(a, p);
     if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_attention: launch");
     return GOFANN_OK;
 }

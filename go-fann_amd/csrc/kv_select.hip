@@ -9,6 +9,7 @@ namespace kv {
 namespace {
 
 constexpr int kChunk = 256;                   // blocks that a workgroup scores: 16 tiles of 16
+constexpr int kRepeat = 4;                    // token tiles that a workgroup scores in turn
 constexpr int kBins = 2048;
 constexpr uint32_t kForced = 0xFFFFFFFFu;     // above every score's key
 constexpr uint32_t kIneligible = 0;           // below every score's key
@@ -20,7 +21,7 @@ struct SelectArgs {
     const uint8_t* box_scale;
     uint32_t* keys;     // [queries][kv_heads][key_stride], where a row has several chunks
     int64_t key_stride;
-    uint32_t* arrived;  // [item], zero between calls: chunks scored
+    uint32_t* arrived;  // [item], zero between calls: chunks scored; NULL: kv_pick_kernel picks
     int32_t* out;
     int group;        // heads a key/value head
     int group_shift;  // log2 of the rows a token's heads take of a 16-row tile
@@ -245,20 +246,34 @@ __device__ void pick(const SelectArgs& a, PickShared& sh, int blocks, int32_t* o
     for (uint32_t j = total + tid; j < static_cast<uint32_t>(a.width); j += 256) out[j] = -1;
 }
 
-// Scores of 256 blocks for a tile of tokens; the last workgroup of a tile to
-// finish picks.  The rows of an i8 product are a token's heads (each token
+// The same from the keys that the scores left in memory.
+__device__ void pick_row(const SelectArgs& a, PickShared& sh, int blocks, int64_t row)
+{
+    const uint32_t* const keys = a.keys + row * a.key_stride;
+    if (blocks <= 2048)
+        pick<8>(a, sh, blocks, a.out + row * a.width, [&](int j) { return get(keys + j); });
+    else
+        pick<16>(a, sh, blocks, a.out + row * a.width, [&](int j) { return get(keys + j); });
+}
+
+// Scores of 256 blocks for a tile of tokens, or several: one token a sequence
+// is picked for by the last workgroup to finish, more by a launch of their own,
+// a workgroup each, so that a workgroup here may score one tile of tokens after
+// the other against the same boxes (2 x 300 tokens, 4 heads, up to 625 blocks:
+// 50 us with the last workgroup picking for two tokens in turn, 33 so).  The rows of an i8 product are a token's heads (each token
 // padded to a power of two of rows by repeating its last head, which changes
 // no maximum), the columns blocks: a lane then holds four heads of one block,
 // and the maximum over a token's heads stays in the lane and its neighbours
 // 16 and 32 lanes away.  sum_c max(q most, q least) is one product of length
 // 2 dim, of the positive part of q with `most` and the negative with `least`.
 // kQuads: a token has at least four rows, so a lane's four are one token's.
-template <class E, int D, bool kQuads>
+// kMany: more than one token a sequence.
+template <class E, int D, bool kQuads, bool kMany>
 __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(SelectArgs a)
 {
     constexpr int K = D / 64;               // products of 64 channels
     constexpr int kBatch = D == 256 ? 2 : 4;  // 16-block tiles requested at once
-    __shared__ uint32_t stage[4 * kChunk];  // the keys of up to four tokens, where one chunk is all
+    __shared__ uint32_t stage[kChunk];  // the keys, where one chunk is all
     __shared__ PickShared sh;
     __shared__ int is_last;
     const Batch& t = a.batch;
@@ -275,21 +290,23 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
     const int rows_shift = a.group_shift;  // rows a token takes: 1 << rows_shift
-    const int i0 = blockIdx.y * a.tokens;
-    if (i0 >= n) return;
-    const int i_end = i0 + a.tokens < n ? i0 + a.tokens : n;
-    const int blocks = blocks_to(t, position(len, n, i_end - 1));
+    const int per = kMany ? a.tokens * kRepeat : 1;
+    const int first_token = kMany ? blockIdx.y * per : 0;
+    if (first_token >= n) return;
+    const int stop = first_token + per < n ? first_token + per : n;
+    const int blocks = blocks_to(t, position(len, n, stop - 1));
     const int chunks = (blocks + kChunk - 1) / kChunk;
     if (chunk > 0 && chunk >= chunks) return;
+    const bool whole = !kMany && chunks <= 1;  // all keys of the row are here
 
     // Positive and negative part of the quantized queries, 16 channels a lane
     // and product; the rows' powers of two.
     i32x4 qp[K], qn[K];
     float unit[4];
     uint32_t raw[K][8];
-    const auto request_queries = [&](int ht) {
+    const auto request_queries = [&](int i0, int ht) {
         int i = i0 + (r16 >> rows_shift);
-        i = i < i_end ? i : i_end - 1;
+        i = i < stop ? i : stop - 1;
         int head = 16 * ht + (r16 & ((1 << rows_shift) - 1));
         head = head < a.group ? head : a.group - 1;
         const uint16_t* const row = a.q.p + (q0 + i) * a.q.token_stride +
@@ -384,7 +401,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
         }
         // The queries are requested between the pages and the boxes, so that
         // they are quantized while the boxes are on their way.
-        if (batch == 0) request_queries(0);
+        if (batch == 0) request_queries(first_token, 0);
 #pragma unroll
         for (int x = 0; x < kBatch; ++x) {
             const int64_t ph = static_cast<int64_t>(page[x] < 0 ? 0 : page[x]) * t.kv_heads + h;
@@ -397,61 +414,66 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
             }
             eb[x] = in ? __builtin_bit_cast(float, static_cast<uint32_t>(a.box_scale[ph]) << 23) : 0.0f;
         }
-        float s[kBatch][4];
-        for (int ht = 0; ht < a.head_tiles; ++ht) {
-            if (ht > 0 || (batch > 0 && a.head_tiles > 1)) request_queries(ht);
-            if (batch == 0 || a.head_tiles > 1) quantize_queries();
+        for (int i0 = first_token; i0 < stop; i0 += kMany ? a.tokens : 1) {
+            const int i_end = !kMany || i0 + a.tokens > stop ? stop : i0 + a.tokens;
+            float s[kBatch][4];
+            for (int ht = 0; ht < a.head_tiles; ++ht) {
+                const bool others = kMany || a.head_tiles > 1;  // than the queries held
+                if (ht > 0 || i0 > first_token || (batch > 0 && others)) request_queries(i0, ht);
+                if (batch == 0 || others) quantize_queries();
 #pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-                i32x4 acc = {0, 0, 0, 0};
+                for (int x = 0; x < kBatch; ++x) {
+                    i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qp[k], hi[x][k], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qn[k], lo[x][k], acc, 0, 0, 0);
-                }
-                // |acc| < 2^23, so the conversion and both products are exact
-                // wherever the result is a normal number.
+                    for (int k = 0; k < K; ++k) {
+                        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qp[k], hi[x][k], acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qn[k], lo[x][k], acc, 0, 0, 0);
+                    }
+                    // |acc| < 2^23, so the conversion and both products are exact
+                    // wherever the result is a normal number.
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = static_cast<float>(acc[i]) * unit[i] * eb[x];
-                    s[x][i] = ht == 0 ? f : fmaxf(s[x][i], f);
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = static_cast<float>(acc[i]) * unit[i] * eb[x];
+                        s[x][i] = ht == 0 ? f : fmaxf(s[x][i], f);
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            // Maximum over a token's rows.
-            const int block = chunk * kChunk + 16 * (wave + 4 * (batch * kBatch + x)) + r16;
-            const auto write = [&](int first_row, float score) {
-                const int token = i0 + (first_row >> rows_shift);
-                if (token >= i_end) return;
-                const int pos = position(len, n, token);
-                const int mine = blocks_to(t, pos);
-                uint32_t key = kIneligible;
-                if (block < mine && page[x] >= 0 && any_visible(t, b, block, pos)) {
-                    const uint32_t u = __builtin_bit_cast(uint32_t, score + 0.0f);  // -0 as 0
-                    key = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-                    if (block < a.first || block >= mine - a.last) key = kForced;
+            for (int x = 0; x < kBatch; ++x) {
+                // Maximum over a token's rows.
+                const int block = chunk * kChunk + 16 * (wave + 4 * (batch * kBatch + x)) + r16;
+                const auto write = [&](int first_row, float score) {
+                    const int token = i0 + (first_row >> rows_shift);
+                    if (token >= i_end) return;
+                    const int pos = position(len, n, token);
+                    const int mine = blocks_to(t, pos);
+                    uint32_t key = kIneligible;
+                    if (block < mine && page[x] >= 0 && any_visible(t, b, block, pos)) {
+                        const uint32_t u = __builtin_bit_cast(uint32_t, score + 0.0f);  // -0 as 0
+                        key = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+                        if (block < a.first || block >= mine - a.last) key = kForced;
+                    }
+                    if (whole)
+                        stage[block] = key;
+                    else if (block < mine)
+                        put(a.keys + (row0 + static_cast<int64_t>(token) * t.kv_heads) * a.key_stride + block,
+                            key);
+                };
+                if constexpr (kQuads) {
+                    float m = fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3]));
+                    if (rows_shift >= 3) m = fmaxf(m, __shfl_xor(m, 16));
+                    if (rows_shift >= 4) m = fmaxf(m, __shfl_xor(m, 32));
+                    if ((4 * g4 & ((1 << rows_shift) - 1)) == 0) write(4 * g4, m);
+                } else if (rows_shift == 1) {
+                    write(4 * g4, fmaxf(s[x][0], s[x][1]));
+                    write(4 * g4 + 2, fmaxf(s[x][2], s[x][3]));
+                } else {
+                    for (int i = 0; i < 4; ++i) write(4 * g4 + i, s[x][i]);
                 }
-                if (chunks <= 1)
-                    stage[(token - i0) * kChunk + block] = key;
-                else if (block < mine)
-                    put(a.keys + (row0 + static_cast<int64_t>(token) * t.kv_heads) * a.key_stride + block,
-                        key);
-            };
-            if constexpr (kQuads) {
-                float m = fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3]));
-                if (rows_shift >= 3) m = fmaxf(m, __shfl_xor(m, 16));
-                if (rows_shift >= 4) m = fmaxf(m, __shfl_xor(m, 32));
-                if ((4 * g4 & ((1 << rows_shift) - 1)) == 0) write(4 * g4, m);
-            } else if (rows_shift == 1) {
-                write(4 * g4, fmaxf(s[x][0], s[x][1]));
-                write(4 * g4 + 2, fmaxf(s[x][2], s[x][3]));
-            } else {
-                for (int i = 0; i < 4; ++i) write(4 * g4 + i, s[x][i]);
             }
         }
     }
+    if constexpr (kMany) return;
     if (chunks > 1) {
         // The keys are atomics of the whole device, so that their completion
         // is all that the count has to wait for.
@@ -470,39 +492,41 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
     } else {
         __syncthreads();
     }
-    for (int token = i0; token < i_end; ++token) {
-        const int64_t row = row0 + static_cast<int64_t>(token) * t.kv_heads;
-        const int mine = blocks_to(t, position(len, n, token));
-        int32_t* const out = a.out + row * a.width;
-        if (token > i0) __syncthreads();
-        if (chunks <= 1) {
-            const uint32_t* const keys = stage + (token - i0) * kChunk;
-            pick<1>(a, sh, mine, out, [&](int j) { return keys[j]; });
-        } else {
-            const uint32_t* const keys = a.keys + row * a.key_stride;
-            if (mine <= 2048)
-                pick<8>(a, sh, mine, out, [&](int j) { return get(keys + j); });
-            else
-                pick<16>(a, sh, mine, out, [&](int j) { return get(keys + j); });
-        }
-    }
+    const int mine = blocks_to(t, position(len, n, 0));
+    if (whole)
+        pick<1>(a, sh, mine, a.out + row0 * a.width, [&](int j) { return stage[j]; });
+    else
+        pick_row(a, sh, mine, row0);
+}
+
+// One token and key/value head a workgroup.
+__global__ __launch_bounds__(256) void kv_pick_kernel(SelectArgs a)
+{
+    __shared__ PickShared sh;
+    const Batch& t = a.batch;
+    const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
+    const int len = t.length(b);
+    const int q0 = t.first_query(b);
+    const int n = t.new_tokens(b, q0);
+    if (i >= n) return;
+    pick_row(a, sh, blocks_to(t, position(len, n, i)), static_cast<int64_t>(q0 + i) * t.kv_heads + h);
 }
 
 template <class E>
-void launch(const SelectArgs& a, uint32_t dim, dim3 grid, hipStream_t stream)
+void launch(const SelectArgs& a, uint32_t dim, bool many, dim3 grid, hipStream_t stream)
 {
-    const auto run = [&](auto quads) {
-        constexpr bool kQuads = decltype(quads)::value;
+    const auto run = [&](auto quads, auto many) {
+        constexpr bool kQuads = decltype(quads)::value, kMany = decltype(many)::value;
         switch (dim) {
-            case 64: kv_select_kernel<E, 64, kQuads><<<grid, 256, 0, stream>>>(a); break;
-            case 128: kv_select_kernel<E, 128, kQuads><<<grid, 256, 0, stream>>>(a); break;
-            default: kv_select_kernel<E, 256, kQuads><<<grid, 256, 0, stream>>>(a); break;
+            case 64: kv_select_kernel<E, 64, kQuads, kMany><<<grid, 256, 0, stream>>>(a); break;
+            case 128: kv_select_kernel<E, 128, kQuads, kMany><<<grid, 256, 0, stream>>>(a); break;
+            default: kv_select_kernel<E, 256, kQuads, kMany><<<grid, 256, 0, stream>>>(a); break;
         }
     };
     if (a.group_shift >= 2)
-        run(std::true_type{});
+        many ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
     else
-        run(std::false_type{});
+        many ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
 }
 
 }  // namespace
@@ -522,35 +546,40 @@ int kv_select(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch*
     a.group = static_cast<int>(heads / cache->kv_heads);
     while ((1 << a.group_shift) < a.group && a.group_shift < 4) ++a.group_shift;
     a.head_tiles = (a.group + 15) / 16;
-    // At most four tokens a tile: its last workgroup picks for them in turn.
+    // At most four tokens a tile and its own picks.
     a.tokens = 16 >> a.group_shift;
     if (a.tokens > 4) a.tokens = 4;
     a.width = static_cast<int>(width);
     a.first = static_cast<int>(first);
     a.last = static_cast<int>(last);
     const uint32_t tokens = batch->query_offsets == nullptr ? 1 : batch->max_queries;
-    a.token_tiles = static_cast<int>((tokens + a.tokens - 1) / a.tokens);
-    if (a.token_tiles > 65535)
-        return ctx->fail(GOFANN_ERR_UNSUPPORTED, "kv_select: too many tokens a sequence for one call");
+    if (tokens > 65535)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, "kv_select: at most 65535 tokens a sequence");
+    const uint32_t per = tokens > 1 ? static_cast<uint32_t>(a.tokens * kRepeat) : 1u;
+    a.token_tiles = static_cast<int>((tokens + per - 1) / per);
     const uint32_t most = static_cast<uint32_t>(a.batch.max_positions);
     const uint32_t blocks = (most + cache->page_size - 1) / cache->page_size;
     const uint32_t chunks = blocks > 0 ? (blocks + kChunk - 1) / kChunk : 1;
-    if (chunks > 1) {
+    if (chunks > 1 || tokens > 1) {
         a.key_stride = blocks;
         a.keys = static_cast<uint32_t*>(
             ctx->workspace(Context::kScratchKv,
-                           static_cast<size_t>(batch->queries) * cache->kv_heads * a.key_stride * 4));
+                           static_cast<size_t>(batch->queries) * cache->kv_heads * (blocks + 1) * 4));
         if (a.keys == nullptr) return GOFANN_ERR_NOMEM;
+    }
+    if (chunks > 1 && tokens == 1) {
         a.arrived = static_cast<uint32_t*>(
-            ctx->zeroed(Context::kScratchKvArrived, static_cast<size_t>(batch->sequences) *
-                                                        a.token_tiles * cache->kv_heads * 4));
+            ctx->zeroed(Context::kScratchKvArrived,
+                        static_cast<size_t>(batch->sequences) * cache->kv_heads * 4));
         if (a.arrived == nullptr) return GOFANN_ERR_NOMEM;
     }
     const dim3 grid(chunks * cache->kv_heads, static_cast<uint32_t>(a.token_tiles), batch->sequences);
     if (cache->elem == GOFANN_ELEM_BF16)
-        launch<Bf16>(a, cache->dim, grid, ctx->stream);
+        launch<Bf16>(a, cache->dim, tokens > 1, grid, ctx->stream);
     else
-        launch<F16>(a, cache->dim, grid, ctx->stream);
+        launch<F16>(a, cache->dim, tokens > 1, grid, ctx->stream);
+    if (tokens > 1)
+        kv_pick_kernel<<<dim3(cache->kv_heads, tokens, batch->sequences), 256, 0, ctx->stream>>>(a);
     if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_select: launch");
     return GOFANN_OK;
 }

@@ -305,6 +305,33 @@ def test_attend_of_long_chunks(ctx, elem, dim, group, heads):
     check_attend(out[pick], lse[pick], *want)
 
 
+def test_attend_of_a_mixed_batch(ctx):
+    """Long chunks that fill the chip beside sequences of one and of a few tokens."""
+    new = [2100, 1, 5, 2049, 0, 17]
+    lens = [2100, 300, 5, 2060, 90, 400]
+    heads, group, dim = 8, 2, 64
+    b = ref.Batch(32, lens, new, seed=9)
+    c = ref.Cache(b.pages, heads, 32, dim, "bf16", seed=1)
+    r = np.random.default_rng(4)
+    for name in ("k_codes", "v_codes"):
+        getattr(c, name)[:] = r.integers(0, 256, getattr(c, name).shape)
+    for name in ("k_scales", "v_scales"):
+        getattr(c, name)[:] = r.integers(124, 128, getattr(c, name).shape)
+    q, q64 = rows(r, b.queries, heads * group, dim, "bf16")
+    d = device_cache(ctx, c)
+    lse = torch.full((b.queries, heads * group), 7.0, device="cuda")
+    out = torch.full_like(q, 99.0)
+    d.attend(device_batch(b), q, out=out, lse=lse)
+    tok = {row: (s, p) for row, s, p in b.tokens()}
+    pick = [0, 1, 2099, 2100, 2101, 2105, 2106, 2107, 3000, 4154, 4155, 4160, 4171]
+    sub = ref.Batch(32, [tok[i][1] + 1 for i in pick], [1] * len(pick), pages=b.pages)
+    sub.table = np.stack([b.table[tok[i][0]] for i in pick])
+    sub.width = b.width
+    want = ref.attend(c, sub, q64[pick], dim ** -0.5)
+    check_attend(out[pick], lse[pick], *want)
+    assert (out != 99.0).any(-1).all() and (lse != 7.0).all()
+
+
 def test_attend_scores_far_apart(ctx):
     """A maximum that grows along the sequence, and scores that underflow against it."""
     b = ref.Batch(64, [640], [1], seed=1)
