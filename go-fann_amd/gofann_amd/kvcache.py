@@ -158,7 +158,11 @@ class KvCache:
     # -- checks ----------------------------------------------------------
     def _rows(self, name: str, t: torch.Tensor, queries: int, heads: int | None,
               written: bool = False) -> _lib.KvRows:
-        shape, (st, sh, sd) = t.shape, t.stride() if t.dim() == 3 else (0, 0, 0)
+        shape = t.shape
+        if shape == (queries, heads, self.dim) and t.dtype is self.dtype and \
+                t.is_contiguous() and t.device == self.device:
+            return _lib.KvRows(t.data_ptr(), heads * self.dim, self.dim)
+        st, sh, sd = t.stride() if t.dim() == 3 else (0, 0, 0)
         if len(shape) != 3 or shape[0] != queries or shape[2] != self.dim or \
                 (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [{queries}][{heads if heads is not None else 'heads'}]"
@@ -202,7 +206,7 @@ class KvCache:
         last ones, then those whose boxes score highest against any of the
         group's queries."""
         self._ready(batch)
-        rq = self._rows("q", q, batch.queries, None)
+        rq = self._rows("q", q, batch.queries, q.shape[1] if q.dim() == 3 else None)
         shape = (batch.queries, self.kv_heads, width)
         if out is None:
             out = torch.empty(shape, dtype=torch.int32, device=self.device)
@@ -222,8 +226,8 @@ class KvCache:
         by default.  lse [queries][heads] f32 gets the log of the sums of
         exponentials.  A row with nothing to read is zero (lse -inf)."""
         self._ready(batch)
-        rq = self._rows("q", q, batch.queries, None)
-        heads = q.shape[1]
+        heads = q.shape[1] if q.dim() == 3 else None
+        rq = self._rows("q", q, batch.queries, heads)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
             ro = _lib.KvRows(out.data_ptr(), heads * self.dim, self.dim)
