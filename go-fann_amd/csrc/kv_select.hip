@@ -266,6 +266,11 @@ __device__ void pick_row(const SelectArgs& a, PickShared& sh, int blocks, int64_
 // and the maximum over a token's heads stays in the lane and its neighbours
 // 16 and 32 lanes away.  sum_c max(q most, q least) is one product of length
 // 2 dim, of the positive part of q with `most` and the negative with `least`.
+//
+// 16 sequences of 20,000 to 131,000 positions, 8 heads (38 MB of boxes): 18.4
+// us, 2.1 TB/s.  One long row after the other, latency bounds it: of 12.5 us for
+// one sequence 7.8 are the chain from its length over pages and queries to
+// the boxes and keys, 0.5 the count of arrivals, 4.2 the choice.
 // kQuads: a token has at least four rows, so a lane's four are one token's.
 // kMany: more than one token a sequence.
 template <class E, int D, bool kQuads, bool kMany>

@@ -574,6 +574,41 @@ def test_workspace_too_small_under_capture_is_an_error(gpu_ctx):
     own.close()
 
 
+def test_session_of_the_example(ctx, capsys):
+    """Prompt in chunks, then steps, against one attention over all of it."""
+    from gofann_amd import longcontext
+    r = np.random.default_rng(6)
+    s = longcontext.Session(ctx, sequences=2, capacity=200, kv_heads=2, dim=64, page=32)
+    c = ref.Cache(14, 2, 32, 64, "bf16")
+    at, last = 0, None
+    s.hide(1, 32, 96)
+    for tokens, width in ((70, 0), (50, 7), (1, 0), (1, 3)):
+        q, q64 = rows(r, 2 * tokens, 8, 64, "bf16")
+        k, k64 = rows(r, 2 * tokens, 2, 64, "bf16")
+        v, v64 = rows(r, 2 * tokens, 2, 64, "bf16")
+        out = s.step(q, k, v, width)
+        for b in range(2):
+            for i in range(tokens):
+                pos = at + i
+                c.write(7 * b + pos // 32, pos % 32, k64[b * tokens + i], v64[b * tokens + i])
+        at += tokens
+        b = ref.Batch(32, [at, at], [tokens, tokens], pages=14,
+                      visible=lambda i, n, _: ~((i == 1) & (np.arange(n) >= 32) & (np.arange(n) < 96)))
+        b.table = np.arange(14, dtype=np.int32).reshape(2, 7)
+        b.width = 7
+        for j in range(14):
+            n = min(32, at - 32 * (j % 7))
+            if n > 0:
+                c.renew_box(j, n)
+        blocks = ref.select(c, b, q64, width, 1, 2) if width else None
+        want = ref.attend(c, b, q64, 64 ** -0.5, blocks)
+        check_attend(out, None, want[0], None, want[2])
+    with pytest.raises(ValueError):
+        s.grow(100)
+    longcontext.main(["--context", "1500", "--steps", "2", "--sequences", "2", "--width", "8"])
+    assert "8 blocks a token" in capsys.readouterr().out
+
+
 # ---- refusals ----------------------------------------------------------------
 
 def test_refusals_at_the_c_entry(ctx):
