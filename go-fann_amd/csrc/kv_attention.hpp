@@ -197,8 +197,8 @@ struct Raw {
 // the positions fill the chip where there are few rows.  HBM bounds long calls:
 // one token of 64 heads over 500,001 positions (544 MB) takes 100 us, 5.4 TB/s
 // (a large copy: 4.8), and 11 us for the join of 96 splits.  At 126 registers
-// four workgroups are resident a CU; at three, sequences of 500 to 16,000
-// positions took 9% longer.  Short calls are a chain of dependent loads: 8.6 us
+// four workgroups are resident a CU; with three, and masked tiles not yet loaded
+// ahead, sequences of 500 to 16,000 positions took 9% longer.  Short calls are a chain of dependent loads: 8.6 us
 // for 1,999 positions of 8 heads.
 template <class E, int D, int NT>
 __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention_kernel(AttendArgs a)
@@ -550,11 +550,11 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
 //
 // 2,048 tokens of 32 heads over 16,390 positions, 516 GFLOP: 0.52 to 0.63 ms by
 // the chip's clock, 990 to 820 TFLOP/s, 0.72 to 0.60 of what a large matrix
-// product of the library reaches.  The
-// chip's power bounds it: half of the workgroups on half of the CUs run 1.65
-// times as fast each, and one or two tiles a turn, or scores formed a turn
-// ahead of their softmax, end within 3% of each other.  Without LDS, each wave
-// converting for itself (16 x 16 products): 0.69 ms.
+// product of the library reaches.  The chip's power seems to bound it: with 64
+// rows a wave, one workgroup a CU, 256 workgroups took 700 us each and 128 of
+// the same 322; and one or two tiles a turn, or scores formed a turn ahead of
+// their softmax, end within 3% of each other.  Without LDS, each wave
+// converting for itself (16 x 16 products): 0.69 ms where this took 0.63.
 template <class E, int D>
 __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
 {
