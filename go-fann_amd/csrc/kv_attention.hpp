@@ -17,7 +17,7 @@ struct AttendArgs {
     const int32_t* blocks;  // [queries][kv_heads][width] or NULL
     float* lse;             // [queries][heads] or NULL
     float* part_o;          // [item][split][rows][dim], splits > 1
-    float* part_ml;         // [item][split][rows][2]: running maximum, sum
+    float* part_ml;         // [item][split][rows][2]: reference, sum
     uint32_t* arrived;      // [item], zero between calls: splits done; NULL: kv_join_kernel joins
     float scale_log2;       // scale * log2(e)
     int group;              // heads a key/value head
@@ -59,7 +59,9 @@ __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int 
 }
 
 // How far, in powers of two, a score may pass the running maximum before that
-// is renewed.
+// is renewed.  The reference m that weights are taken against lies E::kRaise
+// below it, so weights reach 2^(kSlack + kRaise): with 0 for bf16 and 7 for f16,
+// whose weights would otherwise lose, below 2^-25, a tail of many small ones.
 constexpr float kSlack = 8.0f;
 
 // Splits up to which the last workgroup of an item to finish joins them
@@ -129,12 +131,12 @@ __device__ __forceinline__ void mask_scores(f32x4 (&s)[2], uint32_t mine, int le
     for (int e = 0; e < 8; ++e) s[e / 4][e % 4] = (ok >> e & 1u) ? s[e / 4][e % 4] : -__builtin_inff();
 }
 
-// Weights 2^(score - m) of a row's scores, the row's running maximum m, sum of
+// Weights 2^(score - m) of a row's scores, the row's reference m, sum of
 // weights and weighted values o brought along; mu is m, or 0 while there is
-// none.  The maximum is renewed only where a score passes it by more than
-// kSlack (in powers of two): until then the weights are at most 2^kSlack, which
-// costs 32-bit sums nothing.  The weights enter the product in 16 bits, as the
-// values do; their sum stays in 32.
+// none.  The reference is renewed only where a score passes the maximum it was
+// made from by more than kSlack (in powers of two): until then the weights are
+// at most 2^(kSlack + kRaise), which costs 32-bit sums nothing.  The weights
+// enter the product in 16 bits, as the values do; their sum stays in 32.
 template <class E, int kUnit>
 __device__ __forceinline__ typename E::V8 weigh(const f32x4 (&s)[2], float scale_log2, float& m,
                                                 float& mu, float& sum, f32x4 (&o)[kUnit])
@@ -143,10 +145,10 @@ __device__ __forceinline__ typename E::V8 weigh(const f32x4 (&s)[2], float scale
 #pragma unroll
     for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e / 4][e % 4]);
     top *= scale_log2;
-    if (__any(top > m + kSlack)) {
+    if (__any(top > m + (kSlack + E::kRaise))) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float fresh = fmaxf(m, top);
+        const float fresh = fmaxf(m, top - E::kRaise);
         const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
         const float f = __builtin_amdgcn_exp2f(m - keep);
         sum *= f;
@@ -743,9 +745,9 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
         top *= a.scale_log2;
-        if (__any(top > m + kSlack)) {
+        if (__any(top > m + (kSlack + E::kRaise))) {
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float fresh = fmaxf(m, top);
+            const float fresh = fmaxf(m, top - E::kRaise);
             const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
             const float f = __builtin_amdgcn_exp2f(m - keep);
             sum *= f;

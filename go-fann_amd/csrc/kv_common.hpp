@@ -30,6 +30,7 @@ struct Bf16 {
     using V2 = __bf16 __attribute__((ext_vector_type(2)));
     using V8 = __bf16 __attribute__((ext_vector_type(8)));
     static constexpr int kMinExp = -125, kMaxExp = 125;  // a group's exponents
+    static constexpr float kRaise = 0.0f;  // of attention weights, in powers of two
     static __device__ f32x4 mfma(V8 a, V8 b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -53,6 +54,7 @@ struct F16 {
     using V8 = _Float16 __attribute__((ext_vector_type(8)));
     // Every code times 2^e in this range is a finite f16, without rounding.
     static constexpr int kMinExp = -23, kMaxExp = 13;
+    static constexpr float kRaise = 7.0f;
     static __device__ f32x4 mfma(V8 a, V8 b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);

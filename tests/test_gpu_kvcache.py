@@ -348,6 +348,38 @@ def test_attend_scores_far_apart(ctx):
     check_attend(device_cache(ctx, c).attend(device_batch(b), q.cuda(), scale=1.0, lse=lse), lse, *want)
 
 
+@pytest.mark.parametrize("heads,group,new", [(1, 3, 1), (1, 3, 9), (8, 4, 1024)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_attend_f16_keeps_a_tail_of_small_weights(ctx, dim, heads, group, new):
+    """One position's weight of 1 over thousands of 2^-25.5, which f16 alone would
+    round to nothing: the small ones have all of the values, so their sum is the
+    result.  In one launch, in splits and in long chunks."""
+    n = 3000 + new
+    b = ref.Batch(64, [n], [new], seed=3)
+    c = ref.Cache(b.pages, heads, 64, dim, "f16")
+    c.k_scales[:], c.v_scales[:], c.k_codes[:] = 127, 127, 0
+    c.v_codes[:] = 0x77                                  # 6, 6
+    pid = b.table[0, 10 // 64]
+    c.k_codes[pid, :, 10, 0] = 7                         # a key of (6, 0, ..), its value 0
+    c.v_codes[pid, :, 10 // 8, :, 10 % 8] = 0
+    x = torch.tensor(25.5 * np.log(2.0) / 6, dtype=torch.float16)
+    q = torch.zeros(new, heads * group, dim, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = x
+    w = np.exp(-6.0 * float(x))
+    many = n - new + np.arange(new, dtype=np.float64)    # small ones of each token
+    z = 1 + many * w
+    want = 6 * many * w / z
+    lse = torch.empty(new, heads * group, device="cuda")
+    out = device_cache(ctx, c).attend(device_batch(b), q, scale=1.0, lse=lse)
+    # A weight is off by 2^-25 of at least 2^7 at the maximum, the result by half
+    # an f16 unit; sums in 32 bits by 2^-24 a term, exponentials by 2^-21 of 18.
+    bound = 2.0 ** -32 * 6 * many + 2.0 ** -25 + want * (2.0 ** -11 + (n + 64) * 2.0 ** -24 + 2.0 ** -16)
+    off = np.abs(out.double().cpu().numpy() - want[:, None, None])
+    assert (off <= bound[:, None, None]).all(), (off / bound[:, None, None]).max()
+    got = lse.double().cpu().numpy()
+    assert np.abs(got - (6.0 * float(x) + np.log(z))[:, None]).max() < 1e-4
+
+
 def test_attend_infinite_and_nan_queries_stay_in_their_rows(ctx):
     b = ref.Batch(64, [100, 70], [1, 1], seed=1)
     c = ref.Cache(b.pages, 1, 64, 128, "bf16", seed=1)
