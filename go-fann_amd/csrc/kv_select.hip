@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
     // Positive and negative part of the quantized queries, 16 channels a lane
     // and product; the rows' powers of two.
     i32x4 qp[K], qn[K];
-    float unit[4];
+    int unit[4];
     uint32_t raw[K][8];
     const auto request_queries = [&](int i0, int ht) {
         int i = i0 + (r16 >> rows_shift);
@@ -387,16 +387,15 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
                 qp[k][w] = static_cast<int>(x & ~mask);
                 qn[k][w] = static_cast<int>(x & mask);
             }
-        const float mine = __builtin_bit_cast(float, static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) unit[i4] = __shfl(mine, 4 * g4 + i4);
+        for (int i4 = 0; i4 < 4; ++i4) unit[i4] = __shfl(e, 4 * g4 + i4);
     };
 
     const int64_t row0 = static_cast<int64_t>(q0) * t.kv_heads + h;  // row of token i: + i kv_heads
     // Tiles of the chunk: wave w has w, w + 4, w + 8, w + 12.
     for (int batch = 0; batch < 4 / kBatch; ++batch) {
         int page[kBatch];
-        float eb[kBatch];
+        int eb[kBatch];
         i32x4 hi[kBatch][K], lo[kBatch][K];
 #pragma unroll
         for (int x = 0; x < kBatch; ++x) {
@@ -417,7 +416,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
                 hi[x][k] = in ? *reinterpret_cast<const i32x4*>(p + 64 * k) : i32x4{0, 0, 0, 0};
                 lo[x][k] = in ? *reinterpret_cast<const i32x4*>(p + D + 64 * k) : i32x4{0, 0, 0, 0};
             }
-            eb[x] = in ? __builtin_bit_cast(float, static_cast<uint32_t>(a.box_scale[ph]) << 23) : 0.0f;
+            eb[x] = in ? static_cast<int>(a.box_scale[ph]) - 127 : 0;
         }
         for (int i0 = first_token; i0 < stop; i0 += kMany ? a.tokens : 1) {
             const int i_end = !kMany || i0 + a.tokens > stop ? stop : i0 + a.tokens;
@@ -434,11 +433,12 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
                         acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qp[k], hi[x][k], acc, 0, 0, 0);
                         acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qn[k], lo[x][k], acc, 0, 0, 0);
                     }
-                    // |acc| < 2^23, so the conversion and both products are exact
-                    // wherever the result is a normal number.
+                    // |acc| < 2^23, so the conversion is exact, and so is the
+                    // product wherever the result is a normal number: both
+                    // powers at once, as one alone may leave the range.
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float f = static_cast<float>(acc[i]) * unit[i] * eb[x];
+                        const float f = __builtin_ldexpf(static_cast<float>(acc[i]), unit[i] + eb[x]);
                         s[x][i] = ht == 0 ? f : fmaxf(s[x][i], f);
                     }
                 }

@@ -442,6 +442,22 @@ def test_select_of_many_blocks_with_ties(ctx, blocks, width):
     assert np.array_equal(got.cpu().numpy(), ref.select(c, b, q64, width, 1, 2))
 
 
+@pytest.mark.parametrize("up", [118, -110])
+@pytest.mark.parametrize("new", [1, 3])
+def test_select_of_queries_and_boxes_far_from_one(ctx, up, new):
+    """Queries near the end of bf16's range against boxes at its other end: the
+    scores lie in the middle, the integer product times one power alone does not."""
+    b = ref.Batch(32, [32 * 40], [new], seed=3)
+    c = ref.Cache(b.pages, 1, 32, 64, "bf16", seed=1)
+    r = np.random.default_rng(4)
+    c.box = np.sort(r.integers(-127, 128, c.box.shape), axis=2)[:, :, ::-1].astype(np.int8).copy()
+    c.box_scale = (127 - up + r.integers(-2, 3, c.box_scale.shape)).astype(np.uint8)
+    q, _ = rows(r, new, 2, 64, "bf16", 1.0)
+    q = (q.float() * 2.0 ** up).to(torch.bfloat16)
+    got = device_cache(ctx, c).select(device_batch(b), q, 9)
+    assert np.array_equal(got.cpu().numpy(), ref.select(c, b, q.double().cpu().numpy(), 9, 1, 2))
+
+
 def test_select_of_zero_and_nonfinite_queries(ctx):
     b = ref.Batch(32, [800], [3], seed=3)
     c = ref.Cache(b.pages, 1, 32, 128, "bf16", seed=1)
