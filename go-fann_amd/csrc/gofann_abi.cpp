@@ -203,6 +203,8 @@ int kv_check(Context* ctx, const char* call, const gofann_kv_cache* c, const gof
         return ctx->fail(GOFANN_ERR_INVALID, at + "page_table or lengths is null");
     if (b->table_stride < b->table_width)
         return ctx->fail(GOFANN_ERR_INVALID, at + "table_stride below table_width");
+    if (b->visible != nullptr && b->visible_stride < b->visible_width)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "visible_stride below visible_width");
     if (b->query_offsets == nullptr && b->queries != b->sequences)
         return ctx->fail(GOFANN_ERR_INVALID, at + "without query_offsets there is one token a sequence");
     if (b->query_offsets != nullptr && b->max_queries > b->queries)

@@ -133,7 +133,8 @@ struct Batch {
     const int32_t* query_offsets;
     const uint32_t* visible;
     int64_t table_stride;
-    int64_t visible_stride;  // words a sequence
+    int64_t visible_stride;
+    int64_t visible_width;   // words of a row that are read
     int table_width;
     int queries;
     int page_shift;  // log2 of the page size
@@ -171,7 +172,7 @@ struct Batch {
     __device__ uint32_t word(int b, int w) const
     {
         if (visible == nullptr) return 0xFFFFFFFFu;
-        return w < visible_stride ? visible[b * visible_stride + w] : 0u;
+        return w < visible_width ? visible[b * visible_stride + w] : 0u;
     }
 };
 
@@ -187,6 +188,7 @@ inline Batch batch_of(const gofann_kv_cache* c, const gofann_kv_batch* b)
                  b->visible,
                  static_cast<int64_t>(b->table_stride),
                  static_cast<int64_t>(b->visible_stride),
+                 static_cast<int64_t>(b->visible_width != 0 ? b->visible_width : b->visible_stride),
                  static_cast<int>(b->table_width),
                  static_cast<int>(b->queries),
                  shift,

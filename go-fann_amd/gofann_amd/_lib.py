@@ -138,6 +138,18 @@ class KvBatchView(C.Structure):
         (n, U32) for n in ("sequences", "table_width", "table_stride", "visible_stride",
                            "queries", "max_queries", "max_length")]
 
+    # The struct's last member lies where the fields above end and ctypes pads,
+    # so that a view of them alone has it as 0: all words of visible_stride.
+    _WIDTH_AT = 4 * C.sizeof(P) + 7 * C.sizeof(U32)
+
+    @property
+    def visible_width(self) -> int:
+        return U32.from_buffer(self, self._WIDTH_AT).value
+
+    @visible_width.setter
+    def visible_width(self, words: int) -> None:
+        U32.from_buffer(self, self._WIDTH_AT).value = words
+
 
 class KvRows(C.Structure):
     _fields_ = [("data", P), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]

@@ -99,6 +99,8 @@ class KvBatch:
             page_table.data_ptr(), lengths.data_ptr(), _lib.ptr(query_offsets), _lib.ptr(visible),
             n, page_table.shape[1], stride(page_table), 0 if visible is None else stride(visible),
             queries, max_queries, max_length)
+        if visible is not None:
+            self.view.visible_width = visible.shape[1]
 
 
 class KvCache:

@@ -986,9 +986,9 @@ typedef struct {
     const int32_t* page_table;    /* [sequences][table_stride], table_width used */
     const int32_t* lengths;       /* [sequences] */
     const int32_t* query_offsets; /* [sequences + 1]; NULL: one token each */
-    const uint32_t* visible;      /* [sequences][visible_stride] bits, bit t % 32 of word t / 32:
-                                     position t may be attended to; NULL: all.  Positions
-                                     past the words may not. */
+    const uint32_t* visible;      /* [sequences][visible_stride] words, visible_width used, bit
+                                     t % 32 of word t / 32: position t may be attended to;
+                                     NULL: all.  Positions past the used words may not. */
     uint32_t sequences;
     uint32_t table_width;
     uint32_t table_stride;
@@ -996,6 +996,7 @@ typedef struct {
     uint32_t queries;     /* rows of the call in all */
     uint32_t max_queries; /* at least the tokens of any sequence */
     uint32_t max_length;  /* at least any length; only so many positions are read */
+    uint32_t visible_width; /* at most visible_stride; 0: visible_stride */
 } gofann_kv_batch;
 
 /* Rows [token][head][dim] of the cache's element type; strides in elements,
