@@ -101,6 +101,10 @@ class KvBatch:
             queries, max_queries, max_length)
         if visible is not None:
             self.view.visible_width = visible.shape[1]
+            if visible.shape[1] == 0:
+                # Nothing is visible, where NULL would be everything; the
+                # address is not read.
+                self.view.visible, self.view.visible_stride = lengths.data_ptr(), 0
 
 
 class KvCache:

@@ -51,3 +51,14 @@ def test_a_sliced_filter_hides_what_lies_past_its_words(ctx, width, new):
     assert np.array_equal(got.cpu().numpy(), ref.select(c, b, q64, 5, 1, 2))
     check_attend(d.attend(db, q, blocks=got, lse=lse), lse,
                  *ref.attend(c, b, q64, 64 ** -0.5, got.cpu().numpy()))
+
+
+def test_a_filter_without_words_hides_everything(ctx):
+    b = ref.Batch(32, [70, 40], [1, 3], seed=5)
+    c = ref.Cache(b.pages, 1, 32, 64, "bf16", seed=1)
+    ref.fill(c, b, seed=2)
+    q, _ = rows(np.random.default_rng(3), b.queries, 2, 64, "bf16")
+    d, db = device_cache(ctx, c), with_filter(b, torch.empty((2, 0), dtype=torch.int32, device="cuda"))
+    lse = torch.zeros((b.queries, 2), device="cuda")
+    assert (d.attend(db, q, lse=lse) == 0).all() and torch.isneginf(lse).all()
+    assert (d.select(db, q, 4) == -1).all()

@@ -36,6 +36,15 @@ def test_a_column_slice_of_a_filter_ends_at_its_words():
     assert _batch().view.visible_width == 0
 
 
+@pytest.mark.parametrize("sequences", [1, 3])
+def test_a_filter_without_words_is_not_no_filter(sequences):
+    import torch
+    for t in (torch.empty((sequences, 0), dtype=torch.int32),
+              torch.zeros((sequences, 8), dtype=torch.int32)[:, 3:3]):
+        v = _batch(sequences, visible=t).view
+        assert v.visible and v.visible_stride == v.visible_width == 0
+
+
 def test_the_batch_view_is_the_header_struct():
     """visible_width is the struct's last member, where the other fields' padding is."""
     from gofann_amd import _lib
