@@ -100,12 +100,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a)
     const int start = len - n;  // below 0 where the batch has more tokens than positions
     const int begin = start < 0 ? 0 : start;
     const int block = (begin >> t.page_shift) + static_cast<int>(blockIdx.y);
+    if (n == 0 || block >= t.table_width) return;
     const int page_begin = block << t.page_shift;
-    if (n == 0 || page_begin >= len) return;
+    const int stop = len < t.max_positions ? len : t.max_positions;
+    if (page_begin >= stop || begin >= stop) return;
     const int page = t.page(b, block);
     if (page < 0) return;
     const int fresh = (begin > page_begin ? begin : page_begin) - page_begin;
-    const int there = (len - page_begin < P ? len - page_begin : P);
+    const int there = (stop - page_begin < P ? stop - page_begin : P);
 
     const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
     const int64_t ph = static_cast<int64_t>(page) * t.kv_heads + h;

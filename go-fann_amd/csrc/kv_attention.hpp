@@ -34,7 +34,8 @@ struct AttendArgs {
 // (token, head of the group) rows, and the positions they reach.
 struct RowTile {
     int begin, end;
-    int first_pos, last_pos;  // of the first and the last row's token
+    int first_pos;            // of the first row's token
+    int last_pos;             // of the last row's, or the last that may have a page
     int token;                // listed: the one token
 };
 
@@ -55,6 +56,7 @@ __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int 
     if (t.end > t.begin + rows) t.end = t.begin + rows;
     t.first_pos = len - n + t.begin / a.group;
     t.last_pos = len - n + (t.end - 1) / a.group;
+    if (t.last_pos >= a.batch.max_positions) t.last_pos = a.batch.max_positions - 1;
     return t;
 }
 
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
     const int tile_begin = split * a.split_tiles;
     if (split > 0 && tile_begin >= tiles) return;
     const int tile_end = tile_begin + a.split_tiles < tiles ? tile_begin + a.split_tiles : tiles;
-    const int hi_pos = rt.last_pos + 1;                         // positions of the last row
+    const int hi_pos = rt.last_pos + 1;                         // positions that are read
     const int all_see = rt.first_pos + 1;                       // positions that every row sees
 
     // The rows' queries and limits.

@@ -140,12 +140,14 @@ struct Batch {
     int page_shift;  // log2 of the page size
     int pages;
     int kv_heads;
-    int max_positions;  // the most positions that a sequence is read to
+    int max_positions;  // positions from here on have no page
 
+    // Positions of sequence b, those without a page among them: its tokens are
+    // the last ones, wherever its page table ends.
     __device__ int length(int b) const
     {
         const int n = lengths[b];
-        return n < 0 ? 0 : n > max_positions ? max_positions : n;
+        return n < 0 ? 0 : n;
     }
     // First row of sequence b's tokens and their number.
     __device__ int first_query(int b) const

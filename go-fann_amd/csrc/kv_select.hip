@@ -39,10 +39,18 @@ __device__ __forceinline__ int blocks_to(const Batch& t, int pos)
     return pos < 0 ? 0 : (pos >> t.page_shift) + 1;
 }
 
+// Those of `blocks` that may have a page.
+__device__ __forceinline__ int paged(const Batch& t, int blocks)
+{
+    const int most = (t.max_positions + (1 << t.page_shift) - 1) >> t.page_shift;
+    return blocks < most ? blocks : most;
+}
+
 // Whether block j (page_size positions) has a visible position up to pos.
 __device__ __forceinline__ bool any_visible(const Batch& t, int b, int j, int pos)
 {
     if (t.visible == nullptr) return true;
+    if (pos >= t.max_positions) pos = t.max_positions - 1;
     const int words = 1 << (t.page_shift - 5);
     const int w0 = j * words;
     uint32_t any = 0;
@@ -299,7 +307,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
     const int first_token = kMany ? blockIdx.y * per : 0;
     if (first_token >= n) return;
     const int stop = first_token + per < n ? first_token + per : n;
-    const int blocks = blocks_to(t, position(len, n, stop - 1));
+    const int blocks = paged(t, blocks_to(t, position(len, n, stop - 1)));
     const int chunks = (blocks + kChunk - 1) / kChunk;
     if (chunk > 0 && chunk >= chunks) return;
     const bool whole = !kMany && chunks <= 1;  // all keys of the row are here
@@ -451,12 +459,12 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
                     const int token = i0 + (first_row >> rows_shift);
                     if (token >= i_end) return;
                     const int pos = position(len, n, token);
-                    const int mine = blocks_to(t, pos);
+                    const int upto = blocks_to(t, pos), mine = paged(t, upto);
                     uint32_t key = kIneligible;
                     if (block < mine && page[x] >= 0 && any_visible(t, b, block, pos)) {
                         const uint32_t u = __builtin_bit_cast(uint32_t, score + 0.0f);  // -0 as 0
                         key = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-                        if (block < a.first || block >= mine - a.last) key = kForced;
+                        if (block < a.first || block >= upto - a.last) key = kForced;
                     }
                     if (whole)
                         stage[block] = key;
@@ -497,7 +505,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
     } else {
         __syncthreads();
     }
-    const int mine = blocks_to(t, position(len, n, 0));
+    const int mine = paged(t, blocks_to(t, position(len, n, 0)));
     if (whole)
         pick<1>(a, sh, mine, a.out + row0 * a.width, [&](int j) { return stage[j]; });
     else
@@ -514,7 +522,8 @@ __global__ __launch_bounds__(256) void kv_pick_kernel(SelectArgs a)
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
     if (i >= n) return;
-    pick_row(a, sh, blocks_to(t, position(len, n, i)), static_cast<int64_t>(q0 + i) * t.kv_heads + h);
+    pick_row(a, sh, paged(t, blocks_to(t, position(len, n, i))),
+             static_cast<int64_t>(q0 + i) * t.kv_heads + h);
 }
 
 template <class E>

@@ -981,7 +981,8 @@ typedef struct {
 /* The sequences of one call.  Sequence b holds lengths[b] positions, the last
  * query_offsets[b+1] - query_offsets[b] of which are this call's tokens (rows
  * query_offsets[b] ..).  A page id outside [0, pages) is a hole: its
- * positions are neither written nor read. */
+ * positions are neither written nor read, no more than those past the page
+ * table's width; they count in a token's position all the same. */
 typedef struct {
     const int32_t* page_table;    /* [sequences][table_stride], table_width used */
     const int32_t* lengths;       /* [sequences] */
@@ -995,7 +996,7 @@ typedef struct {
     uint32_t visible_stride;
     uint32_t queries;     /* rows of the call in all */
     uint32_t max_queries; /* at least the tokens of any sequence */
-    uint32_t max_length;  /* at least any length; only so many positions are read */
+    uint32_t max_length;  /* at least any length; only so many positions are used */
     uint32_t visible_width; /* at most visible_stride; 0: visible_stride */
 } gofann_kv_batch;
 

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import kv_reference as ref
-from test_gpu_kvcache import check_attend, device_cache, rows
+from test_gpu_kvcache import check_attend, device_batch, device_cache, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,71 @@ def test_a_filter_without_words_hides_everything(ctx):
     lse = torch.zeros((b.queries, 2), device="cuda")
     assert (d.attend(db, q, lse=lse) == 0).all() and torch.isneginf(lse).all()
     assert (d.select(db, q, 4) == -1).all()
+
+
+# ---- sequences longer than their page table ------------------------------------
+
+def cut(b: ref.Batch, width: int):
+    """The batch with page tables of only `width` blocks."""
+    b.table, b.width = np.ascontiguousarray(b.table[:, :width]), width
+    return b
+
+
+PAST = [
+    # elem, dim, page, kv heads, group, lengths, new, table width
+    ("bf16", 128, 64, 2, 4, [129, 200, 128], [1, 1, 1], 2),
+    ("f16", 64, 32, 1, 3, [70, 100, 33], [9, 40, 2], 2),
+    ("bf16", 256, 32, 1, 2, [90, 65], [30, 1], 2),
+]
+
+
+@pytest.mark.parametrize("elem,dim,page,heads,group,lens,new,width", PAST)
+def test_positions_past_the_page_table_are_holes(ctx, elem, dim, page, heads, group, lens, new, width):
+    """Tokens there are written nowhere, and those that have a page keep their positions."""
+    b = ref.Batch(page, lens, new, seed=dim)
+    cut(b, width)
+    c = ref.Cache(b.pages, heads, page, dim, elem, seed=1)
+    old = ref.Batch(page, [min(n - m, width * page) for n, m in zip(lens, new)], [0] * len(new), pages=b.pages)
+    old.table, old.width = b.table, width
+    ref.fill(c, old, seed=2)
+    r = np.random.default_rng(3)
+    k, k64 = rows(r, b.queries, heads, dim, elem)
+    v, v64 = rows(r, b.queries, heads, dim, elem)
+    q, q64 = rows(r, b.queries, heads * group, dim, elem)
+    d, db = device_cache(ctx, c), device_batch(b)
+    kh = torch.full_like(k, 7.0)
+    d.append(db, k, v, k_held=kh)
+    touched = set()
+    want = np.full(k64.shape, 7.0)
+    for row, s, pos in b.tokens():
+        if pos // page < width:
+            want[row] = c.write(b.table[s, pos // page], pos % page, k64[row], v64[row])[0]
+            touched.add((s, pos // page))
+    for s, j in touched:
+        c.renew_box(b.table[s, j], min(page, lens[s] - j * page))
+    torch.cuda.synchronize()
+    for name in c.NAMES:
+        assert np.array_equal(getattr(d, name).cpu().numpy(), getattr(c, name)), name
+    assert np.array_equal(kh.double().cpu().numpy(), want)
+    lse = torch.empty((b.queries, heads * group), device="cuda")
+    check_attend(d.attend(db, q, lse=lse), lse, *ref.attend(c, b, q64, dim ** -0.5))
+    for n, first, last in ((1, 0, 1), (3, 1, 2)):
+        got = d.select(db, q, n, first=first, last=last)
+        assert np.array_equal(got.cpu().numpy(), ref.select(c, b, q64, n, first, last))
+    check_attend(d.attend(db, q, blocks=got, lse=lse), lse,
+                 *ref.attend(c, b, q64, dim ** -0.5, got.cpu().numpy()))
+
+
+def test_a_token_past_the_table_leaves_the_cache_as_it_was(ctx):
+    """Position 128 of a sequence with two pages of 64: position 127 keeps its key."""
+    b = ref.Batch(64, [129], [1], seed=1)
+    c = ref.Cache(b.pages, 2, 64, 128, "bf16", seed=1)
+    ref.fill(c, b)
+    cut(b, 2)
+    d = device_cache(ctx, c)
+    k, _ = rows(np.random.default_rng(2), 1, 2, 128, "bf16")
+    d.append(device_batch(b), k, k)
+    d.append(device_batch(b, one_token=True), k, k)
+    torch.cuda.synchronize()
+    for name in c.NAMES:
+        assert np.array_equal(getattr(d, name).cpu().numpy(), getattr(c, name)), name
