@@ -228,6 +228,7 @@ int kv_append(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch*
     // Pages that so many tokens in a row can touch.
     uint64_t touched = (tokens + cache->page_size - 2) / cache->page_size + 1;
     if (touched > batch->table_width) touched = batch->table_width;
+    if (touched == 0) return GOFANN_OK;
     if (touched > 65535)
         return ctx->fail(GOFANN_ERR_UNSUPPORTED, "kv_append: too many tokens a sequence for one call");
     const dim3 grid(cache->kv_heads, static_cast<uint32_t>(touched), batch->sequences);

@@ -77,6 +77,7 @@ PAST = [
     ("bf16", 128, 64, 2, 4, [129, 200, 128], [1, 1, 1], 2),
     ("f16", 64, 32, 1, 3, [70, 100, 33], [9, 40, 2], 2),
     ("bf16", 256, 32, 1, 2, [90, 65], [30, 1], 2),
+    ("bf16", 64, 64, 1, 1, [40, 3], [1, 3], 0),
 ]
 
 

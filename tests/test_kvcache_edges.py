@@ -70,6 +70,13 @@ def case_filter_width(f: Kv):
         assert call(h, batch=batch(0, 0)) == f.L.OK
 
 
+def case_append_without_a_page_table(f: Kv):
+    h = f.context()
+    for table in (None, f.p):
+        assert f.append(h, batch=f.batch(page_table=table, table_width=0, table_stride=0)) == f.L.OK
+    assert not f.launched()  # a grid of no workgroups is an error of the runtime
+
+
 CASES = sorted(k[5:] for k in globals() if k.startswith("case_"))
 
 
