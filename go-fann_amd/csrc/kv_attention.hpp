@@ -16,8 +16,8 @@ struct AttendArgs {
     const uint8_t* v_scales;
     const int32_t* blocks;  // [queries][kv_heads][width] or NULL
     float* lse;             // [queries][heads] or NULL
-    float* part_o;          // [item][split][rows][dim], splits > 1
-    float* part_ml;         // [item][split][rows][2]: reference, sum
+    float* part_o;          // [kv_heads][split][part_count][dim], splits > 1: see part_of()
+    float* part_ml;         // [kv_heads][split][part_count][2]: reference, sum
     uint32_t* arrived;      // [item], zero between calls: splits done; NULL: kv_join_kernel joins
     float scale_log2;       // scale * log2(e)
     int group;              // heads a key/value head
@@ -28,7 +28,70 @@ struct AttendArgs {
     int split_tiles;        // tiles of a split
     int rows_over;          // sequences of at most so many rows are not this launch's,
     int rows_upto;          // nor those of more than so many
+    int64_t part_count;     // rows with partial results: the call's, or of every
+    int part_rows;          // sequence so many where that is not 0
+    int slots;              // row tiles counted through the sequences; 0: a grid of them
+    int sequences;
 };
+
+// What a workgroup works on: row tile `index` of sequence b, the id-th of all.
+struct Item {
+    int b, index;
+    int64_t id;
+};
+
+// Row tiles of a sequence are blockIdx.y, sequences blockIdx.z.  Where sequences
+// differ so much in their tokens that most of that grid would find nothing, the
+// tiles are counted through them instead (slots): those of sequence b begin at
+// offset[b] group / rows + b, which leaves each room for its last, part tile
+// (listed: at its first token's), so that a search of the offsets is all that
+// is needed.  False: no such tile.
+__device__ __forceinline__ bool item_of(const AttendArgs& a, int rows, Item& it)
+{
+    const Batch& t = a.batch;
+    if (a.slots == 0) {
+        it.b = blockIdx.z;
+        it.index = gridDim.y - 1 - blockIdx.y;  // the longest rows first
+        it.id = static_cast<int64_t>(it.b) * a.row_tiles + it.index;
+        return true;
+    }
+    const int64_t from_end = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y;
+    it.id = a.slots - 1 - from_end;
+    if (it.id < 0) return false;
+    const auto begin = [&](int b) {
+        const int64_t q0 = t.first_query(b);
+        return a.blocks != nullptr ? q0 * a.token_tiles : q0 * a.group / rows + b;
+    };
+    // The last sequence that begins no later: 64 are looked at in each round.
+    const int lane = threadIdx.x % 64;
+    int b = 0, count = a.sequences;
+    while (count > 1) {
+        const int step = (count + 63) / 64;
+        const int at = lane * step;
+        const int below = __popcll(__ballot(at < count && begin(b + (at < count ? at : 0)) <= it.id));
+        const int skip = below > 0 ? (below - 1) * step : 0;
+        b += skip;
+        count = count - skip < step ? count - skip : step;
+    }
+    it.b = __builtin_amdgcn_readfirstlane(b);
+    const int q0 = t.first_query(it.b);
+    const int64_t n = t.new_tokens(it.b, q0);
+    const int64_t index = it.id - begin(it.b);
+    const int64_t tiles = a.blocks != nullptr ? n * a.token_tiles : (n * a.group + rows - 1) / rows;
+    if (index < 0 || index >= tiles) return false;
+    it.index = static_cast<int>(index);
+    return true;
+}
+
+// Where the partial results of a sequence's first row lie, in rows: a tile's
+// rows lie together, as they are written (with a row's splits together instead,
+// 19 sequences of five tokens and four heads a group took 26.1 us, not 25.2).
+__device__ __forceinline__ int64_t part_of(const AttendArgs& a, int b, int q0, int h, int split)
+{
+    const int64_t first = a.part_rows > 0 ? static_cast<int64_t>(b) * a.part_rows
+                                          : static_cast<int64_t>(q0) * a.group;
+    return (static_cast<int64_t>(h) * a.splits + split) * a.part_count + first;
+}
 
 // The rows of one row tile: rows [begin, end) of the sequence's flattened
 // (token, head of the group) rows, and the positions they reach.
@@ -216,8 +279,9 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
     const int r16 = lane % 16, g4 = lane / 16;
     const int h = blockIdx.x % t.kv_heads;
     const int split = blockIdx.x / t.kv_heads;
-    const int index = gridDim.y - 1 - blockIdx.y;  // the longest rows first
-    const int b = blockIdx.z;
+    Item it;
+    if (!item_of(a, kRows, it)) return;
+    const int index = it.index, b = it.b;
     const int len = t.length(b);
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
@@ -438,9 +502,8 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
     __shared__ float wm[4][kRows], ws[4][kRows];
     __shared__ __attribute__((aligned(16))) float wo[4][16][kPad];
     const int active = (tiles + a.split_tiles - 1) / a.split_tiles;
-    const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
-    float* const po = a.part_o + item * a.splits * kRows * D;
-    float* const pm = a.part_ml + item * a.splits * kRows * 2;
+    const int64_t item = it.id * t.kv_heads + h;
+    const int64_t my_part = part_of(a, b, q0, h, split);
     const int my_ch = 4 * (threadIdx.x % kLanes);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -476,15 +539,16 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
             if (active <= 1) {
                 finish<E>(a, t, q0, h, row, my_ch, acc, top, total);
             } else {
-                const int at = split * kRows + 16 * nt + r;
-                float* const to = po + static_cast<int64_t>(at) * D + my_ch;
+                const int64_t at = my_part + row;
+                float* const to = a.part_o + at * D + my_ch;
+                float* const pm = a.part_ml + 2 * at;
                 if (a.arrived != nullptr) {
                     put2(to, acc[0], acc[1]);
                     put2(to + 2, acc[2], acc[3]);
-                    if (my_ch == 0) put2(pm + 2 * at, top, total);
+                    if (my_ch == 0) put2(pm, top, total);
                 } else {
                     *reinterpret_cast<f32x4*>(to) = acc;
-                    if (my_ch == 0) *reinterpret_cast<float2*>(pm + 2 * at) = float2{top, total};
+                    if (my_ch == 0) *reinterpret_cast<float2*>(pm) = float2{top, total};
                 }
             }
         }
@@ -509,11 +573,13 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
     __syncthreads();
     if (!last) return;
     __shared__ float jm[kJoinSplits][kRows], js[kJoinSplits][kRows];
+    const int64_t first_part = part_of(a, b, q0, h, 0) + rt.begin;
     for (int x = threadIdx.x; x < active * kRows; x += 256) {
-        const bool in = rt.begin + x % kRows < rt.end;
-        const float2 v = in ? get2(pm + 2 * x) : float2{0.0f, 0.0f};
-        jm[x / kRows][x % kRows] = v.x;
-        js[x / kRows][x % kRows] = v.y;
+        const int w = x / kRows, r = x % kRows;
+        if (rt.begin + r >= rt.end) continue;
+        const float2 v = get2(a.part_ml + 2 * (first_part + w * a.part_count + r));
+        jm[w][r] = v.x;
+        js[w][r] = v.y;
     }
     __syncthreads();
     for (int r = threadIdx.x / kLanes; rt.begin + r < rt.end; r += kStep) {
@@ -522,11 +588,12 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
         const float keep = top == -__builtin_inff() ? 0.0f : top;
         float total = 0.0f;
         f32x4 acc{0, 0, 0, 0};
+        const float* const po = a.part_o + (first_part + r) * D + my_ch;
 #pragma unroll 4
         for (int w = 0; w < active; ++w) {
             const float f = __builtin_amdgcn_exp2f(jm[w][r] - keep);
             total += f * js[w][r];
-            const float* const from = po + (static_cast<int64_t>(w) * kRows + r) * D + my_ch;
+            const float* const from = po + w * a.part_count * D;
             const float2 lo = get2(from), hi = get2(from + 2);
             acc += f * f32x4{lo.x, lo.y, hi.x, hi.y};
         }
@@ -896,7 +963,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int h = blockIdx.x % t.kv_heads;
     const int r = blockIdx.x / t.kv_heads;
-    const int index = blockIdx.y, b = blockIdx.z;
+    Item it;
+    if (!item_of(a, kRows, it)) return;
+    const int index = it.index, b = it.b;
     const int len = t.length(b);
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
@@ -905,16 +974,16 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
     if (row >= rt.end) return;
     const int active = (tiles_of(a, rt) + a.split_tiles - 1) / a.split_tiles;
     if (active <= 1) return;  // written already
-    const int64_t item = (static_cast<int64_t>(b) * a.row_tiles + index) * t.kv_heads + h;
-    const float* const ml = a.part_ml + (item * a.splits * kRows + r) * 2;
-    const float* const po = a.part_o + (item * a.splits * kRows + r) * D + lane * kC;
+    const int64_t at = part_of(a, b, q0, h, 0) + row;
+    const float* const ml = a.part_ml + 2 * at;
+    const float* const po = a.part_o + at * D + lane * kC;
     float top = -__builtin_inff(), total = 0.0f;
     float acc[kC] = {};
     for (int base = wave; base < active; base += 256) {
         // Lane l has split base + 4 l.
         const int s = base + 4 * lane;
-        const float m = s < active ? ml[static_cast<int64_t>(s) * kRows * 2] : -__builtin_inff();
-        const float z = s < active ? ml[static_cast<int64_t>(s) * kRows * 2 + 1] : 0.0f;
+        const float m = s < active ? ml[2 * s * a.part_count] : -__builtin_inff();
+        const float z = s < active ? ml[2 * s * a.part_count + 1] : 0.0f;
         float fresh = m;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) fresh = fmaxf(fresh, __shfl_xor(fresh, d));
@@ -933,7 +1002,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
                 float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k));
 #pragma unroll
             for (int c = 0; c < kC; ++c)
-                acc[c] += fk * po[static_cast<int64_t>(base + 4 * k) * kRows * D + c];
+                acc[c] += fk * po[(base + 4 * k) * a.part_count * D + c];
         }
     }
 #pragma unroll

@@ -19,6 +19,7 @@ namespace {
 struct Launch {
     std::string name;
     unsigned grid;
+    uint64_t workgroups;
     size_t lds;
     const void* stream;
 };
@@ -63,6 +64,7 @@ void fake_clear() { g_launches.clear(); }
 int fake_launches() { return static_cast<int>(g_launches.size()); }
 const char* fake_name(int i) { return g_launches[i].name.c_str(); }
 unsigned fake_grid(int i) { return g_launches[i].grid; }
+uint64_t fake_workgroups(int i) { return g_launches[i].workgroups; }
 
 void** __hipRegisterFatBinary(const void*)
 {
@@ -99,7 +101,8 @@ hipError_t __hipPopCallConfiguration(dim3* grid, dim3* block, size_t* lds, hipSt
 hipError_t hipLaunchKernel(const void* f, dim3 grid, dim3, void**, size_t lds, hipStream_t stream)
 {
     const auto it = names().find(f);
-    g_launches.push_back(Launch{it == names().end() ? "?" : it->second, grid.x, lds, stream});
+    g_launches.push_back(Launch{it == names().end() ? "?" : it->second, grid.x,
+                                static_cast<uint64_t>(grid.x) * grid.y * grid.z, lds, stream});
     return hipSuccess;
 }
 

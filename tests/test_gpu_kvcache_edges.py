@@ -131,3 +131,53 @@ def test_a_token_past_the_table_leaves_the_cache_as_it_was(ctx):
     torch.cuda.synchronize()
     for name in c.NAMES:
         assert np.array_equal(getattr(d, name).cpu().numpy(), getattr(c, name)), name
+
+
+# ---- batches of very unequal chunks -------------------------------------------
+
+MANY = [
+    # elem, dim, page, kv heads, group, new tokens of the sequences, lengths beside them
+    ("bf16", 128, 64, 2, 4, [1] * 9 + [70] + [0, 1, 3] + [1] * 8, 300),
+    ("f16", 64, 32, 1, 7, [0, 0, 41] + [1] * 70 + [0], 90),
+    ("bf16", 256, 64, 1, 3, [2] * 6 + [90] + [1] * 6, 200),
+]
+
+
+@pytest.mark.parametrize("elem,dim,page,heads,group,new,most", MANY)
+@pytest.mark.parametrize("filtered", [False, True])
+def test_a_chunk_beside_many_short_sequences(ctx, elem, dim, page, heads, group, new, most, filtered):
+    """Few row tiles of many sequences: whole, listed and split under a far bound."""
+    r = np.random.default_rng(4)
+    lens = [n + int(r.integers(0, most)) for n in new]
+    b = ref.Batch(page, lens, new, seed=dim, visible=(lambda s, n, g: g.random(n) < 0.6) if filtered else None)
+    c = ref.Cache(b.pages, heads, page, dim, elem, seed=1)
+    ref.fill(c, b, seed=2)
+    q, q64 = rows(r, b.queries, heads * group, dim, elem)
+    d = device_cache(ctx, c)
+    lse = torch.full((b.queries, heads * group), 7.0, device="cuda")
+    want = ref.attend(c, b, q64, dim ** -0.5)
+    for bound in (max(lens), 1 << 21):
+        check_attend(d.attend(device_batch(b, max_length=bound), q, lse=lse), lse, *want)
+    blocks = d.select(device_batch(b), q, 4)
+    check_attend(d.attend(device_batch(b), q, blocks=blocks, lse=lse), lse,
+                 *ref.attend(c, b, q64, dim ** -0.5, blocks.cpu().numpy()))
+
+
+def test_row_tiles_of_rows_the_batch_does_not_have(ctx):
+    """Offsets that leave rows out, before the first sequence and past the last."""
+    from gofann_amd import kvcache
+    new = [0, 1, 40, 1, 1, 1, 1, 1, 1, 1, 1, 1]
+    b = ref.Batch(32, [n + 20 for n in new], new, seed=1)
+    c = ref.Cache(b.pages, 1, 32, 64, "bf16", seed=1)
+    ref.fill(c, b, seed=2)
+    q, q64 = rows(np.random.default_rng(3), b.queries, 2, 64, "bf16")
+    want = ref.attend(c, b, q64, 64 ** -0.5)
+    big = torch.zeros((b.queries + 8, 2, 64), dtype=torch.bfloat16, device="cuda")
+    big[3:3 + b.queries] = q
+    db = kvcache.KvBatch(torch.from_numpy(b.table).cuda(), torch.tensor(b.lens, dtype=torch.int32, device="cuda"),
+                         torch.from_numpy(b.offsets + 3).cuda(), queries=b.queries + 8, max_queries=40,
+                         max_length=1 << 16)
+    out = torch.full_like(big, 99.0)
+    device_cache(ctx, c).attend(db, big, out=out)
+    check_attend(out[3:3 + b.queries], None, want[0], None, want[2])
+    assert (out[:3] == 99.0).all() and (out[3 + b.queries:] == 99.0).all()

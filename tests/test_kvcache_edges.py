@@ -77,6 +77,45 @@ def case_append_without_a_page_table(f: Kv):
     assert not f.launched()  # a grid of no workgroups is an error of the runtime
 
 
+def _mixed(f: Kv, **kw):
+    """63 sequences of one token beside a chunk of 512, under a far bound on the length."""
+    b = dict(sequences=64, queries=63 + 512, max_queries=512, max_length=131072, table_width=2048,
+             table_stride=2048)
+    b.update(kw)
+    return f.batch(**b)
+
+
+def case_workspace_by_the_rows_there_are(f: Kv):
+    f.hip.fake_workgroups.restype = C.c_uint64
+    f.hip.fake_limit(8 * host.GIB)  # the arrays are never touched
+    before = f.hip.fake_used()
+    # one token each: 64 x 32 rows of 86 splits of 130 floats
+    h = f.context()
+    b = f.batch(sequences=64, queries=64, max_length=131072, table_width=2048, table_stride=2048)
+    assert f.attend(h, batch=b) == f.L.OK
+    assert f.hip.fake_used() - before <= 64 * 32 * 86 * 130 * 4
+    f.lib.gofann_destroy(h)
+    for kw in ({}, dict(blocks=f.p, width=64), dict(batch=_mixed(f, max_length=1 << 20, table_width=1 << 14,
+                                                                table_stride=1 << 14))):
+        h = f.context()
+        f.launched()
+        assert f.attend(h, batch=kw.pop("batch", _mixed(f)), **kw) == f.L.OK
+        assert f.hip.fake_used() - before <= 520 << 20
+        # 135 tiles of 32 rows, listed 575 of 16, of 8 heads in at most 56 splits
+        assert f.hip.fake_workgroups(0) <= 575 * 8 * 56
+        f.lib.gofann_destroy(h)
+
+
+def case_workspace_beside_long_chunks(f: Kv):
+    """What the wide launch leaves, however many rows it has itself."""
+    f.hip.fake_limit(8 * host.GIB)
+    before = f.hip.fake_used()
+    h = f.context()
+    assert f.attend(h, batch=_mixed(f, queries=63 + 4096, max_queries=4096)) == f.L.OK
+    assert ["wide" in n for n, _ in f.launched()] == [True, False, False]
+    assert f.hip.fake_used() - before <= 520 << 20
+
+
 CASES = sorted(k[5:] for k in globals() if k.startswith("case_"))
 
 
