@@ -31,6 +31,7 @@ _ELEM = {torch.bfloat16: _lib.ELEM_BF16, torch.float16: _lib.ELEM_F16}
 # The handle of torch's current stream, as torch.cuda.current_stream(i).cuda_stream.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 DIMS = (64, 128, 256)
 PAGE_SIZES = (32, 64, 128, 256)
 
@@ -142,6 +143,7 @@ class KvCache:
                 raise ValueError(f"{name} must be contiguous and on one device with k_codes")
         self.ctx, self.lib = ctx, ctx.lib
         self.dtype, self.device = dtype, k_codes.device
+        self._index = k_codes.device.index if k_codes.device.type == "cuda" else -1
         self.pages, self.kv_heads, self.page, self.dim = pages, heads, page, dim
         self.__dict__.update(arrays)
         self.boxed = box is not None
@@ -186,7 +188,11 @@ class KvCache:
     def _ready(self, batch: KvBatch) -> None:
         if batch.device != self.device:
             raise ValueError("the batch is on another device")
-        if _raw_stream(self.device.index or 0) != self.ctx.stream:
+        if self._index != self.ctx.device:
+            raise ValueError("the cache is not on the context's device")
+        if _current_device() != self._index:
+            raise _lib.GofannError("torch's current device is not the context's")
+        if _raw_stream(self._index) != self.ctx.stream:
             raise _lib.GofannError("the context is bound to another stream than torch's current "
                                    "one: call ctx.bind_stream")
 

@@ -11,7 +11,7 @@ import pytest
 
 sys.path.insert(0, str(Path(__file__).resolve().parent))
 import test_host_dispatch as host  # noqa: E402
-from test_kvcache import Kv  # noqa: E402
+from test_kvcache import Kv, _cpu_cache  # noqa: E402
 
 
 def _batch(sequences=3, blocks=4, **kw):
@@ -52,6 +52,31 @@ def test_the_batch_view_is_the_header_struct():
     v = _lib.KvBatchView()
     v.max_length, v.visible_width = 5, 7
     assert bytes(v)[-8:] == bytes([5, 0, 0, 0, 7, 0, 0, 0]) and v.visible_width == 7
+
+
+def _calls(cache, batch):
+    import torch
+    n, h = batch.queries, cache.kv_heads
+    k, q = (torch.zeros(n, m, cache.dim, dtype=cache.dtype) for m in (h, 4 * h))
+    return (lambda: cache.append(batch, k, k), lambda: cache.select(batch, q, 4),
+            lambda: cache.attend(batch, q))
+
+
+def test_arrays_on_another_device_than_the_contexts_are_refused(monkeypatch):
+    """Host arrays, or another GPU's, would be addresses that the kernels cannot read."""
+    from gofann_amd import _lib, kvcache
+    monkeypatch.setattr(kvcache, "_raw_stream", lambda i: 0)
+    d = _cpu_cache()
+    d.ctx.device = 0
+    for call in _calls(d, _batch()):
+        with pytest.raises(ValueError, match="context's device"):
+            call()
+    # arrays in place, but torch's current device another: so is the default stream's
+    monkeypatch.setattr(kvcache, "_current_device", lambda: 1, raising=False)
+    d._index = 0
+    for call in _calls(d, _batch()):
+        with pytest.raises(_lib.GofannError, match="current device"):
+            call()
 
 
 # ---- C entries over the stand-in runtime ------------------------------------------
