@@ -54,12 +54,23 @@ class Session:
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, width: int = 0,
              lse: torch.Tensor | None = None) -> torch.Tensor:
         """Appends the tokens' keys and values and attends with their queries:
-        over everything visible, or over the `width` blocks chosen for each."""
-        tokens = q.shape[0] // self.sequences
+        over everything visible, or over the `width` blocks chosen for each.  A
+        step that is refused leaves the sequences as long as they were."""
+        tokens, rest = divmod(q.shape[0], self.sequences)
+        if rest:
+            raise ValueError("a step has as many tokens for each of the sequences")
+        before = self.filled
         batch = self.grow(tokens)
-        self.cache.append(batch, k, v)
-        blocks = self.cache.select(batch, q, width) if width else None
-        return self.cache.attend(batch, q, blocks=blocks, lse=lse)
+        try:
+            self.cache.append(batch, k, v)
+            blocks = self.cache.select(batch, q, width) if width else None
+            return self.cache.attend(batch, q, blocks=blocks, lse=lse)
+        except Exception:
+            # What was written lies past the end again; the next step's append
+            # writes over it and renews its pages' boxes.
+            self.filled = before
+            self.lengths.fill_(before)
+            raise
 
 
 def main(argv=None) -> None:

@@ -181,3 +181,15 @@ def test_row_tiles_of_rows_the_batch_does_not_have(ctx):
     device_cache(ctx, c).attend(db, big, out=out)
     check_attend(out[3:3 + b.queries], None, want[0], None, want[2])
     assert (out[:3] == 99.0).all() and (out[3 + b.queries:] == 99.0).all()
+
+
+def test_a_refused_step_of_the_example_is_as_if_never_made(ctx):
+    from gofann_amd import _lib, longcontext
+    r = np.random.default_rng(6)
+    a, b = (longcontext.Session(ctx, sequences=2, capacity=200, kv_heads=2, dim=64, page=32) for _ in range(2))
+    for tokens, width in ((70, 0), (9, 4), (1, 4)):
+        q, k, v = (rows(r, 2 * tokens, h, 64, "bf16")[0] for h in (8, 2, 2))
+        with pytest.raises(_lib.GofannError, match="width"):
+            a.step(q + 1, k + 1, v + 1, 2)  # refused by the choice, once its tokens are written
+        assert torch.equal(a.step(q, k, v, width), b.step(q, k, v, width))
+        assert torch.equal(a.lengths, b.lengths)

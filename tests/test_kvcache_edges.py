@@ -6,6 +6,7 @@ import ctypes as C
 import subprocess
 import sys
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 
@@ -77,6 +78,36 @@ def test_arrays_on_another_device_than_the_contexts_are_refused(monkeypatch):
     for call in _calls(d, _batch()):
         with pytest.raises(_lib.GofannError, match="current device"):
             call()
+
+
+@pytest.mark.parametrize("fails", ["append", "select", "attend"])
+def test_a_refused_step_of_the_example_leaves_its_lengths(fails):
+    import torch
+    from gofann_amd.longcontext import Session
+    s = Session.__new__(Session)
+    s.sequences, s.capacity, s.filled = 2, 100, 10
+    s.table = torch.zeros((2, 4), dtype=torch.int32)
+    s.lengths = torch.full((2,), 10, dtype=torch.int32)
+    s.visible = torch.full((2, 4), -1, dtype=torch.int32)
+
+    def call(name):
+        def f(batch, *a, **kw):
+            assert batch.max_length == 13 and s.lengths.tolist() == [13, 13]
+            if name == fails:
+                raise ValueError("refused")
+        return f
+
+    s.cache = SimpleNamespace(**{n: call(n) for n in ("append", "select", "attend")})
+    q = torch.zeros((6, 4, 64))
+    with pytest.raises(ValueError, match="refused"):
+        s.step(q, q, q, 8)
+    assert s.filled == 10 and s.lengths.tolist() == [10, 10]
+    with pytest.raises(ValueError, match="sequences"):
+        s.step(q[:5], q[:5], q[:5], 8)
+    assert s.filled == 10 and s.lengths.tolist() == [10, 10]
+    fails = None
+    s.step(q, q, q, 8)
+    assert s.filled == 13
 
 
 # ---- C entries over the stand-in runtime ------------------------------------------
