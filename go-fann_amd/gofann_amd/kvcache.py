@@ -43,6 +43,12 @@ def _shapes(pages: int, heads: int, page: int, dim: int) -> dict:
                 box=(pages, heads, 2, dim), box_scale=(pages, heads))
 
 
+def _counts(**kw: int) -> None:
+    for name, n in kw.items():
+        if not 0 <= n < 1 << 32:
+            raise ValueError(f"{name} must be in [0, 2^32)")
+
+
 class KvBatch:
     """The sequences of one call (gofann_kv_batch).
 
@@ -74,8 +80,7 @@ class KvBatch:
             raise ValueError("query_offsets is [sequences + 1]")
         elif queries is None or max_queries is None:
             raise ValueError("query_offsets needs queries and max_queries")
-        if min(queries, max_queries, max_length) < 0:
-            raise ValueError("queries, max_queries and max_length are not negative")
+        _counts(queries=queries, max_queries=max_queries, max_length=max_length)
         if visible is not None and (visible.dim() != 2 or visible.shape[0] != n):
             raise ValueError("visible is [sequences][words]")
         for name, t in (("page_table", page_table), ("lengths", lengths),
@@ -218,6 +223,7 @@ class KvCache:
         last ones, then those whose boxes score highest against any of the
         group's queries."""
         self._ready(batch)
+        _counts(width=width, first=first, last=last)
         rq = self._rows("q", q, batch.queries, q.shape[1] if q.dim() == 3 else None)
         shape = (batch.queries, self.kv_heads, width)
         if out is None:

@@ -55,6 +55,30 @@ def test_the_batch_view_is_the_header_struct():
     assert bytes(v)[-8:] == bytes([5, 0, 0, 0, 7, 0, 0, 0]) and v.visible_width == 7
 
 
+@pytest.mark.parametrize("name", ["queries", "max_queries", "max_length"])
+def test_bounds_past_32_bits_are_refused(name):
+    """ctypes would hand on their low bits: a bound of 2^32 as one of 0."""
+    import torch
+    from gofann_amd.kvcache import KvBatch
+    table, off = torch.zeros((3, 4), dtype=torch.int32), torch.arange(4, dtype=torch.int32)
+    kw = dict(queries=3, max_queries=1, max_length=9)
+    for wrong in (2 ** 32, 2 ** 32 + 9, -2 ** 32 + 9, -1):
+        with pytest.raises(ValueError, match=name):
+            KvBatch(table, off[1:], off, **{**kw, name: wrong})
+    assert getattr(KvBatch(table, off[1:], off, **{**kw, name: 2 ** 32 - 1}).view, name) == 2 ** 32 - 1
+
+
+@pytest.mark.parametrize("name", ["width", "first", "last"])
+def test_counts_of_blocks_past_32_bits_are_refused(name, monkeypatch):
+    import torch
+    d = _cpu_cache()
+    monkeypatch.setattr(d, "_ready", lambda batch: None)
+    kw = dict(width=4, first=1, last=2)
+    for wrong in (2 ** 32 + 1, -2 ** 32 + 4, -1):
+        with pytest.raises(ValueError, match=name):
+            d.select(_batch(), torch.zeros((3, 8, 128), dtype=d.dtype), **{**kw, name: wrong})
+
+
 def _calls(cache, batch):
     import torch
     n, h = batch.queries, cache.kv_heads
