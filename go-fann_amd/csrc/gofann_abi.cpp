@@ -726,8 +726,9 @@ int gofann_kv_attention(gofann_ctx* c, const gofann_kv_cache* cache, const gofan
         bool empty = false;
         if (int rc = kv_check(ctx, "kv_attention", cache, batch, &empty)) return rc;
         if (int rc = kv_check_heads(ctx, "kv_attention", cache, heads)) return rc;
-        if (!(scale > 0.0f) || !(scale <= 3.0e38f))
-            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: scale must be positive and finite");
+        // The kernels take it times log2(e).
+        if (!(scale > 0.0f) || !(scale <= 2.35e38f))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: scale must be in (0, 2.35e38]");
         if (blocks != nullptr && (width == 0 || width > (1u << 24)))
             return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: width of a block list must be in [1, 2^24]");
         if (empty) return GOFANN_OK;

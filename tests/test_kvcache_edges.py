@@ -150,6 +150,13 @@ def case_filter_width(f: Kv):
         assert call(h, batch=batch(0, 0)) == f.L.OK
 
 
+def case_scales_past_the_range(f: Kv):
+    """A scale is taken times log2(e): past 2.36e38 that is infinite, and 0 times it no number."""
+    h = f.context()
+    for scale, rc in ((2.4e38, f.L.ERR_INVALID), (3.0e38, f.L.ERR_INVALID), (2.3e38, f.L.OK), (1e-40, f.L.OK)):
+        assert f.attend(h, scale=scale) == rc, scale
+
+
 def case_append_without_a_page_table(f: Kv):
     h = f.context()
     for table in (None, f.p):
