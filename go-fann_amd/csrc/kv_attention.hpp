@@ -129,6 +129,13 @@ __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int 
 // whose weights would otherwise lose, below 2^-25, a tail of many small ones.
 constexpr float kSlack = 8.0f;
 
+// References past this are multiples of 1/2 and more, and a score's weight would
+// be that of its exact product against a rounded one, off by powers of two (from
+// 2^31 on zeros and infinities).  There the products are rounded as the
+// reference was, in the way of a renewal: chunks of 2,048 tokens take 1% longer
+// for it, single tokens what they did.
+constexpr float kFar = 4194304.0f;
+
 // Splits up to which the last workgroup of an item to finish joins them
 // itself; past it the partial results are too many for one workgroup.
 constexpr int kJoinSplits = 16;
@@ -196,38 +203,68 @@ __device__ __forceinline__ void mask_scores(f32x4 (&s)[2], uint32_t mine, int le
     for (int e = 0; e < 8; ++e) s[e / 4][e % 4] = (ok >> e & 1u) ? s[e / 4][e % 4] : -__builtin_inff();
 }
 
-// Weights 2^(score - m) of a row's scores, the row's reference m, sum of
-// weights and weighted values o brought along; mu is m, or 0 while there is
-// none.  The reference is renewed only where a score passes the maximum it was
-// made from by more than kSlack (in powers of two): until then the weights are
-// at most 2^(kSlack + kRaise), which costs 32-bit sums nothing.  The weights
-// enter the product in 16 bits, as the values do; their sum stays in 32.
+// A row's softmax so far.
+struct Row {
+    float m = -__builtin_inff();  // the reference: weights are 2^(scaled score - m)
+    float mu = 0.0f;              // m, or 0 while there is none or it is past kFar
+    float sum = 0.0f;             // of the weights
+};
+
+// The reference renewed by a tile's scaled maximum; returns the factor of what
+// was summed so far.  is_far: it is past kFar, to be taken off by far_score().
+template <class E>
+__device__ __forceinline__ float renew(Row& w, float top, bool& is_far)
+{
+    const float fresh = fmaxf(w.m, top - E::kRaise);
+    const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
+    const float f = __builtin_amdgcn_exp2f(w.m - keep);
+    is_far = __builtin_fabsf(keep) > kFar && __builtin_fabsf(keep) < __builtin_inff();
+    w.m = fresh;
+    w.mu = is_far ? 0.0f : keep;
+    w.sum *= f;
+    return f;
+}
+
+// A score whose scaled value is less by the reference.
+__device__ __forceinline__ float far_score(float s, float scale_log2, float m)
+{
+    return (s * scale_log2 - m) * __builtin_amdgcn_rcpf(scale_log2);
+}
+
+// Weights 2^(score - m) of a row's scores, the row's statistics and weighted
+// values o brought along; far: a row of the wave has a reference past kFar, and
+// all tiles go the way of a renewal.  The reference is renewed only where a
+// score passes the maximum it was made from by more than kSlack (in powers of
+// two): until then the weights are at most 2^(kSlack + kRaise), which costs
+// 32-bit sums nothing.  The weights enter the product in 16 bits, as the values
+// do; their sum stays in 32.
 template <class E, int kUnit>
-__device__ __forceinline__ typename E::V8 weigh(const f32x4 (&s)[2], float scale_log2, float& m,
-                                                float& mu, float& sum, f32x4 (&o)[kUnit])
+__device__ __forceinline__ typename E::V8 weigh(f32x4 (&s)[2], float scale_log2, Row& row, bool& far,
+                                                f32x4 (&o)[kUnit])
 {
     float top = s[0][0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e / 4][e % 4]);
     top *= scale_log2;
-    if (__any(top > m + (kSlack + E::kRaise))) {
+    if (far || __any(top - row.m > kSlack + E::kRaise)) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float fresh = fmaxf(m, top - E::kRaise);
-        const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
-        const float f = __builtin_amdgcn_exp2f(m - keep);
-        sum *= f;
+        bool mine;
+        const float f = renew<E>(row, top, mine);
 #pragma unroll
         for (int c = 0; c < kUnit; ++c) o[c] *= f;
-        m = fresh;
-        mu = keep;
+        far = __any(mine);
+        if (mine) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e / 4][e % 4] = far_score(s[e / 4][e % 4], scale_log2, row.m);
+        }
     }
     typename E::V8 p;
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], scale_log2, -mu));
-        sum += w[e];
+        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4], scale_log2, -row.mu));
+        row.sum += w[e];
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = static_cast<typename E::T>(w[e]);
@@ -268,7 +305,7 @@ struct Raw {
 // ahead, sequences of 500 to 16,000 positions took 9% longer.  Short calls are a chain of dependent loads: 8.6 us
 // for 1,999 positions of 8 heads.
 template <class E, int D, int NT>
-__global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention_kernel(AttendArgs a)
+__global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) void kv_attention_kernel(AttendArgs a)
 {
     using V8 = typename E::V8;
     constexpr int kRows = 16 * NT;
@@ -314,14 +351,12 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
     }
 
     f32x4 o[NT][kUnit];
-    float m[NT], mu[NT], sum[NT];
+    Row st[NT];
+    bool far[NT] = {};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int c = 0; c < kUnit; ++c) o[nt][c] = f32x4{0, 0, 0, 0};
-        m[nt] = -__builtin_inff();
-        mu[nt] = 0.0f;
-        sum[nt] = 0.0f;
     }
 
     // Keys and values of tile `at`, loaded apart: a tile's keys are requested
@@ -469,7 +504,7 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                    p[nt] = weigh<E, kUnit>(s[nt], a.scale_log2, m[nt], mu[nt], sum[nt], o[nt]);
+                    p[nt] = weigh<E, kUnit>(s[nt], a.scale_log2, st[nt], far[nt], o[nt]);
                 value_scales();
                 if constexpr (kMasked) {
                     // A position that no row sees may hold anything: its scale
@@ -490,8 +525,8 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        sum[nt] += __shfl_xor(sum[nt], 16);
-        sum[nt] += __shfl_xor(sum[nt], 32);
+        st[nt].sum += __shfl_xor(st[nt].sum, 16);
+        st[nt].sum += __shfl_xor(st[nt].sum, 32);
     }
 
     // The four waves' maxima, sums and outputs joined through LDS, sixteen
@@ -508,8 +543,8 @@ __global__ __launch_bounds__(256, NT == 1 && D <= 128 ? 4 : 2) void kv_attention
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         if (g4 == 0) {
-            wm[wave][16 * nt + r16] = m[nt];
-            ws[wave][16 * nt + r16] = sum[nt];
+            wm[wave][16 * nt + r16] = st[nt].m;
+            ws[wave][16 * nt + r16] = st[nt].sum;
         }
 #pragma unroll
         for (int x = 0; x < kUnit; ++x) {
@@ -676,7 +711,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
     for (int c = 0; c < kTiles; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
-    float m = -__builtin_inff(), mu = 0.0f, sum = 0.0f;
+    Row st;
+    bool far = false;
 
     // This wave's share of a tile as it is in the cache: the key of one
     // position a lane (row r of S^T is position 16 u + 8 g + 4 a + b for
@@ -814,16 +850,19 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
         top *= a.scale_log2;
-        if (__any(top > m + (kSlack + E::kRaise))) {
+        if (far || __any(top - st.m > kSlack + E::kRaise)) {
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float fresh = fmaxf(m, top - E::kRaise);
-            const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
-            const float f = __builtin_amdgcn_exp2f(m - keep);
-            sum *= f;
+            bool mine;
+            const float f = renew<E>(st, top, mine);
 #pragma unroll
             for (int c = 0; c < kTiles; ++c) o[c] *= f;
-            m = fresh;
-            mu = keep;
+            far = __any(mine);
+            if (mine) {
+#pragma unroll
+                for (int x = 0; x < kPer; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[x][i] = far_score(s[x][i], a.scale_log2, st.m);
+            }
         }
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
@@ -833,8 +872,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
                 float w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][8 * u + e], a.scale_log2, -mu));
-                    sum += w[e];
+                    w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][8 * u + e], a.scale_log2, -st.mu));
+                    st.sum += w[e];
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) p[u][e] = static_cast<typename E::T>(w[e]);
@@ -924,10 +963,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
         run(std::true_type{}, part);
     }
 
-    sum += __shfl_xor(sum, 32);
+    st.sum += __shfl_xor(st.sum, 32);
     if (!in) return;
     uint16_t* const p = a.out.p + (q0 + token) * a.out.token_stride + head * a.out.head_stride;
-    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = st.sum != 0.0f ? 1.0f / st.sum : 0.0f;
     // Rows 8 x + 4 g + y of O^T, y < 4, hold channels dim/32 (8 x + 4 g) ..
 #pragma unroll
     for (int x = 0; x < 4; ++x)
@@ -947,7 +986,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
         }
     if (a.lse != nullptr && g2 == 0)
         a.lse[static_cast<int64_t>(q0 + token) * t.kv_heads * a.group + head] =
-            (m + __builtin_log2f(sum)) * 0.69314718055994531f;
+            (st.m + __builtin_log2f(st.sum)) * 0.69314718055994531f;
 }
 
 // Joins the splits' partial results of one row: four waves a row, wave w the

@@ -193,3 +193,37 @@ def test_a_refused_step_of_the_example_is_as_if_never_made(ctx):
             a.step(q + 1, k + 1, v + 1, 2)  # refused by the choice, once its tokens are written
         assert torch.equal(a.step(q, k, v, width), b.step(q, k, v, width))
         assert torch.equal(a.lengths, b.lengths)
+
+
+# ---- scores of large magnitude -------------------------------------------------
+
+@pytest.mark.parametrize("elem,dim,up", [("bf16", 64, 55), ("bf16", 256, 18), ("bf16", 64, 13), ("bf16", 128, 9),
+                                         ("f16", 256, 13), ("f16", 64, 12), ("f16", 128, 8)])
+@pytest.mark.parametrize("heads,group,new", [(1, 3, 1), (1, 3, 9), (8, 4, 1024)])
+@pytest.mark.parametrize("sign,at", [(1, [10]), (1, [700]), (-1, [700]), (1, [31, 300])])
+def test_attend_of_scores_far_past_the_others_is_a_choice(ctx, elem, dim, up, heads, group, new, sign, at):
+    """Scores of up to 2^118, whose distance is infinite next to a weight's range:
+    the highest position's values are the result, or the mean of two.  sign < 0:
+    every score is as large, and negative."""
+    n = 900 + new
+    b = ref.Batch(64, [n], [new], seed=3)
+    c = ref.Cache(b.pages, heads, 64, dim, elem)
+    r = np.random.default_rng(5)
+    c.k_scales[:], c.v_scales[:] = 127 + up, 127
+    c.k_codes[:] = 0x77 if sign < 0 else 0                      # 6 or 0 in all channels
+    c.v_codes[:] = r.integers(0, 256, c.v_codes.shape)
+    for t in at:
+        c.k_codes[b.table[0, t // 64], :, t % 64] = 0x66 if sign < 0 else 0x77   # 4 or 6
+    v = np.mean([c.read(b.table[0, t // 64], t % 64)[1] for t in at], 0)
+    mass = np.mean([np.abs(c.read(b.table[0, t // 64], t % 64)[1]) for t in at], 0)
+    d, db = device_cache(ctx, c), device_batch(b)
+    for x in (1.125, 1.359375, 1.734375, 1.984375):             # exact in both types
+        q = torch.full((new, heads * group, dim), sign * x * 2.0 ** up, device="cuda").to(d.dtype)
+        lse = torch.empty(new, heads * group, device="cuda")
+        got = d.attend(db, q, lse=lse).double().cpu().numpy().reshape(new, heads, group, dim)
+        u = ref.UNIT[elem]
+        bound = 1.02 * u * (mass + np.abs(v)) + 2.0 ** -25
+        assert (np.abs(got - v[None, :, None]) <= bound[None, :, None]).all(), x
+        top = sign * (4 if sign < 0 else 6) * x * 4.0 ** up * dim ** 0.5 + np.log(len(at))
+        # products and their sum exact, then four roundings in 32 bits
+        assert (np.abs(lse.double().cpu().numpy() - top) <= 4 * 2.0 ** -23 * abs(top)).all()
