@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import kv_reference as ref
-from test_gpu_kvcache import check_attend, device_batch, device_cache, rows
+from test_gpu_kvcache import check_attend, device_batch, device_cache, documents, rows, spread
 
 pytestmark = pytest.mark.gpu
 
@@ -227,3 +227,97 @@ def test_attend_of_scores_far_past_the_others_is_a_choice(ctx, elem, dim, up, he
         top = sign * (4 if sign < 0 else 6) * x * 4.0 ** up * dim ** 0.5 + np.log(len(at))
         # products and their sum exact, then four roundings in 32 bits
         assert (np.abs(lse.double().cpu().numpy() - top) <= 4 * 2.0 ** -23 * abs(top)).all()
+
+
+# ---- long chunks ----------------------------------------------------------------
+
+def sampled(b: ref.Batch, pick):
+    """One-token sequences that are the picked rows of a batch."""
+    tok = {row: (s, p) for row, s, p in b.tokens()}
+    sub = ref.Batch(b.page, [max(0, tok[i][1] + 1) for i in pick], [1] * len(pick), pages=b.pages)
+    sub.table = np.stack([b.table[tok[i][0]] for i in pick])
+    sub.width, sub.visible = b.width, b.visible
+    if b.visible is not None:
+        sub.bits = np.stack([b.bits[tok[i][0]] for i in pick])
+    return sub
+
+
+def random_codes(c: ref.Cache, r):
+    """Every position of the cache written."""
+    for name in ("k_codes", "v_codes"):
+        getattr(c, name)[:] = r.integers(0, 256, getattr(c, name).shape)
+    for name in ("k_scales", "v_scales"):
+        getattr(c, name)[:] = r.integers(124, 128, getattr(c, name).shape)
+
+
+def garbage_where_nothing_is_seen(c: ref.Cache, b: ref.Batch):
+    """Exponents of infinity and NaN at the positions that the filter hides."""
+    for s, n in enumerate(b.lens):
+        for t in range(n):
+            pid = b.page_of(s, t // b.page)
+            if pid >= 0 and not b.sees(s, t):
+                c.k_scales[pid, :, t % b.page] = 255
+                c.v_scales[pid, :, t % b.page // 8, :, t % 8] = 254
+
+
+LONG = [
+    # elem, dim, page, kv heads, group, lengths, new, filter, holes
+    ("bf16", 128, 64, 8, 4, [1300, 500], [700, 400], documents, 0.0),
+    ("bf16", 128, 32, 8, 3, [1300, 500], [1100, 400], None, 0.3),
+    ("f16", 64, 256, 8, 5, [900, 300], [700, 300], documents, 0.2),
+    ("f16", 256, 64, 8, 4, [1150], [1100], lambda s, n, r: r.random(n) < 0.5, 0.1),
+    ("bf16", 256, 128, 8, 4, [1000, 200], [900, 200], documents, 0.0),
+    ("bf16", 64, 32, 2, 20, [700, 100], [800, 100], None, 0.0),     # tokens before position 0
+    ("f16", 128, 64, 8, 4, [1100], [1100], lambda s, n, r: np.zeros(n, bool), 0.0),
+]
+
+
+@pytest.mark.parametrize("elem,dim,page,heads,group,lens,new,filt,holes", LONG)
+def test_long_chunks_under_filters_and_holes(ctx, elem, dim, page, heads, group, lens, new, filt, holes):
+    assert sum(new) * group // 128 * heads >= 256, "not the kernel of long chunks"
+    b = ref.Batch(page, lens, new, seed=dim, holes=holes, visible=filt)
+    c = ref.Cache(b.pages, heads, page, dim, elem, seed=1)
+    r = np.random.default_rng(4)
+    random_codes(c, r)
+    garbage_where_nothing_is_seen(c, b)
+    q, _ = rows(r, b.queries, heads * group, dim, elem)
+    d, db = device_cache(ctx, c), device_batch(b)
+    lse = torch.full((b.queries, heads * group), 1e9, device="cuda")
+    out = d.attend(db, q, lse=lse)
+    assert torch.isfinite(out).all() and (lse < 1e8).all()
+    first = new[0]
+    pick = sorted({0, 1, 31, 32, 127, 300, first // 2, first - 1, first % b.queries, b.queries - 2, b.queries - 1})
+    want = ref.attend(c, sampled(b, pick), q[pick].double().cpu().numpy(), dim ** -0.5)
+    tok = {row: p for row, s, p in b.tokens()}
+    empty = [i for i, row in enumerate(pick) if tok[row] < 0]
+    for w, x in zip(want, (0.0, -np.inf, 0.0)):
+        w[empty] = x
+    check_attend(out[pick], lse[pick], *want)
+    assert torch.equal(out, d.attend(db, q)), "two runs differ"
+    odd = spread(torch.zeros_like(q))
+    d.attend(db, spread(q), out=odd)
+    assert torch.equal(out, odd), "strides change the result"
+    swapped = torch.empty((heads * group, b.queries, dim), dtype=q.dtype, device="cuda").transpose(0, 1)
+    d.attend(db, q.transpose(0, 1).contiguous().transpose(0, 1), out=swapped)
+    assert torch.equal(out, swapped), "the order of tokens and heads changes the result"
+
+
+@pytest.mark.parametrize("elem,dim,group,edge", [("bf16", 128, 4, [16, 17, 31, 32, 33]), ("f16", 64, 1, [63, 64, 65, 127, 128, 129])])
+def test_sequences_of_about_the_rows_that_long_chunks_leave(ctx, elem, dim, group, edge):
+    """64 rows and fewer go to the other kernel, 65 and more do not."""
+    heads, page = 8, 64
+    new = [4200 // group * 2] + edge + [1]
+    lens = [new[0]] + [n + 150 for n in edge] + [200]
+    assert sum(new) * group // 128 * heads >= 256
+    b = ref.Batch(page, lens, new, seed=2)
+    c = ref.Cache(b.pages, heads, page, dim, elem, seed=1)
+    r = np.random.default_rng(4)
+    random_codes(c, r)
+    q, _ = rows(r, b.queries, heads * group, dim, elem)
+    lse = torch.full((b.queries, heads * group), 1e9, device="cuda")
+    out = torch.full_like(q, 99.0)
+    device_cache(ctx, c).attend(device_batch(b), q, out=out, lse=lse)
+    assert (out != 99.0).any(-1).all() and (lse < 1e8).all()
+    pick = [0] + [int(b.offsets[s]) + i for s in range(1, len(new)) for i in {0, new[s] // 2, new[s] - 1}]
+    want = ref.attend(c, sampled(b, pick), q[pick].double().cpu().numpy(), dim ** -0.5)
+    check_attend(out[pick], lse[pick], *want)
