@@ -163,6 +163,40 @@ def test_a_chunk_beside_many_short_sequences(ctx, elem, dim, page, heads, group,
                  *ref.attend(c, b, q64, dim ** -0.5, blocks.cpu().numpy()))
 
 
+def test_more_row_tiles_than_one_axis_of_a_grid(ctx):
+    """65,000 sequences of one token beside one of 200."""
+    from gofann_amd import kvcache
+    n = 65_000
+    d = kvcache.KvCache.empty(ctx, pages=300, kv_heads=1, dim=64, page=32)
+    r = np.random.default_rng(1)
+    for t in (d.k_codes, d.v_codes):
+        t.random_(0, 256)
+    for t in (d.k_scales, d.v_scales):
+        t.random_(124, 128)
+    new = np.ones(n + 1, np.int64)
+    new[40_000] = 200
+    lens = np.where(new == 1, r.integers(1, 65, n + 1), 256)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()  # noqa: E731
+    table = r.integers(0, 300, (n + 1, 8))
+    off = np.concatenate(([0], np.cumsum(new)))
+    q, _ = rows(r, int(off[-1]), 1, 64, "bf16")
+    lse = torch.full((int(off[-1]), 1), 1e9, device="cuda")
+    out = d.attend(kvcache.KvBatch(dev(table), dev(lens), dev(off), queries=int(off[-1]), max_queries=200,
+                                   max_length=256), q, lse=lse)
+    # every token as a sequence of its own, no more than a launch takes at once
+    seq = np.repeat(np.arange(n + 1), new)
+    pos = lens[seq] - new[seq] + np.arange(int(off[-1])) - off[seq]
+    for i in range(0, int(off[-1]), 40_000):
+        j = min(i + 40_000, int(off[-1]))
+        one = kvcache.KvBatch(dev(table[seq[i:j]]), dev(pos[i:j] + 1), max_length=256)
+        each = torch.empty((j - i, 1), device="cuda")
+        want = d.attend(one, q[i:j], lse=each)
+        # one bf16 rounding of the weights and one of the result in each
+        assert ((out[i:j].float() - want.float()).abs() <= 4 * 2.0 ** -8 * 12).all()
+        assert (out[i:j].float() - want.float()).abs().mean() < 1e-2
+        assert ((lse[i:j] - each).abs() <= 1e-4).all()
+
+
 def test_row_tiles_of_rows_the_batch_does_not_have(ctx):
     """Offsets that leave rows out, before the first sequence and past the last."""
     from gofann_amd import kvcache
