@@ -65,8 +65,11 @@ struct Context {
     // allocation in the default capture mode would break.
     void* optional_scratch(int slot, size_t bytes);
     // The same for a buffer whose address a captured graph may keep: where it
-    // must grow, the old one stays until gofann_destroy (sizes at least double,
-    // so all of them hold no more than twice the last).  nullptr, with the
+    // must grow, the old one stays until gofann_destroy.  Sizes at least double,
+    // so all of them hold no more than twice the last, while memory for double
+    // can be had; where it cannot, a buffer grows to what is needed.  Calls of
+    // the context and replays of its graphs share it: the caller orders them, as
+    // calls on one stream are.  nullptr, with the
     // reason in `error`, on failure and where the stream is captured and the
     // buffer too small.
     void* workspace(int slot, size_t bytes);

@@ -299,11 +299,13 @@ struct Raw {
 //
 // Four waves take every fourth tile each and are joined through LDS; splits of
 // the positions fill the chip where there are few rows.  HBM bounds long calls:
-// one token of 64 heads over 500,001 positions (544 MB) takes 100 us, 5.4 TB/s
-// (a large copy: 4.8), and 11 us for the join of 96 splits.  At 126 registers
-// four workgroups are resident a CU; with three, and masked tiles not yet loaded
-// ahead, sequences of 500 to 16,000 positions took 9% longer.  Short calls are a chain of dependent loads: 8.6 us
-// for 1,999 positions of 8 heads.
+// one token of 64 heads over 500,001 positions (544 MB) takes 98 us, 5.6 TB/s
+// (a large copy, read and written: 4.8), and 11 us for the join of 96 splits.
+// At 128 channels it has 128 registers and four workgroups resident a CU; with
+// three, and masked tiles not yet loaded ahead, sequences of 500 to 16,000
+// positions took 9% longer.  64 channels: five; 256: two, by 201 registers and
+// by the 69 KB of LDS that join the waves.  Short calls are a chain of dependent
+// loads: 8.6 us for 1,999 positions of 8 heads.
 template <class E, int D, int NT>
 __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) void kv_attention_kernel(AttendArgs a)
 {
@@ -593,9 +595,11 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
     if (a.arrived == nullptr) return;
     // The workgroup that arrives last joins the splits, in their order
     // whichever that is.  Every access to the partial results is an atomic
-    // of the whole device (put, get), which no XCD's cache holds back, so
-    // their completion is all that the count has to wait for; a fence of
-    // the device would write back the XCD's cache and take 5 us a call.
+    // of the whole device (put2, get2: as compiled, stores and loads with sc1
+    // set, which write through the XCD's cache and read past it), so their
+    // completion is all that the count has to wait for.  A release fence of
+    // the device is the same wait behind a write-back of the XCD's cache, for
+    // plain stores that there are none of here; it took 5 us a call.
     __shared__ int last;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -656,11 +660,13 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
 //
 // 2,048 tokens of 32 heads over 16,390 positions, 516 GFLOP: 0.52 to 0.63 ms by
 // the chip's clock, 990 to 820 TFLOP/s, 0.72 to 0.60 of what a large matrix
-// product of the library reaches.  The chip's power seems to bound it: with 64
-// rows a wave, one workgroup a CU, 256 workgroups took 700 us each and 128 of
-// the same 322; and one or two tiles a turn, or scores formed a turn ahead of
-// their softmax, end within 3% of each other.  Without LDS, each wave
-// converting for itself (16 x 16 products): 0.69 ms where this took 0.63.
+// product of the library reaches.  The chip's power may bound it, which no
+// recorded clock shows: with 64 rows a wave, one workgroup a CU, 256 workgroups
+// took more than twice as long as 128 of the same did on half of the CUs; and
+// one or two tiles a turn, or scores formed a turn ahead of their softmax, end
+// within 3% of each other.  Without LDS, each wave converting for itself (16 x
+// 16 products): 0.69 ms where this took 0.63.  At 256 channels (1.44 ms) the
+// output and the queries leave 29 registers too few, spilled.
 template <class E, int D>
 __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
 {

@@ -13,8 +13,8 @@ constexpr int kFewRows = 64;
 // so that the chip is full all the same.
 constexpr uint64_t kPartBytes = 512ull << 20;
 
-// Tiles of a split of `items` row tiles of at most `most` tiles: enough
-// workgroups that all of them are resident at once, at least one tile a wave,
+// Tiles of a split of `items` row tiles of at most `most` tiles: three workgroups
+// a CU (two to five are resident, by the kernel), at least one tile a wave,
 // and where sequences may differ in length at most 48, so that a long one does
 // not outlast the others: 48 sequences of 500 to 16,000 positions take 64 us
 // with 16, 55 with 32, 52 with 48 and 56 with 64; 8 of them 19, 21, 18 and 18.

@@ -488,8 +488,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_select_kernel(Select
     }
     if constexpr (kMany) return;
     if (chunks > 1) {
-        // The keys are atomics of the whole device, so that their completion
-        // is all that the count has to wait for.
+        // The keys are atomics of the whole device (as compiled, stores and
+        // loads with sc1 set, which no XCD's cache holds back), so that their
+        // completion is all that the count has to wait for.
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (threadIdx.x == 0) {

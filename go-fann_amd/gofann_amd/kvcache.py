@@ -16,8 +16,10 @@ those reads nothing else.  The reference has no counterpart.
     out = cache.attend(batch, q, blocks=cache.select(batch, q, 64))
 
 Calls are asynchronous on the context's stream, which has to be torch's
-current one.  Everything may be captured in a graph once a call of the same
-sizes has run.
+current one, on the context's device.  Everything may be captured in a graph
+once a call of the same sizes has run.  The graph then uses the context's
+scratch: order its replays with each other and with the context's other calls,
+as work on one stream is.
 """
 from __future__ import annotations
 

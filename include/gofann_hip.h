@@ -958,7 +958,13 @@ int gofann_build_reach(gofann_ctx* ctx, const uint32_t* graph, uint32_t n, uint3
  * least with max|x| <= 6 * 2^e, clamped to [-125, 125] (BF16) or [-23, 13]
  * (F16); code = the nearest of {0, .5, 1, 1.5, 2, 3, 4, 6} to |x| / 2^e,
  * halfway to the even code, in bits 2:0, the sign of x in bit 3.  A NaN is
- * held as zero, an infinity (left out of max|x|) as the group's largest. */
+ * held as zero, an infinity (left out of max|x|) as the group's largest.
+ *
+ * Calls are asynchronous on the context's stream and use its scratch, which
+ * only grows.  Under stream capture a call needs that a call of its sizes ran
+ * before (else GOFANN_ERR_NOMEM); the graph then keeps the scratch's address,
+ * so its replays have to be ordered with each other and with all other calls
+ * of the context, as work on one stream is. */
 typedef struct {
     uint8_t* k_codes;  /* [pages][kv_heads][page_size][dim/2], low nibble: even channel */
     uint8_t* k_scales; /* [pages][kv_heads][page_size][dim/32], e + 127 */
@@ -1026,7 +1032,7 @@ int gofann_kv_append(gofann_ctx* ctx, const gofann_kv_cache* cache, const gofann
  * with eq[h] = x - 7 for 2^(x-1) <= max|q[h]| < 2^x, clamped to [-125, 125],
  * q8 = q / 2^eq rounded to nearest even and clamped to [-127, 127] (NaN: 0;
  * infinities left out of the maximum): whole numbers, so no order of
- * summation changes the choice. */
+ * summation changes the choice.  Scores are compared as 32-bit floats. */
 int gofann_kv_select(gofann_ctx* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
                      const gofann_kv_rows* q, uint32_t heads, uint32_t width, uint32_t first,
                      uint32_t last, int32_t* out_blocks);
@@ -1037,7 +1043,10 @@ int gofann_kv_select(gofann_ctx* ctx, const gofann_kv_cache* cache, const gofann
  * any order; negative: none).  Head h reads key/value head
  * h / (heads / kv_heads).  A row with no position left gives zeros.
  * out_lse (optional) [queries][heads]: the natural log of the sum of
- * exponentials, -inf for such a row. */
+ * exponentials, -inf for such a row.  Scores, their maximum and the sum are
+ * held in 32 bits; the weights are rounded to the element type before they
+ * meet the values, the result once more.  Rows of out that no sequence has are
+ * left as they are. */
 int gofann_kv_attention(gofann_ctx* ctx, const gofann_kv_cache* cache,
                         const gofann_kv_batch* batch, const gofann_kv_rows* q, uint32_t heads,
                         float scale, const int32_t* blocks, uint32_t width,
