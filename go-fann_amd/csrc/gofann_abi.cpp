@@ -169,6 +169,28 @@ bool kv_rows(const gofann_kv_rows* r)
     return r != nullptr && r->data != nullptr && aligned(r->data, 2);
 }
 
+int kv_check_batch(Context* ctx, const std::string& at, const gofann_kv_batch* b, bool* empty)
+{
+    if (b->sequences > 65535)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "at most 65535 sequences");
+    if (b->queries > 0x7FFFFFFFu || b->max_length > 0x7FFFFF00u || b->table_width > 0x7FFFFFu)
+        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "queries, max_length or table_width too large");
+    *empty = b->sequences == 0 || b->queries == 0 ||
+             (b->query_offsets != nullptr && b->max_queries == 0);
+    if (*empty) return GOFANN_OK;
+    if (b->lengths == nullptr || (b->page_table == nullptr && b->table_width > 0))
+        return ctx->fail(GOFANN_ERR_INVALID, at + "page_table or lengths is null");
+    if (b->table_stride < b->table_width)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "table_stride below table_width");
+    if (b->visible != nullptr && b->visible_stride < b->visible_width)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "visible_stride below visible_width");
+    if (b->query_offsets == nullptr && b->queries != b->sequences)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "without query_offsets there is one token a sequence");
+    if (b->query_offsets != nullptr && b->max_queries > b->queries)
+        return ctx->fail(GOFANN_ERR_INVALID, at + "max_queries above queries");
+    return GOFANN_OK;
+}
+
 int kv_check(Context* ctx, const char* call, const gofann_kv_cache* c, const gofann_kv_batch* b, bool* empty)
 {
     const std::string at = std::string(call) + ": ";
@@ -192,24 +214,7 @@ int kv_check(Context* ctx, const char* call, const gofann_kv_cache* c, const gof
         return ctx->fail(GOFANN_ERR_INVALID, at + "codes and boxes must be 16-byte aligned, v_scales 8-byte");
     if ((c->box == nullptr) != (c->box_scale == nullptr))
         return ctx->fail(GOFANN_ERR_INVALID, at + "box and box_scale come together");
-    if (b->sequences > 65535)
-        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "at most 65535 sequences");
-    if (b->queries > 0x7FFFFFFFu || b->max_length > 0x7FFFFF00u || b->table_width > 0x7FFFFFu)
-        return ctx->fail(GOFANN_ERR_UNSUPPORTED, at + "queries, max_length or table_width too large");
-    *empty = b->sequences == 0 || b->queries == 0 ||
-             (b->query_offsets != nullptr && b->max_queries == 0);
-    if (*empty) return GOFANN_OK;
-    if (b->lengths == nullptr || (b->page_table == nullptr && b->table_width > 0))
-        return ctx->fail(GOFANN_ERR_INVALID, at + "page_table or lengths is null");
-    if (b->table_stride < b->table_width)
-        return ctx->fail(GOFANN_ERR_INVALID, at + "table_stride below table_width");
-    if (b->visible != nullptr && b->visible_stride < b->visible_width)
-        return ctx->fail(GOFANN_ERR_INVALID, at + "visible_stride below visible_width");
-    if (b->query_offsets == nullptr && b->queries != b->sequences)
-        return ctx->fail(GOFANN_ERR_INVALID, at + "without query_offsets there is one token a sequence");
-    if (b->query_offsets != nullptr && b->max_queries > b->queries)
-        return ctx->fail(GOFANN_ERR_INVALID, at + "max_queries above queries");
-    return GOFANN_OK;
+    return kv_check_batch(ctx, at, b, empty);
 }
 
 int kv_check_heads(Context* ctx, const char* call, const gofann_kv_cache* c, uint32_t heads)
@@ -217,6 +222,24 @@ int kv_check_heads(Context* ctx, const char* call, const gofann_kv_cache* c, uin
     if (heads == 0 || heads % c->kv_heads != 0 || heads / c->kv_heads > 1024)
         return ctx->fail(GOFANN_ERR_INVALID,
                          std::string(call) + ": heads must be 1 to 1024 times kv_heads");
+    return GOFANN_OK;
+}
+
+int kv_check_attention(Context* ctx, const char* call, const gofann_kv_cache* cache,
+                       const gofann_kv_batch* batch, const gofann_kv_rows* q, uint32_t heads, float scale,
+                       const int32_t* blocks, uint32_t width, const gofann_kv_rows* out, bool* empty)
+{
+    const std::string at = std::string(call) + ": ";
+    if (int rc = kv_check(ctx, call, cache, batch, empty)) return rc;
+    if (int rc = kv_check_heads(ctx, call, cache, heads)) return rc;
+    // The kernels take it times log2(e).
+    if (!(scale > 0.0f) || !(scale <= 2.35e38f))
+        return ctx->fail(GOFANN_ERR_INVALID, at + "scale must be in (0, 2.35e38]");
+    if (blocks != nullptr && (width == 0 || width > (1u << 24)))
+        return ctx->fail(GOFANN_ERR_INVALID, at + "width of a block list must be in [1, 2^24]");
+    if (*empty) return GOFANN_OK;
+    if (!kv_rows(q) || !kv_rows(out))
+        return ctx->fail(GOFANN_ERR_INVALID, at + "q or out rows missing or misaligned");
     return GOFANN_OK;
 }
 }  // namespace
@@ -724,17 +747,122 @@ int gofann_kv_attention(gofann_ctx* c, const gofann_kv_cache* cache, const gofan
 {
     return guarded(c, [&](Context* ctx) {
         bool empty = false;
-        if (int rc = kv_check(ctx, "kv_attention", cache, batch, &empty)) return rc;
-        if (int rc = kv_check_heads(ctx, "kv_attention", cache, heads)) return rc;
-        // The kernels take it times log2(e).
-        if (!(scale > 0.0f) || !(scale <= 2.35e38f))
-            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: scale must be in (0, 2.35e38]");
-        if (blocks != nullptr && (width == 0 || width > (1u << 24)))
-            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: width of a block list must be in [1, 2^24]");
+        if (int rc = kv_check_attention(ctx, "kv_attention", cache, batch, q, heads, scale, blocks, width,
+                                        out, &empty))
+            return rc;
         if (empty) return GOFANN_OK;
-        if (!kv_rows(q) || !kv_rows(out))
-            return ctx->fail(GOFANN_ERR_INVALID, "kv_attention: q or out rows missing or misaligned");
         return gofann::kv_attention(ctx, cache, batch, q, heads, scale, blocks, width, out, out_lse);
+    });
+}
+
+int gofann_kv_draft_attention(gofann_ctx* c, const gofann_kv_cache* cache,
+                              const gofann_kv_batch* batch, const gofann_kv_rows* q, uint32_t heads,
+                              float scale, const uint32_t* sees, uint32_t sees_width,
+                              uint32_t sees_stride, const int32_t* blocks, uint32_t width,
+                              const gofann_kv_rows* out, float* out_lse)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (int rc = kv_check_attention(ctx, "kv_draft_attention", cache, batch, q, heads, scale, blocks,
+                                        width, out, &empty))
+            return rc;
+        if (sees_width > sees_stride || sees_width > 0x7FFFFFFu)
+            return ctx->fail(GOFANN_ERR_INVALID,
+                             "kv_draft_attention: sees_width must be below 2^27 and at most sees_stride");
+        if (empty) return GOFANN_OK;
+        if (sees == nullptr || !aligned(sees, 4))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_attention: sees missing or misaligned");
+        gofann::KvReach reach;
+        reach.sees = sees;
+        reach.sees_width = sees_width;
+        reach.sees_stride = sees_stride;
+        return gofann::kv_attention(ctx, cache, batch, q, heads, scale, blocks, width, out, out_lse, reach);
+    });
+}
+
+int gofann_kv_cross_attention(gofann_ctx* c, const gofann_kv_cache* cache,
+                              const gofann_kv_batch* batch, const gofann_kv_rows* q, uint32_t heads,
+                              float scale, const gofann_kv_rows* out, float* out_lse)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (int rc = kv_check_attention(ctx, "kv_cross_attention", cache, batch, q, heads, scale, nullptr,
+                                        0, out, &empty))
+            return rc;
+        if (empty) return GOFANN_OK;
+        gofann::KvReach reach;
+        reach.cross = true;
+        return gofann::kv_attention(ctx, cache, batch, q, heads, scale, nullptr, 0, out, out_lse, reach);
+    });
+}
+
+int gofann_kv_read(gofann_ctx* c, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                   const gofann_kv_rows* k, const gofann_kv_rows* v)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (int rc = kv_check(ctx, "kv_read", cache, batch, &empty)) return rc;
+        if (empty) return GOFANN_OK;
+        if (k == nullptr && v == nullptr)
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_read: neither keys nor values are asked for");
+        if ((k && !kv_rows(k)) || (v && !kv_rows(v)))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_read: k or v rows missing or misaligned");
+        return gofann::kv_read(ctx, cache, batch, k, v);
+    });
+}
+
+int gofann_kv_draft_tree(gofann_ctx* c, const gofann_kv_batch* batch, const int32_t* parents,
+                         uint32_t words, uint32_t* out_sees, int32_t* out_depths)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (batch == nullptr) return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_tree: null batch");
+        if (int rc = kv_check_batch(ctx, "kv_draft_tree: ", batch, &empty)) return rc;
+        if (words > 0x7FFFFFFu) return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_tree: too many words");
+        if (empty) return GOFANN_OK;
+        if (parents == nullptr || !aligned(parents, 4) || !aligned(out_sees, 4) || !aligned(out_depths, 4))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_tree: parents missing, or an array misaligned");
+        if (out_sees == nullptr && out_depths == nullptr)
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_tree: neither bits nor depths are asked for");
+        return gofann::kv_draft_tree(ctx, batch, parents, words, out_sees, out_depths);
+    });
+}
+
+int gofann_kv_draft_accept(gofann_ctx* c, const gofann_kv_batch* batch, const int32_t* parents,
+                           const int32_t* drafted, const int32_t* chosen, uint32_t width,
+                           int32_t* out_path, int32_t* out_lengths, int32_t* out_next)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (batch == nullptr) return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_accept: null batch");
+        if (int rc = kv_check_batch(ctx, "kv_draft_accept: ", batch, &empty)) return rc;
+        if (width == 0 || width > (1u << 24))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_accept: width must be in [1, 2^24]");
+        // Without a token there is a path too, an empty one.
+        if (batch->sequences == 0) return GOFANN_OK;
+        if (batch->lengths == nullptr)
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_accept: lengths is null");
+        if (!empty && (parents == nullptr || drafted == nullptr || chosen == nullptr))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_accept: parents, drafted or chosen is null");
+        if (out_path == nullptr || !aligned(out_path, 4) || !aligned(parents, 4) || !aligned(drafted, 4) ||
+            !aligned(chosen, 4) || !aligned(out_lengths, 4) || !aligned(out_next, 4))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_draft_accept: out_path missing, or an array misaligned");
+        return gofann::kv_draft_accept(ctx, batch, parents, drafted, chosen, width, out_path, out_lengths,
+                                       out_next);
+    });
+}
+
+int gofann_kv_keep(gofann_ctx* c, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                   const int32_t* path, uint32_t width)
+{
+    return guarded(c, [&](Context* ctx) {
+        bool empty = false;
+        if (int rc = kv_check(ctx, "kv_keep", cache, batch, &empty)) return rc;
+        if (width > (1u << 24)) return ctx->fail(GOFANN_ERR_INVALID, "kv_keep: width must be at most 2^24");
+        if (empty) return GOFANN_OK;
+        if ((path == nullptr && width > 0) || !aligned(path, 4))
+            return ctx->fail(GOFANN_ERR_INVALID, "kv_keep: path missing or misaligned");
+        return gofann::kv_keep(ctx, cache, batch, path, width);
     });
 }
 

@@ -245,8 +245,25 @@ int kv_append(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch*
 int kv_select(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
               const gofann_kv_rows* q, uint32_t heads, uint32_t width, uint32_t first,
               uint32_t last, int32_t* out_blocks);
+// Which positions tokens attend to beside those up to their own: `sees` bits
+// among the call's tokens, or all positions of a sequence that they are no part of.
+struct KvReach {
+    bool cross = false;
+    const uint32_t* sees = nullptr;
+    uint32_t sees_width = 0;
+    uint32_t sees_stride = 0;
+};
 int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
                  const gofann_kv_rows* q, uint32_t heads, float scale, const int32_t* blocks,
-                 uint32_t width, const gofann_kv_rows* out, float* out_lse);
+                 uint32_t width, const gofann_kv_rows* out, float* out_lse, const KvReach& reach = {});
+int kv_read(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+            const gofann_kv_rows* k, const gofann_kv_rows* v);
+int kv_draft_tree(Context* ctx, const gofann_kv_batch* batch, const int32_t* parents, uint32_t words,
+                  uint32_t* out_sees, int32_t* out_depths);
+int kv_draft_accept(Context* ctx, const gofann_kv_batch* batch, const int32_t* parents,
+                    const int32_t* drafted, const int32_t* chosen, uint32_t width, int32_t* out_path,
+                    int32_t* out_lengths, int32_t* out_next);
+int kv_keep(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+            const int32_t* path, uint32_t width);
 
 }  // namespace gofann

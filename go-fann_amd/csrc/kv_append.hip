@@ -66,14 +66,6 @@ __device__ __forceinline__ Octet<E> quantize(u32x4 raw)
     return o;
 }
 
-template <class E>
-__device__ __forceinline__ u32x4 held(uint32_t codes, uint32_t exponent)
-{
-    const uint32_t s = exponent << 23;
-    return u32x4{E::template decode<0>(codes, s), E::template decode<1>(codes, s),
-                 E::template decode<2>(codes, s), E::template decode<3>(codes, s)};
-}
-
 // A workgroup takes one page of one key/value head.  Eight channels a thread,
 // D / 8 threads a token, 256 / (D / 8) tokens at a time.  With a box to renew
 // the page's earlier tokens are decoded again: the box depends on the page's
@@ -172,35 +164,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a)
     }
     if (!boxed) return;
 
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        most[row][8 * lane + i] = hi[i];
-        least[row][8 * lane + i] = lo[i];
-    }
-    __syncthreads();
-    const int c = threadIdx.x % D;
-    float mh = -__builtin_inff(), ml = __builtin_inff();
-    for (int r = 0; r < kTokens; ++r) {
-        mh = fmaxf(mh, most[r][c]);
-        ml = fminf(ml, least[r][c]);
-    }
-    float amax = fmaxf(__builtin_fabsf(mh), __builtin_fabsf(ml));
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
-    if (threadIdx.x % 64 == 0) amax_part[threadIdx.x / 64] = amax;
-    __syncthreads();
-    amax = fmaxf(fmaxf(amax_part[0], amax_part[1]), fmaxf(amax_part[2], amax_part[3]));
-    // Exact: the values are codes times powers of two, so amax = m 2^t has
-    // m 2^7 <= 127, and so is the division by a power of two.
-    int e = __builtin_amdgcn_frexp_expf(amax) - 7;
-    e = e < -125 ? -125 : e > 125 ? 125 : e;
-    if (!(amax > 0.0f)) e = -125;
-    const float inv = __builtin_bit_cast(float, static_cast<uint32_t>(127 - e) << 23);
-    if (static_cast<int>(threadIdx.x) < D) {
-        a.box[ph * 2 * D + c] = static_cast<int8_t>(__builtin_ceilf(mh * inv));
-        a.box[ph * 2 * D + D + c] = static_cast<int8_t>(__builtin_floorf(ml * inv));
-    }
-    if (threadIdx.x == 0) a.box_scale[ph] = static_cast<uint8_t>(e + 127);
+    join_box<D>(hi, lo, most, least, amax_part, a.box + ph * 2 * D, a.box_scale + ph);
 }
 
 template <class E>

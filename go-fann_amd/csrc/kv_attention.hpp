@@ -32,7 +32,16 @@ struct AttendArgs {
     int part_rows;          // sequence so many where that is not 0
     int slots;              // row tiles counted through the sequences; 0: a grid of them
     int sequences;
+    const uint32_t* sees;   // kDraft: [queries][sees_stride] words, sees_width used
+    int64_t sees_stride;
+    int sees_width;
 };
+
+// Which positions a token may look at, the filter apart: those up to its own;
+// those before its sequence's tokens and of these the ones that its `sees` bits
+// name; or all of a sequence that it is no part of.  Each is compiled by itself,
+// so that the first has nothing to carry for the others.
+enum Reach { kOwn = 0, kDraft = 1, kCross = 2 };
 
 // What a workgroup works on: row tile `index` of sequence b, the id-th of all.
 struct Item {
@@ -97,11 +106,12 @@ __device__ __forceinline__ int64_t part_of(const AttendArgs& a, int b, int q0, i
 // (token, head of the group) rows, and the positions they reach.
 struct RowTile {
     int begin, end;
-    int first_pos;            // of the first row's token
-    int last_pos;             // of the last row's, or the last that may have a page
+    int first_pos;            // the last that every row sees: the first row's token's
+    int last_pos;             // the last that any row sees, or that may have a page
     int token;                // listed: the one token
 };
 
+template <int kReach>
 __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int rows, int len, int n)
 {
     RowTile t;
@@ -117,8 +127,13 @@ __device__ __forceinline__ RowTile row_tile(const AttendArgs& a, int index, int 
     }
     if (n * a.group <= a.rows_over || n * a.group > a.rows_upto) t.end = t.begin;
     if (t.end > t.begin + rows) t.end = t.begin + rows;
-    t.first_pos = len - n + t.begin / a.group;
-    t.last_pos = len - n + (t.end - 1) / a.group;
+    if constexpr (kReach == kOwn) {
+        t.first_pos = len - n + t.begin / a.group;
+        t.last_pos = len - n + (t.end - 1) / a.group;
+    } else {
+        t.first_pos = kReach == kDraft ? len - n - 1 : len - 1;
+        t.last_pos = len - 1;
+    }
     if (t.last_pos >= a.batch.max_positions) t.last_pos = a.batch.max_positions - 1;
     return t;
 }
@@ -201,6 +216,38 @@ __device__ __forceinline__ void mask_scores(f32x4 (&s)[2], uint32_t mine, int le
     const uint32_t ok = mine & ((1u << left) - 1u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e / 4][e % 4] = (ok >> e & 1u) ? s[e / 4][e % 4] : -__builtin_inff();
+}
+
+// The bits of a draft's token (row `row` of `sees`) for the 32 positions that
+// begin `rel` past the draft's first: positions before that are all seen.  Two
+// words, loaded ahead of their use.
+struct Sees {
+    uint32_t lo, hi;
+};
+__device__ __forceinline__ Sees load_sees(const AttendArgs& a, int row, int rel)
+{
+    Sees s{0, 0};
+    const int w = rel >> 5;
+    const uint32_t* const p = a.sees + static_cast<int64_t>(row) * a.sees_stride;
+    if (row >= 0 && w >= 0 && w < a.sees_width) s.lo = p[w];
+    if (row >= 0 && w >= -1 && w + 1 < a.sees_width) s.hi = p[w + 1];
+    return s;
+}
+__device__ __forceinline__ uint32_t sees_bits(Sees s, int row, int rel)
+{
+    uint32_t v = __builtin_amdgcn_alignbit(s.hi, s.lo, rel & 31);
+    if (rel < 0) v |= rel <= -32 ? 0xFFFFFFFFu : (1u << -rel) - 1u;
+    return row < 0 ? 0u : v;
+}
+
+// The scale of a position that was never written may be anything, and a weight
+// of zero times an infinity or NaN is NaN: exponents that append writes to no
+// group become 1.
+template <class E>
+__device__ __forceinline__ uint32_t written_scale(uint32_t scale)
+{
+    const uint32_t e = scale >> 23 & 255u;
+    return e - (127 + E::kMinExp) <= static_cast<uint32_t>(E::kMaxExp - E::kMinExp) ? scale : 127u << 23;
 }
 
 // A row's softmax so far.
@@ -306,7 +353,7 @@ struct Raw {
 // positions took 9% longer.  64 channels: five; 256: two, by 201 registers and
 // by the 69 KB of LDS that join the waves.  Short calls are a chain of dependent
 // loads: 8.6 us for 1,999 positions of 8 heads.
-template <class E, int D, int NT>
+template <class E, int D, int kReach, int NT>
 __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) void kv_attention_kernel(AttendArgs a)
 {
     using V8 = typename E::V8;
@@ -324,7 +371,7 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
     const int len = t.length(b);
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
-    const RowTile rt = row_tile(a, index, kRows, len, n);
+    const RowTile rt = row_tile<kReach>(a, index, kRows, len, n);
     if (rt.end <= rt.begin) return;
     const int tiles = tiles_of(a, rt);
     const int tile_begin = split * a.split_tiles;
@@ -333,7 +380,8 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
     const int hi_pos = rt.last_pos + 1;                         // positions that are read
     const int all_see = rt.first_pos + 1;                       // positions that every row sees
 
-    // The rows' queries and limits.
+    // The rows' queries and limits: positions that they see, or, of a draft's
+    // tokens, the row of their bits (-1: not a row).
     V8 q[NT][D / 32];
     int limit[NT];
 #pragma unroll
@@ -342,7 +390,7 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
         const bool in = row < rt.end;
         const int i = (in ? row : rt.begin) / a.group;
         const int head = h * a.group + (in ? row : rt.begin) % a.group;
-        limit[nt] = in ? len - n + i + 1 : 0;
+        limit[nt] = kReach == kDraft ? (in ? q0 + i : -1) : !in ? 0 : kReach == kCross ? len : len - n + i + 1;
         const uint16_t* const p = a.q.p + (q0 + i) * a.q.token_stride + head * a.q.head_stride;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
@@ -495,14 +543,25 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
                 const bool more = live != 0;
                 const int next = more ? __builtin_ctzll(live) : i;
                 const uint32_t ahead = __builtin_amdgcn_readlane(at, next);
+                const int first = __builtin_amdgcn_readlane(t0, i);
+                [[maybe_unused]] const int rel = first - (len - n);
+                [[maybe_unused]] Sees sees[NT];
+                if constexpr (kMasked && kReach == kDraft) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) sees[nt] = load_sees(a, limit[nt], rel);
+                }
                 scores();
                 if (more) load_keys(ahead);
                 uint32_t mine = 0;
                 if constexpr (kMasked) {
-                    const int from = __builtin_amdgcn_readlane(t0, i) + 8 * g4;
                     mine = static_cast<uint32_t>(__builtin_amdgcn_readlane(word, i)) >> (8 * g4);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mask_scores(s[nt], mine, limit[nt] - from);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if constexpr (kReach == kDraft)
+                            mask_scores(s[nt], mine & sees_bits(sees[nt], limit[nt], rel) >> (8 * g4), 8);
+                        else
+                            mask_scores(s[nt], mine, limit[nt] - (first + 8 * g4));
+                    }
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -512,8 +571,10 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
                     // A position that no row sees may hold anything: its scale
                     // must not turn a weight of zero into a NaN.
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
+                    for (int e = 0; e < 8; ++e) {
                         if (!(mine >> e & 1u)) scale[e] = 127u << 23;
+                        if constexpr (kReach == kDraft) scale[e] = written_scale<E>(scale[e]);
+                    }
                 }
                 product();
                 if (!more) break;
@@ -688,7 +749,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
     const int len = t.length(b);
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
-    const RowTile all = row_tile(a, index, 4 * kRows, len, n);
+    const RowTile all = row_tile<kOwn>(a, index, 4 * kRows, len, n);
     if (all.end <= all.begin) return;
     const int tiles = tiles_of(a, all);
     const int hi_pos = all.last_pos + 1;
@@ -997,7 +1058,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
 
 // Joins the splits' partial results of one row: four waves a row, wave w the
 // splits w, w + 4, .., each lane D / 64 channels.
-template <class E, int D, int NT>
+template <class E, int D, int kReach, int NT>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
 {
     constexpr int kRows = 16 * NT;
@@ -1014,7 +1075,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
     const int len = t.length(b);
     const int q0 = t.first_query(b);
     const int n = t.new_tokens(b, q0);
-    const RowTile rt = row_tile(a, index, kRows, len, n);
+    const RowTile rt = row_tile<kReach>(a, index, kRows, len, n);
     const int row = rt.begin + r;
     if (row >= rt.end) return;
     const int active = (tiles_of(a, rt) + a.split_tiles - 1) / a.split_tiles;
@@ -1088,19 +1149,21 @@ struct AttendPlan {
 // Rows of a workgroup of kv_attention_wide_kernel.
 constexpr int kWideRows = 128;
 
-// One launch each; defined per element type and dim.
-template <class E, int D>
+// One launch each; defined per element type, dim and reach.
+template <class E, int D, int kReach>
 void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
 {
-    if (p.wide) {
-        kv_attention_wide_kernel<E, D><<<p.grid, 256, 0, stream>>>(a);
-        return;
+    if constexpr (kReach == kOwn) {
+        if (p.wide) {
+            kv_attention_wide_kernel<E, D><<<p.grid, 256, 0, stream>>>(a);
+            return;
+        }
     }
     const auto run = [&](auto nt) {
         constexpr int kNt = decltype(nt)::value;
-        kv_attention_kernel<E, D, kNt><<<p.grid, 256, 0, stream>>>(a);
+        kv_attention_kernel<E, D, kReach, kNt><<<p.grid, 256, 0, stream>>>(a);
         if (a.splits > 1 && a.arrived == nullptr)
-            kv_join_kernel<E, D, kNt><<<p.join, 256, 0, stream>>>(a);
+            kv_join_kernel<E, D, kReach, kNt><<<p.join, 256, 0, stream>>>(a);
     };
     if constexpr (D < 256) {
         if (p.nt == 2) return run(std::integral_constant<int, 2>{});
@@ -1108,12 +1171,19 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
     run(std::integral_constant<int, 1>{});
 }
 
-extern template void attend_launch<Bf16, 64>(const AttendArgs&, const AttendPlan&, hipStream_t);
-extern template void attend_launch<Bf16, 128>(const AttendArgs&, const AttendPlan&, hipStream_t);
-extern template void attend_launch<Bf16, 256>(const AttendArgs&, const AttendPlan&, hipStream_t);
-extern template void attend_launch<F16, 64>(const AttendArgs&, const AttendPlan&, hipStream_t);
-extern template void attend_launch<F16, 128>(const AttendArgs&, const AttendPlan&, hipStream_t);
-extern template void attend_launch<F16, 256>(const AttendArgs&, const AttendPlan&, hipStream_t);
+// The instantiations: one file for each dim and reach.
+#define GOFANN_KV_ATTEND(kind, D, reach)                                                       \
+    kind template void attend_launch<Bf16, D, reach>(const AttendArgs&, const AttendPlan&,     \
+                                                     hipStream_t);                             \
+    kind template void attend_launch<F16, D, reach>(const AttendArgs&, const AttendPlan&,      \
+                                                    hipStream_t)
+#define GOFANN_KV_ATTEND_EXTERN(reach)   \
+    GOFANN_KV_ATTEND(extern, 64, reach); \
+    GOFANN_KV_ATTEND(extern, 128, reach); \
+    GOFANN_KV_ATTEND(extern, 256, reach)
+GOFANN_KV_ATTEND_EXTERN(kOwn);
+GOFANN_KV_ATTEND_EXTERN(kDraft);
+GOFANN_KV_ATTEND_EXTERN(kCross);
 
 }  // namespace kv
 }  // namespace gofann

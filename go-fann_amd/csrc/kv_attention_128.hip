@@ -3,7 +3,6 @@
 
 namespace gofann {
 namespace kv {
-template void attend_launch<Bf16, 128>(const AttendArgs&, const AttendPlan&, hipStream_t);
-template void attend_launch<F16, 128>(const AttendArgs&, const AttendPlan&, hipStream_t);
+GOFANN_KV_ATTEND(, 128, kOwn);
 }  // namespace kv
 }  // namespace gofann

@@ -3,7 +3,6 @@
 
 namespace gofann {
 namespace kv {
-template void attend_launch<Bf16, 256>(const AttendArgs&, const AttendPlan&, hipStream_t);
-template void attend_launch<F16, 256>(const AttendArgs&, const AttendPlan&, hipStream_t);
+GOFANN_KV_ATTEND(, 256, kOwn);
 }  // namespace kv
 }  // namespace gofann

@@ -39,10 +39,13 @@ int split_tiles(const Context* ctx, uint64_t items, uint64_t most, bool ragged, 
 
 int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
                  const gofann_kv_rows* q, uint32_t heads, float scale, const int32_t* blocks,
-                 uint32_t width, const gofann_kv_rows* out, float* out_lse)
+                 uint32_t width, const gofann_kv_rows* out, float* out_lse, const KvReach& reach)
 {
     using namespace kv;
     AttendArgs a{};
+    a.sees = reach.sees;
+    a.sees_stride = static_cast<int64_t>(reach.sees_stride);
+    a.sees_width = static_cast<int>(reach.sees_width);
     a.batch = batch_of(cache, batch);
     a.q = rows_of(q);
     a.out = rows_of(out);
@@ -61,12 +64,21 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         blocks != nullptr ? width * (cache->page_size / kTile)
                           : (static_cast<uint32_t>(a.batch.max_positions) + kTile - 1) / kTile;
     const auto launch = [&](const AttendArgs& x, const AttendPlan& p) {
-        const bool bf = cache->elem == GOFANN_ELEM_BF16;
-        switch (dim) {
-            case 64: (bf ? attend_launch<Bf16, 64> : attend_launch<F16, 64>)(x, p, ctx->stream); break;
-            case 128: (bf ? attend_launch<Bf16, 128> : attend_launch<F16, 128>)(x, p, ctx->stream); break;
-            default: (bf ? attend_launch<Bf16, 256> : attend_launch<F16, 256>)(x, p, ctx->stream); break;
-        }
+        const auto of_reach = [&](auto kind) {
+            constexpr int kReach = decltype(kind)::value;
+            const bool bf = cache->elem == GOFANN_ELEM_BF16;
+            switch (dim) {
+                case 64: (bf ? attend_launch<Bf16, 64, kReach> : attend_launch<F16, 64, kReach>)(x, p, ctx->stream); break;
+                case 128: (bf ? attend_launch<Bf16, 128, kReach> : attend_launch<F16, 128, kReach>)(x, p, ctx->stream); break;
+                default: (bf ? attend_launch<Bf16, 256, kReach> : attend_launch<F16, 256, kReach>)(x, p, ctx->stream); break;
+            }
+        };
+        if (reach.cross)
+            of_reach(std::integral_constant<int, kCross>{});
+        else if (reach.sees != nullptr)
+            of_reach(std::integral_constant<int, kDraft>{});
+        else
+            of_reach(std::integral_constant<int, kOwn>{});
     };
     const char* const too_many = "kv_attention: too many tokens a sequence for one call";
     uint64_t rows = blocks != nullptr ? static_cast<uint64_t>(a.group)
@@ -80,7 +92,8 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
     // the decoding ones of a mixed batch, would each keep a workgroup busy with
     // all of their positions; they are left to the other kernel.
     const uint64_t all_rows = static_cast<uint64_t>(batch->queries) * a.group;
-    if (blocks == nullptr && rows > kFewRows &&
+    const bool own = !reach.cross && reach.sees == nullptr;
+    if (own && blocks == nullptr && rows > kFewRows &&
         all_rows / kWideRows * cache->kv_heads >= static_cast<uint64_t>(ctx->compute_units)) {
         AttendPlan p{};
         p.wide = true;

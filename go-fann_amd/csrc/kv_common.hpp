@@ -199,5 +199,66 @@ inline Batch batch_of(const gofann_kv_cache* c, const gofann_kv_batch* b)
                  static_cast<int>(most)};
 }
 
+// A batch whose rows alone are of interest, no cache's positions.
+inline Batch rows_only(const gofann_kv_batch* b)
+{
+    Batch t{};
+    t.lengths = b->lengths;
+    t.query_offsets = b->query_offsets;
+    t.queries = static_cast<int>(b->queries);
+    return t;
+}
+
+// Eight channels of codes under their group's exponent as elements.
+template <class E>
+__device__ __forceinline__ u32x4 held(uint32_t codes, uint32_t exponent)
+{
+    const uint32_t s = exponent << 23;
+    return u32x4{E::template decode<0>(codes, s), E::template decode<1>(codes, s),
+                 E::template decode<2>(codes, s), E::template decode<3>(codes, s)};
+}
+
+// The most and least of every channel over a page's keys, eight channels
+// (8 lane ..) of the rows row, row + 256 / (D / 8), .. a thread, joined through
+// LDS and written as the page's box by the 256 threads of a workgroup.
+template <int D>
+__device__ __forceinline__ void join_box(const float (&hi)[8], const float (&lo)[8],
+                                         float (&most)[256 * 8 / D][D], float (&least)[256 * 8 / D][D],
+                                         float (&amax_part)[4], int8_t* box, uint8_t* box_scale)
+{
+    constexpr int kLanes = D / 8;
+    constexpr int kTokens = 256 / kLanes;
+    const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        most[row][8 * lane + i] = hi[i];
+        least[row][8 * lane + i] = lo[i];
+    }
+    __syncthreads();
+    const int c = threadIdx.x % D;
+    float mh = -__builtin_inff(), ml = __builtin_inff();
+    for (int r = 0; r < kTokens; ++r) {
+        mh = fmaxf(mh, most[r][c]);
+        ml = fminf(ml, least[r][c]);
+    }
+    float amax = fmaxf(__builtin_fabsf(mh), __builtin_fabsf(ml));
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
+    if (threadIdx.x % 64 == 0) amax_part[threadIdx.x / 64] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(amax_part[0], amax_part[1]), fmaxf(amax_part[2], amax_part[3]));
+    // Exact: the values are codes times powers of two, so amax = m 2^t has
+    // m 2^7 <= 127, and so is the division by a power of two.
+    int e = __builtin_amdgcn_frexp_expf(amax) - 7;
+    e = e < -125 ? -125 : e > 125 ? 125 : e;
+    if (!(amax > 0.0f)) e = -125;
+    const float inv = __builtin_bit_cast(float, static_cast<uint32_t>(127 - e) << 23);
+    if (static_cast<int>(threadIdx.x) < D) {
+        box[c] = static_cast<int8_t>(__builtin_ceilf(mh * inv));
+        box[D + c] = static_cast<int8_t>(__builtin_floorf(ml * inv));
+    }
+    if (threadIdx.x == 0) *box_scale = static_cast<uint8_t>(e + 127);
+}
+
 }  // namespace kv
 }  // namespace gofann

@@ -1,0 +1,8 @@
+// Cross attention over the 4-bit key/value cache for heads of 128 channels.
+#include "kv_attention.hpp"
+
+namespace gofann {
+namespace kv {
+GOFANN_KV_ATTEND(, 128, kCross);
+}  // namespace kv
+}  // namespace gofann

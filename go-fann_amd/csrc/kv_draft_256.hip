@@ -1,0 +1,8 @@
+// Attention of drafted tokens over the 4-bit key/value cache for heads of 256 channels.
+#include "kv_attention.hpp"
+
+namespace gofann {
+namespace kv {
+GOFANN_KV_ATTEND(, 256, kDraft);
+}  // namespace kv
+}  // namespace gofann

@@ -307,6 +307,16 @@ SIGNATURES = {
     "gofann_kv_attention": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView),
                                       C.POINTER(KvRows), U32, C.c_float, P, U32,
                                       C.POINTER(KvRows), P]),
+    "gofann_kv_draft_attention": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView),
+                                            C.POINTER(KvRows), U32, C.c_float, P, U32, U32, P, U32,
+                                            C.POINTER(KvRows), P]),
+    "gofann_kv_cross_attention": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView),
+                                            C.POINTER(KvRows), U32, C.c_float, C.POINTER(KvRows), P]),
+    "gofann_kv_read": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView),
+                                 C.POINTER(KvRows), C.POINTER(KvRows)]),
+    "gofann_kv_draft_tree": (C.c_int, [P, C.POINTER(KvBatchView), P, U32, P, P]),
+    "gofann_kv_draft_accept": (C.c_int, [P, C.POINTER(KvBatchView), P, P, P, U32, P, P, P]),
+    "gofann_kv_keep": (C.c_int, [P, C.POINTER(KvCacheView), C.POINTER(KvBatchView), P, U32]),
 }
 
 _lib = None

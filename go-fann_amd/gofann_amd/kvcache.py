@@ -15,6 +15,19 @@ those reads nothing else.  The reference has no counterpart.
     out = cache.attend(batch, q)                                 # all positions
     out = cache.attend(batch, q, blocks=cache.select(batch, q, 64))
 
+Tokens that were drafted, as a tree, are settled in the cache by what the
+model answers to them:
+
+    sees, depths = draft_tree(ctx, batch, parents)               # once a step
+    cache.append(batch, k, v)                                    # in each layer
+    out = cache.attend(batch, q, sees=sees)
+    path, lengths, answer = draft_accept(ctx, batch, parents, drafted, chosen, 8)
+    cache.keep(batch, path)                                      # in each layer
+    batch_lengths.copy_(lengths)                                 # and not before
+
+`cross` attends to a sequence that the tokens are no part of, and `read` gives
+back what the cache holds.
+
 Calls are asynchronous on the context's stream, which has to be torch's
 current one, on the context's device.  Everything may be captured in a graph
 once a call of the same sizes has run.  The graph then uses the context's
@@ -49,6 +62,20 @@ def _counts(**kw: int) -> None:
     for name, n in kw.items():
         if not 0 <= n < 1 << 32:
             raise ValueError(f"{name} must be in [0, 2^32)")
+
+
+def _current(ctx: _lib.Context) -> None:
+    if _current_device() != ctx.device:
+        raise _lib.GofannError("torch's current device is not the context's")
+    if _raw_stream(ctx.device) != ctx.stream:
+        raise _lib.GofannError("the context is bound to another stream than torch's current "
+                               "one: call ctx.bind_stream")
+
+
+def _ints(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> torch.Tensor:
+    if t.shape != shape or t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)} on {device}")
+    return t
 
 
 class KvBatch:
@@ -197,11 +224,7 @@ class KvCache:
             raise ValueError("the batch is on another device")
         if self._index != self.ctx.device:
             raise ValueError("the cache is not on the context's device")
-        if _current_device() != self._index:
-            raise _lib.GofannError("torch's current device is not the context's")
-        if _raw_stream(self._index) != self.ctx.stream:
-            raise _lib.GofannError("the context is bound to another stream than torch's current "
-                                   "one: call ctx.bind_stream")
+        _current(self.ctx)
 
     # -- calls -----------------------------------------------------------
     def append(self, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, *,
@@ -238,13 +261,58 @@ class KvCache:
         return out
 
     def attend(self, batch: KvBatch, q: torch.Tensor, *, scale: float | None = None,
-               blocks: torch.Tensor | None = None, out: torch.Tensor | None = None,
-               lse: torch.Tensor | None = None) -> torch.Tensor:
+               blocks: torch.Tensor | None = None, sees: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
         """softmax(scale q.k) v of queries [queries][heads][dim] over the
         positions up to each token's own that the filter leaves, or of these
-        only the ones in `blocks` (as `select` gives them).  scale: dim ** -0.5
-        by default.  lse [queries][heads] f32 gets the log of the sums of
-        exponentials.  A row with nothing to read is zero (lse -inf)."""
+        only the ones in `blocks` (as `select` gives them).  With `sees`
+        [queries][words] i32 a token looks at all positions before its
+        sequence's tokens and at those of them that its bits name, itself no
+        exception: bit j % 32 of word j / 32 for the j-th (`draft_tree` gives
+        those of a tree).  scale: dim ** -0.5 by default.  lse [queries][heads]
+        f32 gets the log of the sums of exponentials.  A row with nothing to
+        read is zero (lse -inf)."""
+        rq, ro, out, heads, scale = self._attention(batch, q, scale, out, lse)
+        width = 0
+        if blocks is not None:
+            if blocks.dim() != 3 or blocks.shape[:2] != (batch.queries, self.kv_heads) or \
+                    blocks.dtype != torch.int32 or blocks.device != self.device or \
+                    not blocks.is_contiguous():
+                raise ValueError("blocks must be contiguous int32 [queries][kv_heads][width]")
+            width = blocks.shape[2]
+        if sees is None:
+            self.ctx.check(self.lib.gofann_kv_attention(
+                self.ctx.handle, self.view, batch.view, rq, heads, scale, _lib.ptr(blocks), width, ro,
+                _lib.ptr(lse)))
+            return out
+        if sees.dim() != 2 or sees.shape[0] != batch.queries or sees.dtype != torch.int32 or \
+                sees.device != self.device:
+            raise ValueError("sees must be int32 [queries][words] on the cache's device")
+        words = sees.shape[1]
+        if sees.numel() and (sees.stride(1) != 1 or (sees.shape[0] > 1 and sees.stride(0) < words)):
+            raise ValueError("sees must be contiguous along its last axis, its rows apart")
+        stride = sees.stride(0) if sees.shape[0] > 1 else words
+        # Without words there is no address, and none is read.
+        at = sees.data_ptr() if words else out.data_ptr() & ~3
+        self.ctx.check(self.lib.gofann_kv_draft_attention(
+            self.ctx.handle, self.view, batch.view, rq, heads, scale, at, words, max(stride, words),
+            _lib.ptr(blocks), width, ro, _lib.ptr(lse)))
+        return out
+
+    def cross(self, batch: KvBatch, q: torch.Tensor, *, scale: float | None = None,
+              out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+        """Cross attention: as `attend`, of tokens that are no part of their
+        sequence, over all of its positions that the filter leaves.  `lengths`
+        of the batch are those of the sequences (an encoder's states), whatever
+        the number of tokens."""
+        rq, ro, out, heads, scale = self._attention(batch, q, scale, out, lse)
+        self.ctx.check(self.lib.gofann_kv_cross_attention(
+            self.ctx.handle, self.view, batch.view, rq, heads, scale, ro, _lib.ptr(lse)))
+        return out
+
+    def _attention(self, batch: KvBatch, q: torch.Tensor, scale: float | None,
+                   out: torch.Tensor | None, lse: torch.Tensor | None):
+        """The checks that attention calls share: rows of q and out, out, heads and scale."""
         self._ready(batch)
         heads = q.shape[1] if q.dim() == 3 else None
         rq = self._rows("q", q, batch.queries, heads)
@@ -253,17 +321,79 @@ class KvCache:
             ro = _lib.KvRows(out.data_ptr(), heads * self.dim, self.dim)
         else:
             ro = self._rows("out", out, batch.queries, heads, True)
-        width = 0
-        if blocks is not None:
-            if blocks.dim() != 3 or blocks.shape[:2] != (batch.queries, self.kv_heads) or \
-                    blocks.dtype != torch.int32 or blocks.device != self.device or \
-                    not blocks.is_contiguous():
-                raise ValueError("blocks must be contiguous int32 [queries][kv_heads][width]")
-            width = blocks.shape[2]
         if lse is not None and (lse.shape != (batch.queries, heads) or lse.dtype != torch.float32
                                 or lse.device != self.device or not lse.is_contiguous()):
             raise ValueError("lse must be contiguous float32 [queries][heads]")
-        self.ctx.check(self.lib.gofann_kv_attention(
-            self.ctx.handle, self.view, batch.view, rq, heads,
-            self.dim ** -0.5 if scale is None else scale, _lib.ptr(blocks), width, ro, _lib.ptr(lse)))
-        return out
+        return rq, ro, out, heads, self.dim ** -0.5 if scale is None else scale
+
+    def read(self, batch: KvBatch, *, k: torch.Tensor | None = None,
+             v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The keys and values [queries][kv_heads][dim] that the cache holds of
+        the batch's tokens, exactly; with k or v given, only what is given, into
+        it.  Rows of tokens without a page are zero."""
+        self._ready(batch)
+        n, h = batch.queries, self.kv_heads
+        if k is None and v is None:
+            k, v = torch.empty((2, n, h, self.dim), dtype=self.dtype, device=self.device)
+        rk = None if k is None else self._rows("k", k, n, h, True)
+        rv = None if v is None else self._rows("v", v, n, h, True)
+        self.ctx.check(self.lib.gofann_kv_read(self.ctx.handle, self.view, batch.view, rk, rv))
+        return k, v
+
+    def keep(self, batch: KvBatch, path: torch.Tensor) -> None:
+        """Moves the tokens of each sequence's path [sequences][width] i32 (as
+        `draft_accept` gives it) to the positions of the sequence's first
+        tokens, and renews the boxes up to the last one kept.  The batch's
+        lengths are still those with all tokens; afterwards they have to be set
+        to what `draft_accept` gave."""
+        self._ready(batch)
+        if path.dim() != 2:
+            raise ValueError("path must be contiguous int32 [sequences][width]")
+        _ints("path", path, (batch.sequences, path.shape[1]), self.device)
+        self.ctx.check(self.lib.gofann_kv_keep(self.ctx.handle, self.view, batch.view,
+                                               path.data_ptr(), path.shape[1]))
+
+
+def _draft(ctx: _lib.Context, batch: KvBatch, **rows: torch.Tensor) -> None:
+    if batch.device.type != "cuda" or batch.device.index != ctx.device:
+        raise ValueError("the batch is not on the context's device")
+    for name, t in rows.items():
+        _ints(name, t, (batch.queries,), batch.device)
+    _current(ctx)
+
+
+def draft_tree(ctx: _lib.Context, batch: KvBatch,
+               parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(sees [queries][words] i32, depths [queries] i32) of the trees that the
+    sequences' tokens form: for `attend`, every token's ancestors and itself in
+    bits, and how many ancestors it has (it stands for that many positions past
+    its sequence's first token).  parents [queries] i32: the token before each,
+    by its index in its sequence's tokens and below its own; anything else makes
+    a root.  At most 8192 tokens a sequence."""
+    _draft(ctx, batch, parents=parents)
+    words = (batch.max_queries + 31) // 32
+    sees = torch.empty((batch.queries, words), dtype=torch.int32, device=batch.device)
+    depths = torch.empty_like(parents)
+    ctx.check(ctx.lib.gofann_kv_draft_tree(ctx.handle, batch.view, parents.data_ptr(), words,
+                                           sees.data_ptr(), depths.data_ptr()))
+    return sees, depths
+
+
+def draft_accept(ctx: _lib.Context, batch: KvBatch, parents: torch.Tensor, drafted: torch.Tensor,
+                 chosen: torch.Tensor,
+                 width: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(path [sequences][width], lengths [sequences], next [sequences]), all i32:
+    the tokens of each sequence's tree (`parents`, as for `draft_tree`) that the
+    model's answers accept.  Token 0 is; then of the last one's children the
+    first whose `drafted` [queries] is the answer `chosen` [queries] to the last
+    one, and so on, up to `width` tokens.  path: their indexes, -1 past the last;
+    lengths: the sequences' with only these; next: the answer to the last."""
+    _draft(ctx, batch, parents=parents, drafted=drafted, chosen=chosen)
+    _counts(width=width)
+    n = batch.sequences
+    path = torch.empty((n, width), dtype=torch.int32, device=batch.device)
+    lengths, answer = torch.empty((2, n), dtype=torch.int32, device=batch.device)
+    ctx.check(ctx.lib.gofann_kv_draft_accept(
+        ctx.handle, batch.view, parents.data_ptr(), drafted.data_ptr(), chosen.data_ptr(), width,
+        path.data_ptr(), lengths.data_ptr(), answer.data_ptr()))
+    return path, lengths, answer

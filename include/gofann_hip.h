@@ -1052,6 +1052,66 @@ int gofann_kv_attention(gofann_ctx* ctx, const gofann_kv_cache* cache,
                         float scale, const int32_t* blocks, uint32_t width,
                         const gofann_kv_rows* out, float* out_lse);
 
+/* The same of tokens that are a draft: the sequence's positions before the
+ * call's tokens are all looked at, and of those tokens the ones that a row of
+ * `sees` [queries][sees_stride] (sees_width words used) names: bit j % 32 of
+ * word j / 32 for the sequence's j-th token, itself no exception; those past
+ * the words are not.  Filter and block lists apply as above.  A token that no
+ * row sees need not have been written. */
+int gofann_kv_draft_attention(gofann_ctx* ctx, const gofann_kv_cache* cache,
+                              const gofann_kv_batch* batch, const gofann_kv_rows* q, uint32_t heads,
+                              float scale, const uint32_t* sees, uint32_t sees_width,
+                              uint32_t sees_stride, const int32_t* blocks, uint32_t width,
+                              const gofann_kv_rows* out, float* out_lse);
+
+/* The same of tokens that are no part of their sequence: each attends to all
+ * of its lengths[b] positions that the filter leaves (an encoder's states, of
+ * whatever length).  lengths[b] may be 0 and below the sequence's tokens. */
+int gofann_kv_cross_attention(gofann_ctx* ctx, const gofann_kv_cache* cache,
+                              const gofann_kv_batch* batch, const gofann_kv_rows* q, uint32_t heads,
+                              float scale, const gofann_kv_rows* out, float* out_lse);
+
+/* The values that the cache holds of the batch's tokens (the last positions
+ * of their sequences), as rows [queries][kv_heads][dim]; k or v may be NULL.
+ * Rows of tokens without a page become zero; those that no sequence has are
+ * left as they are. */
+int gofann_kv_read(gofann_ctx* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                   const gofann_kv_rows* k, const gofann_kv_rows* v);
+
+/* ---- drafts --------------------------------------------------------------
+ * A sequence's tokens of a call as a tree: parents [queries], the index in
+ * its sequence's tokens of the token before it, below its own; anything else
+ * makes it a root.  Token 0 is the one that the model chose last.
+ *
+ * out_sees (optional) [queries][words]: every token's ancestors and itself, as
+ * gofann_kv_draft_attention takes them; bits past the words are dropped.
+ * out_depths (optional) [queries]: how many ancestors it has, so that it stands
+ * for the position lengths[b] - tokens + depth of its text.  At most 8192
+ * tokens a sequence. */
+int gofann_kv_draft_tree(gofann_ctx* ctx, const gofann_kv_batch* batch, const int32_t* parents,
+                         uint32_t words, uint32_t* out_sees, int32_t* out_depths);
+
+/* The path of each sequence's draft that the model's answers accept: token 0,
+ * then of the last one's children, the lowest whose drafted [queries] is what
+ * the model answered to the last one (chosen [queries]), and so on, up to
+ * `width` tokens.  out_path [sequences][width]: their indexes, ascending, -1
+ * past the last.  out_lengths (optional) [sequences]: the sequence's length
+ * with only these of the draft.  out_next (optional) [sequences]: the answer to
+ * the last of them, -1 where a sequence has no tokens. */
+int gofann_kv_draft_accept(gofann_ctx* ctx, const gofann_kv_batch* batch, const int32_t* parents,
+                           const int32_t* drafted, const int32_t* chosen, uint32_t width,
+                           int32_t* out_path, int32_t* out_lengths, int32_t* out_next);
+
+/* Moves the keys and values of each sequence's path [sequences][width] (as
+ * gofann_kv_draft_accept gives it; it ends where it no longer ascends within
+ * the sequence's tokens) to the draft's first positions, as if all were read
+ * before any is written, and renews the boxes of the pages from the draft's
+ * first position to the last one kept.  Codes are moved as they are.  Rows
+ * that have no page, or would get none, are not moved.  lengths are still
+ * those with the whole draft. */
+int gofann_kv_keep(gofann_ctx* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                   const int32_t* path, uint32_t width);
+
 #ifdef __cplusplus
 }
 #endif
