@@ -18,6 +18,11 @@ struct AttendArgs {
     float* lse;             // [queries][heads] or NULL
     float* part_o;          // [kv_heads][split][part_count][dim], splits > 1: see part_of()
     float* part_ml;         // [kv_heads][split][part_count][2]: reference, sum
+    int32_t* pieces;        // [row tile][kv_heads][2] of shared tiles: first slot, shares after it
+    const uint32_t* live;   // [sequence][live_stride][4]: tiles that the filter leaves, see
+    const int32_t* live_count;  // kv_live_kernel; NULL: all of them are looked at
+    int64_t live_stride;
+    int join_shift;         // log2 of the groups of lanes that join a row's pieces
     uint32_t* arrived;      // [item], zero between calls: splits done; NULL: kv_join_kernel joins
     float scale_log2;       // scale * log2(e)
     int group;              // heads a key/value head
@@ -701,6 +706,28 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
     }
 }
 
+// Rows of a workgroup of kv_attention_wide_kernel.
+constexpr int kWideRows = 128;
+constexpr int kXcds = 8;
+
+// LDS of a workgroup of long chunks: a turn's tiles as elements, twice.  R waves
+// have rows of their own; with two, two waves share each row's positions.
+template <int D, int kReach>
+struct WideLds {
+    static constexpr int kPer = D == 256 && kReach == kOwn ? 1 : 2;  // tiles a turn
+    static constexpr int kResident = D == 256 && kReach != kOwn ? 1 : 2;
+    u32x4 keys[2][kPer][D / 16][64];
+    u32x4 values[2][kPer][D / 32][2][64];
+};
+
+// What such a workgroup works on: tiles [begin, end) of a row tile.
+struct WidePiece {
+    int b, h, len, q0, n;
+    int begin, end;
+    int slot;  // of its partial result; negative: it has all of the row tile
+    RowTile rows;
+};
+
 // Long chunks: four waves of 32 rows each read the same positions.
 //
 // A tile of 32 positions is D / 16 products S^T += K Q^T and D / 16 products
@@ -728,30 +755,24 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
 // within 3% of each other.  Without LDS, each wave converting for itself (16 x
 // 16 products): 0.69 ms where this took 0.63.  At 256 channels (1.44 ms) the
 // output and the queries leave 29 registers too few, spilled.
-template <class E, int D>
-__global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
+template <class E, int D, int kReach>
+__device__ __forceinline__ void wide_rows(const AttendArgs& a, WideLds<D, kReach>& lds, const WidePiece& piece)
 {
     using V8 = typename E::V8;
     constexpr int kRows = 32;
     constexpr int kKeys = D / 16;     // fragments of a tile's keys
     constexpr int kMine = kKeys / 4;  // of them a wave's
     constexpr int kTiles = D / 32;    // tiles of O
-    constexpr int kPer = D == 256 ? 1 : 2;  // tiles a turn
-    __shared__ u32x4 keys[2][kPer][kKeys][64];
-    __shared__ u32x4 values[2][kPer][kTiles][2][64];
+    constexpr int kPer = WideLds<D, kReach>::kPer;
+    auto& keys = lds.keys;
+    auto& values = lds.values;
     const Batch& t = a.batch;
     const int lane = threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int r32 = lane % 32, g2 = lane / 32;
-    const int h = blockIdx.x;
-    const int index = gridDim.y - 1 - blockIdx.y;  // the longest rows first
-    const int b = blockIdx.z;
-    const int len = t.length(b);
-    const int q0 = t.first_query(b);
-    const int n = t.new_tokens(b, q0);
-    const RowTile all = row_tile<kOwn>(a, index, 4 * kRows, len, n);
-    if (all.end <= all.begin) return;
-    const int tiles = tiles_of(a, all);
+    const int h = piece.h, b = piece.b, len = piece.len, q0 = piece.q0, n = piece.n;
+    const RowTile& all = piece.rows;
+    const int tile_begin = piece.begin, tile_end = piece.end;
     const int hi_pos = all.last_pos + 1;
     const int first_see = all.first_pos + 1;  // positions that every row of the workgroup sees
     // This wave's rows; at a chunk's end maybe none, and it only converts.
@@ -765,7 +786,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
     const bool in = row < end;
     const int token = (in ? row : all.begin) / a.group;
     const int head = h * a.group + (in ? row : all.begin) % a.group;
-    const int limit = in ? len - n + token + 1 : 0;
+    // Positions that the row sees, or, of a draft's token, the row of its bits.
+    const int limit = kReach == kDraft ? (in ? q0 + token : -1) : !in ? 0 : kReach == kCross ? len : len - n + token + 1;
     {
         const uint16_t* const p = a.q.p + (q0 + token) * a.q.token_stride + head * a.q.head_stride;
 #pragma unroll
@@ -845,8 +867,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
         if constexpr (decltype(kind)::value) {
             const uint32_t mine = word >> (16 * half + 8 * g2);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 8; ++e) {
                 if (!(mine >> e & 1u)) scale[e] = 127u << 23;
+                if constexpr (kReach == kDraft) scale[e] = written_scale<E>(scale[e]);
+            }
         }
         // Bytes of a lane's that this wave converts: D = 128: byte w % 2 of two,
         // D = 256: bytes 2 (w % 2) and that plus 1 of four.
@@ -884,6 +908,13 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
     constexpr int kAhead = D == 128 ? 8 : 4;
     const auto multiply = [&](auto kind, int buf, const int (&from)[kPer], const uint32_t (&mine)[kPer]) {
         f32x16 s[kPer];
+        [[maybe_unused]] Sees sees[kPer];
+        if constexpr (decltype(kind)::value && kReach == kDraft) {
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) {
+                sees[x] = load_sees(a, limit, from[x] - (len - n));
+            }
+        }
 #pragma unroll
         for (int x = 0; x < kPer; ++x) {
 #pragma unroll
@@ -898,7 +929,14 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
                 for (int j = 0; j < kAhead; ++j)
                     s[x] = E::mfma(__builtin_bit_cast(V8, f[j]), q[lead + j], s[x]);
             }
-            if constexpr (decltype(kind)::value) {
+            if constexpr (decltype(kind)::value && kReach == kDraft) {
+                const uint32_t ok = (mine[x] & sees_bits(sees[x], limit, from[x] - (len - n))) >> (8 * g2);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        s[x][8 * u + e] = (ok >> (16 * u + e) & 1u) ? s[x][8 * u + e] : -__builtin_inff();
+            } else if constexpr (decltype(kind)::value) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     int left = limit - from[x] - 16 * u - 8 * g2;
@@ -919,12 +957,12 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
         top *= a.scale_log2;
         if (far || __any(top - st.m > kSlack + E::kRaise)) {
             top = fmaxf(top, __shfl_xor(top, 32));
-            bool mine;
-            const float f = renew<E>(st, top, mine);
+            bool is_far;
+            const float f = renew<E>(st, top, is_far);
 #pragma unroll
             for (int c = 0; c < kTiles; ++c) o[c] *= f;
-            far = __any(mine);
-            if (mine) {
+            far = __any(is_far);
+            if (is_far) {
 #pragma unroll
                 for (int x = 0; x < kPer; ++x)
 #pragma unroll
@@ -960,19 +998,30 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
     };
 
     const int page_tiles_shift = t.page_shift - 5;
-    for (int base = 0; base < tiles; base += 64) {
-        const int tile = base + lane;
+    for (int base = tile_begin; base < tile_end; base += 64) {
+        int tile = base + lane;
         uint32_t at = 0, word = 0;
-        const int t0 = tile * kTile;
-        if (tile < tiles) {
-            const int page = t.page(b, tile >> page_tiles_shift);
-            if (page >= 0) {
-                word = t.word(b, tile);
-                if (hi_pos - t0 < 32) word &= (1u << (hi_pos - t0)) - 1u;
-                at = ((static_cast<uint32_t>(page) * t.kv_heads + h) << page_tiles_shift) +
-                     (tile & ((1 << page_tiles_shift) - 1));
+        int page = -1;
+        if (tile < tile_end) {
+            if (kReach != kOwn && a.live != nullptr) {
+                const u32x4 entry = reinterpret_cast<const u32x4*>(a.live)[b * a.live_stride + tile];
+                tile = entry[0];
+                word = entry[1];
+                page = entry[2];
+            } else {
+                page = t.page(b, tile >> page_tiles_shift);
+                if (page >= 0) {
+                    word = t.word(b, tile);
+                    if (hi_pos - tile * kTile < 32) word &= (1u << (hi_pos - tile * kTile)) - 1u;
+                }
             }
         }
+        if (page >= 0)
+            at = ((static_cast<uint32_t>(page) * t.kv_heads + h) << page_tiles_shift) +
+                 (tile & ((1 << page_tiles_shift) - 1));
+        else
+            word = 0;
+        const int t0 = tile * kTile;
         // The same in every wave: tiles that every row sees whole, kPer a turn,
         // then the others.
         uint64_t whole = __ballot(word == 0xFFFFFFFFu && t0 + kTile <= first_see);
@@ -1020,7 +1069,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
                     more = live != 0;
                     if (more) take(next, ahead, i[kPer - 1]);
                 }
-                multiply(kind, buf, from, now);
+                // Waves without rows, past a chunk's end, only convert.
+                if (kReach == kOwn || begin < end) multiply(kind, buf, from, now);
                 __syncthreads();
                 if (!turn) break;
                 buf ^= 1;
@@ -1032,6 +1082,22 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
 
     st.sum += __shfl_xor(st.sum, 32);
     if (!in) return;
+    if constexpr (kReach != kOwn) {
+        if (piece.slot >= 0) {  // joined with the others by kv_join_pieces_kernel
+            const int64_t to = static_cast<int64_t>(piece.slot) * kWideRows + wave * kRows + r32;
+            if (g2 == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * to) = float2{st.m, st.sum};
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int z = 0; z < kTiles; ++z) {
+                    f32x4 v;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) v[y] = o[(4 * z + y) % kTiles][4 * x + (4 * z + y) / kTiles];
+                    *reinterpret_cast<f32x4*>(a.part_o + to * D + kTiles * (8 * x + 4 * g2) + 4 * z) = v;
+                }
+            return;
+        }
+    }
     uint16_t* const p = a.out.p + (q0 + token) * a.out.token_stride + head * a.out.head_stride;
     const float inv = st.sum != 0.0f ? 1.0f / st.sum : 0.0f;
     // Rows 8 x + 4 g + y of O^T, y < 4, hold channels dim/32 (8 x + 4 g) ..
@@ -1054,6 +1120,331 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
     if (a.lse != nullptr && g2 == 0)
         a.lse[static_cast<int64_t>(q0 + token) * t.kv_heads * a.group + head] =
             (st.m + __builtin_log2f(st.sum)) * 0.69314718055994531f;
+}
+
+template <class E, int D>
+__global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
+{
+    __shared__ WideLds<D, kOwn> lds;
+    const Batch& t = a.batch;
+    WidePiece p;
+    p.h = blockIdx.x;
+    p.b = blockIdx.z;
+    p.len = t.length(p.b);
+    p.q0 = t.first_query(p.b);
+    p.n = t.new_tokens(p.b, p.q0);
+    const int index = gridDim.y - 1 - blockIdx.y;  // the longest rows first
+    p.rows = row_tile<kOwn>(a, index, kWideRows, p.len, p.n);
+    if (p.rows.end <= p.rows.begin) return;
+    p.begin = 0;
+    p.end = tiles_of(a, p.rows);
+    p.slot = -1;
+    wide_rows<E, D, kOwn>(a, lds, p);
+}
+
+// Tiles of a sequence of len positions that may have a page.
+__device__ __forceinline__ int paged_tiles(const Batch& t, int len)
+{
+    const int last = len < t.max_positions ? len : t.max_positions;
+    return (last + kTile - 1) / kTile;
+}
+
+// Tiles of a sequence that are looked at.
+__device__ __forceinline__ int shared_tiles(const AttendArgs& a, int b, int len)
+{
+    return a.live != nullptr ? a.live_count[b] : paged_tiles(a.batch, len);
+}
+
+// What it takes to begin a row tile (its queries, the first tiles' way from
+// memory, the part result), in tiles: they are counted into a workgroup's share.
+// Beginning took 5 to 6 us, a tile of 128 channels 0.6 to 1.1; uncounted, a share
+// of ten short sequences took 82 us where the others took 48.
+constexpr int kStartTiles = 6;
+
+// The tiles of a sequence that its filter leaves something of, in order: tile,
+// filter word and page, a place of four words each.  A workgroup lists 1,024
+// tiles and counts for itself what lies before them.
+constexpr int kLiveChunk = 1024;
+static __global__ __launch_bounds__(256) void kv_live_kernel(AttendArgs a, u32x4* live, int32_t* count)
+{
+    __shared__ int part[4];
+    const Batch& t = a.batch;
+    const int b = blockIdx.y;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int len = t.length(b);
+    const int tiles = paged_tiles(t, len);
+    const int begin = blockIdx.x * kLiveChunk;
+    if (begin > 0 && begin >= tiles) return;
+    const auto word_of = [&](int tile) -> uint32_t {
+        if (tile >= tiles) return 0u;
+        const int left = (len < t.max_positions ? len : t.max_positions) - tile * kTile;
+        return t.word(b, tile) & (left < kTile ? (1u << left) - 1u : 0xFFFFFFFFu);
+    };
+    int before = 0;
+#pragma unroll 8
+    for (int tile = threadIdx.x; tile < begin; tile += 256) before += word_of(tile) != 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) before += __shfl_xor(before, d);
+    if (lane == 0) part[wave] = before;
+    __syncthreads();
+    before = part[0] + part[1] + part[2] + part[3];
+    __syncthreads();
+    // Four tiles a thread, next to each other.
+    uint32_t word[4];
+    int own = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        word[i] = word_of(begin + 4 * threadIdx.x + i);
+        own += word[i] != 0;
+    }
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(upto, d);
+        if (lane >= d) upto += x;
+    }
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    int at = before + upto - own;
+    for (int w = 0; w < wave; ++w) at += part[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (word[i] == 0) continue;
+        const int tile = begin + 4 * threadIdx.x + i;
+        const int page = t.page(b, tile >> (t.page_shift - 5));
+        live[static_cast<int64_t>(b) * a.live_stride + at++] =
+            u32x4{static_cast<uint32_t>(tile), word[i], static_cast<uint32_t>(page), 0};
+    }
+    if (begin + kLiveChunk >= tiles && threadIdx.x == 255) count[b] = at;
+}
+
+// Row tiles of a sequence of n tokens, at most as many as there is room for.
+__device__ __forceinline__ int shared_row_tiles(const AttendArgs& a, int rows, int n)
+{
+    const int64_t tiles = (static_cast<int64_t>(n) * a.group + rows - 1) / rows;
+    return tiles < a.row_tiles ? static_cast<int>(tiles) : a.row_tiles;
+}
+
+// The same for drafts and cross attention, whose rows all reach the same
+// positions, shared out evenly: the tiles of all sequences, key/value heads and
+// row tiles stand in one line, and each workgroup takes as long a piece of it,
+// whatever the sequences' lengths, which only the device knows.  A workgroup's
+// piece may end one row tile, hold others whole and begin another: those that it
+// holds in part (at most two) go to slots of their own, which
+// kv_join_pieces_kernel joins.  Row tiles of one sequence and head stand next to
+// each other and a piece goes to the XCD that has its neighbours, so that they
+// find their positions in its L2.
+template <class E, int D, int kReach>
+__global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_attention_shared_kernel(AttendArgs a)
+{
+    __shared__ WideLds<D, kReach> lds;
+    constexpr int kRows = kWideRows;
+    const Batch& t = a.batch;
+    const int lane = threadIdx.x % 64;
+    WidePiece p;
+    p.b = 0;
+    int s = 0, share = 1, from = 0, to = 1, index, padded = 0;
+    if (a.split_tiles == 0) {  // so many row tiles that each is a workgroup's
+        p.b = blockIdx.z;
+        if (a.sequences <= 64) {
+            // The longest sequences first, so that the last ones to run are short.
+            const int mine = lane < a.sequences ? shared_tiles(a, lane, t.length(lane)) : -1;
+            int before = 0;
+            for (int b = 0; b < a.sequences; ++b) {
+                const int other = __builtin_amdgcn_readlane(mine, b);
+                before += other > mine || (other == mine && b < lane);
+            }
+            p.b = __builtin_ctzll(__ballot(before == p.b && lane < a.sequences));
+        }
+        p.h = blockIdx.x;
+        index = blockIdx.y;
+        p.begin = 0;
+    } else {
+        // Tiles of 64 sequences from b on, a sequence a lane: those of the lanes up
+        // to this one, and this one's.
+        const auto tiles_from = [&](int b, int& own) {
+            own = 0;
+            if (b + lane < a.sequences) {
+                const int len = t.length(b + lane), q0 = t.first_query(b + lane);
+                own = shared_row_tiles(a, kRows, t.new_tokens(b + lane, q0)) *
+                      (shared_tiles(a, b + lane, len) + kStartTiles) * t.kv_heads;
+            }
+            int upto = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int x = __shfl_up(upto, d);
+                if (lane >= d) upto += x;
+            }
+            return upto;
+        };
+        int total = 0, own, upto;
+        for (int b = 0; b < a.sequences; b += 64) {
+            upto = tiles_from(b, own);
+            total += __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (total == 0) return;
+        const int workgroups = gridDim.x;
+        share = (total + workgroups - 1) / workgroups;
+        if (share < a.split_tiles) share = a.split_tiles;
+        share += share % 2;
+        if (a.sequences == 1) {
+            // All row tiles have as many tiles: parts that end with them.
+            const int all = shared_tiles(a, 0, t.length(0));
+            const int items = total / (all + kStartTiles), room = workgroups / items;
+            if (room > 0 && all > 0) {
+                int parts = (all + share - 1) / share;
+                parts = parts < room ? parts : room;
+                share = (all + parts - 1) / parts;
+                share += share % 2;
+                parts = (all + share - 1) / share;
+                padded = parts * share;
+                total = items * padded;
+            }
+        }
+        const int shares = (total + share - 1) / share;
+        const int each = (shares + kXcds - 1) / kXcds;
+        s = blockIdx.x % kXcds * each + blockIdx.x / kXcds;
+        if (static_cast<int>(blockIdx.x / kXcds) >= each || s >= shares) return;
+        from = s * share;
+        to = from + share < total ? from + share : total;
+
+        // Where the share begins.
+        p.begin = from;
+        if (padded == 0) {
+            for (;; p.b += 64) {
+                if (a.sequences > 64) upto = tiles_from(p.b, own);
+                const int here = __builtin_amdgcn_readlane(upto, 63);
+                if (p.begin < here) break;
+                p.begin -= here;
+            }
+            const int at = __builtin_ctzll(__ballot(upto > p.begin));
+            p.begin -= __builtin_amdgcn_readlane(upto - own, at);
+            p.b += at;
+        }
+    }
+    const int start = padded != 0 ? 0 : kStartTiles;
+    int count, tiles, row_tiles;  // the sequence's: tiles looked at, counted, row tiles
+    const auto enter = [&] {
+        p.len = t.length(p.b);
+        p.q0 = t.first_query(p.b);
+        p.n = t.new_tokens(p.b, p.q0);
+        count = shared_tiles(a, p.b, p.len);
+        tiles = padded != 0 ? padded : count + start;
+        row_tiles = shared_row_tiles(a, kRows, p.n);
+    };
+    enter();
+    if (a.split_tiles == 0) {
+        if (index >= row_tiles) return;
+        to = tiles;
+    } else {
+        const int unit = p.begin / tiles;
+        p.begin -= unit * tiles;
+        p.h = unit / row_tiles;
+        index = unit - p.h * row_tiles;
+    }
+    for (int at = from; at < to;) {
+        const int left = to - at;
+        const int counted = p.begin, counted_end = left < tiles - counted ? counted + left : tiles;
+        p.begin = counted > start ? counted - start : 0;
+        p.end = counted_end > start ? counted_end - start : 0;
+        if (p.end > count) p.end = count;
+        // A row tile with nothing to read is written by the share that begins it.
+        if (p.begin < p.end || (count == 0 && counted == 0)) {
+            p.rows = row_tile<kReach>(a, index, kRows, p.len, p.n);
+            p.slot = p.begin == 0 && p.end == count ? -1 : 2 * s + (at != from);
+            if (p.begin == 0 && a.split_tiles != 0 && threadIdx.x == 0) {
+                // The row tile's first slot, and how many shares after it have a part.
+                const int64_t id = (a.slots == 0 ? static_cast<int64_t>(p.b) * a.row_tiles
+                                                 : static_cast<int64_t>(p.q0) * a.group / kRows + p.b) + index;
+                reinterpret_cast<int2*>(a.pieces)[id * t.kv_heads + p.h] =
+                    int2{p.slot, (at - counted + tiles - 1) / share - s};
+            }
+            wide_rows<E, D, kReach>(a, lds, p);
+        }
+        at += counted_end - counted;
+        p.begin = 0;
+        if (++index < row_tiles) continue;
+        index = 0;
+        if (++p.h < t.kv_heads) continue;
+        p.h = 0;
+        if (at >= to) break;
+        do {
+            ++p.b;
+            enter();
+        } while (p.n == 0);
+    }
+}
+
+// Joins the pieces of a row tile that several workgroups had a part of, D / 4
+// lanes a row and 1 << a.join_shift such groups of lanes, each with its part of
+// the pieces.  A lane looks up every D / 4-th piece's reference and sum, so that
+// all are under way at once.
+template <class E, int D, int kReach>
+__global__ __launch_bounds__(256) void kv_join_pieces_kernel(AttendArgs a)
+{
+    constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+    __shared__ float2 stats[kGroups];
+    __shared__ f32x4 theirs[kGroups][kLanes];
+    const Batch& t = a.batch;
+    const int h = blockIdx.x % t.kv_heads;
+    const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    const int ways = 1 << a.join_shift, way = group & (ways - 1);
+    const int r = (blockIdx.x / t.kv_heads * kGroups + group) >> a.join_shift;
+    Item it;
+    if (!item_of(a, kWideRows, it)) return;
+    const int2 entry = reinterpret_cast<const int2*>(a.pieces)[it.id * t.kv_heads + h];
+    const int len = t.length(it.b);
+    const int q0 = t.first_query(it.b);
+    const int n = t.new_tokens(it.b, q0);
+    const RowTile rt = row_tile<kReach>(a, it.index, kWideRows, len, n);
+    const int slot = entry.x, pieces = entry.y + 1;
+    if (rt.end <= rt.begin || slot < 0) return;  // no such tile, or written already
+    const bool in = rt.begin + r < rt.end;
+    // The parts after the first begin their shares: slots 2 (slot / 2 + i).
+    const auto row_of = [&](int i) {
+        return static_cast<int64_t>(i == 0 ? slot : 2 * (slot / 2 + i)) * kWideRows + r;
+    };
+    float top = -__builtin_inff(), total = 0.0f;
+    f32x4 acc{0, 0, 0, 0};
+    for (int base = way; in && base < pieces; base += kLanes * ways) {
+        float2 ml{-__builtin_inff(), 0.0f};
+        if (base + lane * ways < pieces)
+            ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * row_of(base + lane * ways));
+        float fresh = ml.x;
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) fresh = fmaxf(fresh, __shfl_xor(fresh, d));
+        fresh = fmaxf(fresh, top);
+        const float keep = fresh == -__builtin_inff() ? 0.0f : fresh;
+        const float old = __builtin_amdgcn_exp2f(top - keep);
+        top = fresh;
+        const float f = __builtin_amdgcn_exp2f(ml.x - keep);
+        total = total * old + f * ml.y;  // a lane's own pieces
+        acc *= old;
+        int count = (pieces - base + ways - 1) >> a.join_shift;
+        count = count < kLanes ? count : kLanes;
+#pragma unroll 8
+        for (int i = 0; i < count; ++i)
+            acc += __shfl(f, i, kLanes) *
+                   *reinterpret_cast<const f32x4*>(a.part_o + row_of(base + i * ways) * D + 4 * lane);
+    }
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1) total += __shfl_xor(total, d);
+    if (ways > 1) {
+        if (lane == 0) stats[group] = float2{top, total};
+        theirs[group][lane] = acc;
+        __syncthreads();
+        if (way != 0) return;
+        for (int w = 1; w < ways; ++w) top = fmaxf(top, stats[group + w].x);
+        const float keep = top == -__builtin_inff() ? 0.0f : top;
+        total = 0.0f;
+        acc = f32x4{0, 0, 0, 0};
+        for (int w = 0; w < ways; ++w) {
+            const float f = __builtin_amdgcn_exp2f(stats[group + w].x - keep);
+            total += f * stats[group + w].y;
+            acc += f * theirs[group + w][lane];
+        }
+    }
+    if (in) finish<E>(a, t, q0, h, rt.begin + r, 4 * lane, acc, top, total);
 }
 
 // Joins the splits' partial results of one row: four waves a row, wave w the
@@ -1146,9 +1537,6 @@ struct AttendPlan {
     dim3 grid, join;
 };
 
-// Rows of a workgroup of kv_attention_wide_kernel.
-constexpr int kWideRows = 128;
-
 // One launch each; defined per element type, dim and reach.
 template <class E, int D, int kReach>
 void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
@@ -1156,6 +1544,12 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
     if constexpr (kReach == kOwn) {
         if (p.wide) {
             kv_attention_wide_kernel<E, D><<<p.grid, 256, 0, stream>>>(a);
+            return;
+        }
+    } else {
+        if (p.wide) {
+            kv_attention_shared_kernel<E, D, kReach><<<p.grid, 256, 0, stream>>>(a);
+            if (a.split_tiles != 0) kv_join_pieces_kernel<E, D, kReach><<<p.join, 256, 0, stream>>>(a);
             return;
         }
     }

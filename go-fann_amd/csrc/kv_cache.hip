@@ -35,6 +35,81 @@ int split_tiles(const Context* ctx, uint64_t items, uint64_t most, bool ragged, 
     return static_cast<int>(n);
 }
 
+// Drafts and cross attention of more rows a sequence than this share their
+// tiles out, 128 rows a workgroup; fewer go to the kernel of few rows.  One
+// sequence of 40,000 positions, eight key/value heads, and 8 of 2,000 to 16,000,
+// us by the shared tiles / by few rows: 128 channels: 72 rows 47 / 40 and 51 / 48,
+// 128 rows 47 / 50 and 47 / 50, 256 rows 67 / 81 and 89 / 103; 64 channels: 128
+// rows 32 / 28 and 36 / 34, 256 rows 44 / 45 and 59 / 62; 256 channels: 72 rows
+// 86 / 72 and 95 / 98, 128 rows 95 / 120 and 98 / 104.
+bool shared_rows(uint64_t rows, uint32_t dim) { return rows > (dim == 64 ? 224u : 96u); }
+
+// Sequences whose tiles a workgroup counts for itself, 64 at a time.
+constexpr uint32_t kMostShared = 1024;
+
+// Tiles of a share at least: 25 tokens on 2,100 positions, 32 heads to 8, take
+// 17.8 us with 8, 21.5 with 16 and 27 with 32.
+constexpr int kLeastShare = 8;
+
+// Bytes that the list of the tiles that a filter leaves may have.
+constexpr uint64_t kLiveBytes = 64ull << 20;
+
+// How the tiles of drafts or of cross attention are shared out.
+struct AttendShape {
+    uint64_t row_tiles;   // of a sequence at most
+    uint64_t slots;       // as AttendArgs has it
+    uint64_t counted;     // tiles that the device counts, at most
+    uint32_t workgroups;  // shares; 0: every row tile is a workgroup's
+    int join_shift;
+    dim3 where;           // row tiles
+    uint64_t o_bytes, ml_bytes, piece_bytes, live_bytes, count_bytes;
+    uint64_t bytes() const { return o_bytes + ml_bytes + piece_bytes + live_bytes + count_bytes; }
+};
+
+AttendShape shared_shape(const Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
+                         uint64_t group, uint64_t tokens, uint64_t most_tiles)
+{
+    using namespace kv;
+    AttendShape s{};
+    const uint64_t heads = cache->kv_heads;
+    s.row_tiles = (tokens * group + kWideRows - 1) / kWideRows;
+    uint64_t all = s.row_tiles * batch->sequences;
+    const uint64_t slots = batch->queries * group / kWideRows + batch->sequences;
+    s.where = dim3(static_cast<uint32_t>(heads), static_cast<uint32_t>(s.row_tiles), batch->sequences);
+    if (batch->query_offsets != nullptr && 2 * slots <= all && slots <= 0x7FFFFFFFu) {
+        s.slots = all = slots;
+        s.where.y = slots < 65535 ? static_cast<uint32_t>(slots) : 65535u;
+        s.where.z = static_cast<uint32_t>((slots + s.where.y - 1) / s.where.y);
+    }
+    s.counted = (all + s.row_tiles) * heads * (most_tiles + kStartTiles);
+    // Two workgroups a CU are resident, at 256 channels one (LDS).
+    const uint64_t resident = static_cast<uint64_t>(ctx->compute_units) * (cache->dim == 256 ? 1 : 2);
+    const uint64_t workgroups = resident / kXcds * kXcds;
+    const uint64_t items = (batch->queries * group + kWideRows - 1) / kWideRows * heads;
+    // Enough row tiles to even out by themselves, the longest first, save the
+    // parts' way through memory: 6 x 701 tokens on 900 to 7,000 positions take 233
+    // us, 245 shared out; 4,096 on 5,000 345 and 364.  Not at 256 channels: 8 x 500
+    // tokens on 8,000 take 866, and 697 shared out.
+    if (s.slots == 0 && cache->dim < 256 && 2 * items >= 3 * workgroups) return s;
+    s.workgroups = static_cast<uint32_t>(workgroups);
+    // Row tiles in so many parts that a lane group has about eight of them.
+    while (s.join_shift < 3 && (8ull << s.join_shift) * items < workgroups) ++s.join_shift;
+    if (cache->dim == 256 && s.join_shift > 2) s.join_shift = 2;  // four lane groups a workgroup
+    const uint64_t parts = 2 * workgroups * kWideRows;
+    s.o_bytes = parts * cache->dim * sizeof(float);
+    s.ml_bytes = parts * 2 * sizeof(float);
+    s.piece_bytes = (all * heads * 2 * sizeof(int32_t) + 15) / 16 * 16;
+    // Where a filter may hide whole tiles, those that are left are listed and
+    // shared out: 16 drafts of 64 tokens on 1,000 to 16,000 positions, 0.6 of them
+    // visible in documents of 40 to 700, take 104 us, 121 without the list.
+    const uint64_t live = batch->visible == nullptr ? 0 : batch->sequences * most_tiles * 4 * sizeof(uint32_t);
+    if (live <= kLiveBytes) {
+        s.live_bytes = live;
+        s.count_bytes = live > 0 ? batch->sequences * sizeof(int32_t) : 0;
+    }
+    return s;
+}
+
 }  // namespace
 
 int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
@@ -114,6 +189,45 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         if (static_cast<uint64_t>(batch->sequences) * kFewRows < part_rows) {
             a.part_rows = kFewRows;
             part_rows = static_cast<uint64_t>(batch->sequences) * kFewRows;
+        }
+    }
+
+    if (!own && blocks == nullptr && shared_rows(rows, dim) && batch->sequences <= kMostShared) {
+        const AttendShape shape = shared_shape(ctx, cache, batch, a.group, tokens, most_tiles);
+        if (shape.row_tiles > 65535) return ctx->fail(GOFANN_ERR_UNSUPPORTED, too_many);
+        // Tiles are counted in 32 bits.
+        if (shape.counted < (1ull << 30)) {
+            AttendPlan p{};
+            p.wide = true;
+            a.row_tiles = static_cast<int>(shape.row_tiles);
+            a.slots = static_cast<int>(shape.slots);
+            if (shape.workgroups == 0) {
+                p.grid = shape.where;
+            } else {
+                a.split_tiles = kLeastShare;
+                a.join_shift = shape.join_shift;
+                a.live_stride = most_tiles;
+                char* const w = static_cast<char*>(ctx->workspace(Context::kScratchKv, shape.bytes()));
+                if (w == nullptr) return GOFANN_ERR_NOMEM;
+                a.part_o = reinterpret_cast<float*>(w);
+                a.part_ml = reinterpret_cast<float*>(w + shape.o_bytes);
+                a.pieces = reinterpret_cast<int32_t*>(w + shape.o_bytes + shape.ml_bytes);
+                if (shape.live_bytes > 0) {
+                    char* const live = w + shape.o_bytes + shape.ml_bytes + shape.piece_bytes;
+                    char* const count = live + shape.live_bytes;
+                    a.live = reinterpret_cast<uint32_t*>(live);
+                    a.live_count = reinterpret_cast<int32_t*>(count);
+                    kv_live_kernel<<<dim3((most_tiles + kLiveChunk - 1) / kLiveChunk, batch->sequences), 256, 0,
+                                     ctx->stream>>>(a, reinterpret_cast<u32x4*>(live),
+                                                    reinterpret_cast<int32_t*>(count));
+                }
+                p.grid = dim3(shape.workgroups);
+                p.join = dim3((cache->kv_heads * kWideRows * dim / 1024) << shape.join_shift, shape.where.y,
+                              shape.where.z);
+            }
+            launch(a, p);
+            if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_attention: launch");
+            return GOFANN_OK;
         }
     }
 
