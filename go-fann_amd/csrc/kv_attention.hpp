@@ -19,7 +19,7 @@ struct AttendArgs {
     float* part_o;          // [kv_heads][split][part_count][dim], splits > 1: see part_of()
     float* part_ml;         // [kv_heads][split][part_count][2]: reference, sum
     int32_t* pieces;        // [row tile][kv_heads][2] of shared tiles: first slot, shares after it
-    const uint32_t* live;   // [sequence][live_stride][4]: tiles that the filter leaves, see
+    const uint32_t* live;   // [sequence][live_stride][4]: tiles that the filter leaves, as kv_live_kernel
     const int32_t* live_count;  // kv_live_kernel; NULL: all of them are looked at
     int64_t live_stride;
     int join_shift;         // log2 of the groups of lanes that join a row's pieces
@@ -333,6 +333,22 @@ struct Raw {
     uint32_t vs[2];
 };
 
+// What a workgroup works on: tiles [begin, end) of a row tile.
+struct Piece {
+    int b, h, len, q0, n;
+    int begin, end;
+    int slot;  // of its partial result; negative: it has all of the row tile
+    RowTile rows;
+};
+
+// Where the four waves of a workgroup of few rows join what they have.
+template <int D, int NT>
+struct FewLds {
+    static constexpr int kResident = NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5;
+    float m[4][16 * NT], sum[4][16 * NT];
+    __attribute__((aligned(16))) float o[4][16][D + 4];  // rows start on other banks
+};
+
 // One row tile of one key/value head over one split of its positions.
 //
 // A tile of 32 positions is two 16 x 16 score tiles S^T = K Q^T and D / 16
@@ -358,30 +374,18 @@ struct Raw {
 // positions took 9% longer.  64 channels: five; 256: two, by 201 registers and
 // by the 69 KB of LDS that join the waves.  Short calls are a chain of dependent
 // loads: 8.6 us for 1,999 positions of 8 heads.
-template <class E, int D, int kReach, int NT>
-__global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) void kv_attention_kernel(AttendArgs a)
+template <class E, int D, int kReach, int NT, class F>
+__device__ __forceinline__ void few_rows(const AttendArgs& a, FewLds<D, NT>& lds, const Piece& piece, F&& put)
 {
     using V8 = typename E::V8;
-    constexpr int kRows = 16 * NT;
     constexpr int kUnit = D / 16;  // channels of a unit, tiles of O
     const Batch& t = a.batch;
     const int lane = threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int r16 = lane % 16, g4 = lane / 16;
-    const int h = blockIdx.x % t.kv_heads;
-    const int split = blockIdx.x / t.kv_heads;
-    Item it;
-    if (!item_of(a, kRows, it)) return;
-    const int index = it.index, b = it.b;
-    const int len = t.length(b);
-    const int q0 = t.first_query(b);
-    const int n = t.new_tokens(b, q0);
-    const RowTile rt = row_tile<kReach>(a, index, kRows, len, n);
-    if (rt.end <= rt.begin) return;
-    const int tiles = tiles_of(a, rt);
-    const int tile_begin = split * a.split_tiles;
-    if (split > 0 && tile_begin >= tiles) return;
-    const int tile_end = tile_begin + a.split_tiles < tiles ? tile_begin + a.split_tiles : tiles;
+    const int h = piece.h, b = piece.b, len = piece.len, q0 = piece.q0, n = piece.n;
+    const RowTile& rt = piece.rows;
+    const int tile_begin = piece.begin, tile_end = piece.end;
     const int hi_pos = rt.last_pos + 1;                         // positions that are read
     const int all_see = rt.first_pos + 1;                       // positions that every row sees
 
@@ -519,18 +523,29 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
         uint32_t at = 0, word = 0;
         int t0 = 0;
         if (tile < tile_end) {
-            int block = tile >> page_tiles_shift;
-            const int within = tile & ((1 << page_tiles_shift) - 1);
-            if (a.blocks != nullptr)
-                block = a.blocks[(static_cast<int64_t>(q0 + rt.token) * t.kv_heads + h) * a.width + block];
-            const int page = t.page(b, block);
-            // A block of a list may lie anywhere: only positions below hi_pos count.
-            if (page >= 0 && block <= (rt.last_pos >> t.page_shift)) {
-                t0 = (block << t.page_shift) + kTile * within;
-                if (t0 < hi_pos) {
-                    word = t.word(b, t0 >> 5);
-                    if (hi_pos - t0 < 32) word &= (1u << (hi_pos - t0)) - 1u;
-                    at = ((static_cast<uint32_t>(page) * t.kv_heads + h) << page_tiles_shift) + within;
+            if (kReach != kOwn && a.live != nullptr) {
+                const u32x4 entry = reinterpret_cast<const u32x4*>(a.live)[b * a.live_stride + tile];
+                const int page = entry[2];
+                t0 = static_cast<int>(entry[0]) * kTile;
+                if (page >= 0) {
+                    word = entry[1];
+                    at = ((static_cast<uint32_t>(page) * t.kv_heads + h) << page_tiles_shift) +
+                         (entry[0] & ((1 << page_tiles_shift) - 1));
+                }
+            } else {
+                int block = tile >> page_tiles_shift;
+                const int within = tile & ((1 << page_tiles_shift) - 1);
+                if (a.blocks != nullptr)
+                    block = a.blocks[(static_cast<int64_t>(q0 + rt.token) * t.kv_heads + h) * a.width + block];
+                const int page = t.page(b, block);
+                // A block of a list may lie anywhere: only positions below hi_pos count.
+                if (page >= 0 && block <= (rt.last_pos >> t.page_shift)) {
+                    t0 = (block << t.page_shift) + kTile * within;
+                    if (t0 < hi_pos) {
+                        word = t.word(b, t0 >> 5);
+                        if (hi_pos - t0 < 32) word &= (1u << (hi_pos - t0)) - 1u;
+                        at = ((static_cast<uint32_t>(page) * t.kv_heads + h) << page_tiles_shift) + within;
+                    }
                 }
             }
         }
@@ -601,13 +616,10 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
     // rows at a time: thread x then has four channels of row x / (D / 4)
     // and of every 256 / (D / 4)-th after it.
     constexpr int kLanes = D / 4, kStep = 256 / kLanes;
-    constexpr int kPad = D + 4;  // rows start on other banks
-    __shared__ float wm[4][kRows], ws[4][kRows];
-    __shared__ __attribute__((aligned(16))) float wo[4][16][kPad];
-    const int active = (tiles + a.split_tiles - 1) / a.split_tiles;
-    const int64_t item = it.id * t.kv_heads + h;
-    const int64_t my_part = part_of(a, b, q0, h, split);
     const int my_ch = 4 * (threadIdx.x % kLanes);
+    auto& wm = lds.m;
+    auto& ws = lds.sum;
+    auto& wo = lds.o;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         if (g4 == 0) {
@@ -639,24 +651,57 @@ __global__ __launch_bounds__(256, NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) vo
                 total += f * ws[w][16 * nt + r];
                 acc += f * *reinterpret_cast<const f32x4*>(&wo[w][r][my_ch]);
             }
-            if (active <= 1) {
-                finish<E>(a, t, q0, h, row, my_ch, acc, top, total);
-            } else {
-                const int64_t at = my_part + row;
-                float* const to = a.part_o + at * D + my_ch;
-                float* const pm = a.part_ml + 2 * at;
-                if (a.arrived != nullptr) {
-                    put2(to, acc[0], acc[1]);
-                    put2(to + 2, acc[2], acc[3]);
-                    if (my_ch == 0) put2(pm, top, total);
-                } else {
-                    *reinterpret_cast<f32x4*>(to) = acc;
-                    if (my_ch == 0) *reinterpret_cast<float2*>(pm) = float2{top, total};
-                }
-            }
+            put(16 * nt + r, my_ch, acc, top, total);
         }
         if (nt + 1 < NT) __syncthreads();
     }
+}
+
+template <class E, int D, int kReach, int NT>
+__global__ __launch_bounds__(256, (FewLds<D, NT>::kResident)) void kv_attention_kernel(AttendArgs a)
+{
+    constexpr int kRows = 16 * NT;
+    __shared__ FewLds<D, NT> lds;
+    const Batch& t = a.batch;
+    const int h = blockIdx.x % t.kv_heads;
+    const int split = blockIdx.x / t.kv_heads;
+    Item it;
+    if (!item_of(a, kRows, it)) return;
+    const int b = it.b;
+    const int len = t.length(b);
+    const int q0 = t.first_query(b);
+    const int n = t.new_tokens(b, q0);
+    const RowTile rt = row_tile<kReach>(a, it.index, kRows, len, n);
+    if (rt.end <= rt.begin) return;
+    const int tiles = tiles_of(a, rt);
+    const int tile_begin = split * a.split_tiles;
+    if (split > 0 && tile_begin >= tiles) return;
+    const int tile_end = tile_begin + a.split_tiles < tiles ? tile_begin + a.split_tiles : tiles;
+    const int active = (tiles + a.split_tiles - 1) / a.split_tiles;
+    const int64_t item = it.id * t.kv_heads + h;
+    const int64_t my_part = part_of(a, b, q0, h, split);
+    few_rows<E, D, kReach, NT>(
+        a, lds, Piece{b, h, len, q0, n, tile_begin, tile_end, -1, rt},
+        [&](int r, int my_ch, f32x4 acc, float top, float total) {
+            const int row = rt.begin + r;
+            if (active <= 1) {
+                finish<E>(a, t, q0, h, row, my_ch, acc, top, total);
+                return;
+            }
+            const int64_t at = my_part + row;
+            float* const to = a.part_o + at * D + my_ch;
+            float* const pm = a.part_ml + 2 * at;
+            if (a.arrived != nullptr) {
+                put2(to, acc[0], acc[1]);
+                put2(to + 2, acc[2], acc[3]);
+                if (my_ch == 0) put2(pm, top, total);
+            } else {
+                *reinterpret_cast<f32x4*>(to) = acc;
+                if (my_ch == 0) *reinterpret_cast<float2*>(pm) = float2{top, total};
+            }
+        });
+    constexpr int kLanes = D / 4, kStep = 256 / kLanes;
+    const int my_ch = 4 * (threadIdx.x % kLanes);
     if (active <= 1) return;
     if (a.arrived == nullptr) return;
     // The workgroup that arrives last joins the splits, in their order
@@ -720,14 +765,6 @@ struct WideLds {
     u32x4 values[2][kPer][D / 32][2][64];
 };
 
-// What such a workgroup works on: tiles [begin, end) of a row tile.
-struct WidePiece {
-    int b, h, len, q0, n;
-    int begin, end;
-    int slot;  // of its partial result; negative: it has all of the row tile
-    RowTile rows;
-};
-
 // Long chunks: four waves of 32 rows each read the same positions.
 //
 // A tile of 32 positions is D / 16 products S^T += K Q^T and D / 16 products
@@ -756,7 +793,7 @@ struct WidePiece {
 // 16 products): 0.69 ms where this took 0.63.  At 256 channels (1.44 ms) the
 // output and the queries leave 29 registers too few, spilled.
 template <class E, int D, int kReach>
-__device__ __forceinline__ void wide_rows(const AttendArgs& a, WideLds<D, kReach>& lds, const WidePiece& piece)
+__device__ __forceinline__ void wide_rows(const AttendArgs& a, WideLds<D, kReach>& lds, const Piece& piece)
 {
     using V8 = typename E::V8;
     constexpr int kRows = 32;
@@ -1127,7 +1164,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_wide_kernel(AttendArgs a)
 {
     __shared__ WideLds<D, kOwn> lds;
     const Batch& t = a.batch;
-    WidePiece p;
+    Piece p;
     p.h = blockIdx.x;
     p.b = blockIdx.z;
     p.len = t.length(p.b);
@@ -1160,63 +1197,7 @@ __device__ __forceinline__ int shared_tiles(const AttendArgs& a, int b, int len)
 // Beginning took 5 to 6 us, a tile of 128 channels 0.6 to 1.1; uncounted, a share
 // of ten short sequences took 82 us where the others took 48.
 constexpr int kStartTiles = 6;
-
-// The tiles of a sequence that its filter leaves something of, in order: tile,
-// filter word and page, a place of four words each.  A workgroup lists 1,024
-// tiles and counts for itself what lies before them.
-constexpr int kLiveChunk = 1024;
-static __global__ __launch_bounds__(256) void kv_live_kernel(AttendArgs a, u32x4* live, int32_t* count)
-{
-    __shared__ int part[4];
-    const Batch& t = a.batch;
-    const int b = blockIdx.y;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int len = t.length(b);
-    const int tiles = paged_tiles(t, len);
-    const int begin = blockIdx.x * kLiveChunk;
-    if (begin > 0 && begin >= tiles) return;
-    const auto word_of = [&](int tile) -> uint32_t {
-        if (tile >= tiles) return 0u;
-        const int left = (len < t.max_positions ? len : t.max_positions) - tile * kTile;
-        return t.word(b, tile) & (left < kTile ? (1u << left) - 1u : 0xFFFFFFFFu);
-    };
-    int before = 0;
-#pragma unroll 8
-    for (int tile = threadIdx.x; tile < begin; tile += 256) before += word_of(tile) != 0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) before += __shfl_xor(before, d);
-    if (lane == 0) part[wave] = before;
-    __syncthreads();
-    before = part[0] + part[1] + part[2] + part[3];
-    __syncthreads();
-    // Four tiles a thread, next to each other.
-    uint32_t word[4];
-    int own = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        word[i] = word_of(begin + 4 * threadIdx.x + i);
-        own += word[i] != 0;
-    }
-    int upto = own;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int x = __shfl_up(upto, d);
-        if (lane >= d) upto += x;
-    }
-    if (lane == 63) part[wave] = upto;
-    __syncthreads();
-    int at = before + upto - own;
-    for (int w = 0; w < wave; ++w) at += part[w];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (word[i] == 0) continue;
-        const int tile = begin + 4 * threadIdx.x + i;
-        const int page = t.page(b, tile >> (t.page_shift - 5));
-        live[static_cast<int64_t>(b) * a.live_stride + at++] =
-            u32x4{static_cast<uint32_t>(tile), word[i], static_cast<uint32_t>(page), 0};
-    }
-    if (begin + kLiveChunk >= tiles && threadIdx.x == 255) count[b] = at;
-}
+constexpr int kStartFew = 16;  // four waves take a tile each
 
 // Row tiles of a sequence of n tokens, at most as many as there is room for.
 __device__ __forceinline__ int shared_row_tiles(const AttendArgs& a, int rows, int n)
@@ -1234,14 +1215,12 @@ __device__ __forceinline__ int shared_row_tiles(const AttendArgs& a, int rows, i
 // kv_join_pieces_kernel joins.  Row tiles of one sequence and head stand next to
 // each other and a piece goes to the XCD that has its neighbours, so that they
 // find their positions in its L2.
-template <class E, int D, int kReach>
-__global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_attention_shared_kernel(AttendArgs a)
+template <int kReach, int kRows, int kStart, class F>
+__device__ __forceinline__ void share_out(const AttendArgs& a, F&& work)
 {
-    __shared__ WideLds<D, kReach> lds;
-    constexpr int kRows = kWideRows;
     const Batch& t = a.batch;
     const int lane = threadIdx.x % 64;
-    WidePiece p;
+    Piece p;
     p.b = 0;
     int s = 0, share = 1, from = 0, to = 1, index, padded = 0;
     if (a.split_tiles == 0) {  // so many row tiles that each is a workgroup's
@@ -1267,7 +1246,7 @@ __global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_atten
             if (b + lane < a.sequences) {
                 const int len = t.length(b + lane), q0 = t.first_query(b + lane);
                 own = shared_row_tiles(a, kRows, t.new_tokens(b + lane, q0)) *
-                      (shared_tiles(a, b + lane, len) + kStartTiles) * t.kv_heads;
+                      (shared_tiles(a, b + lane, len) + kStart) * t.kv_heads;
             }
             int upto = own;
 #pragma unroll
@@ -1290,7 +1269,7 @@ __global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_atten
         if (a.sequences == 1) {
             // All row tiles have as many tiles: parts that end with them.
             const int all = shared_tiles(a, 0, t.length(0));
-            const int items = total / (all + kStartTiles), room = workgroups / items;
+            const int items = total / (all + kStart), room = workgroups / items;
             if (room > 0 && all > 0) {
                 int parts = (all + share - 1) / share;
                 parts = parts < room ? parts : room;
@@ -1322,7 +1301,7 @@ __global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_atten
             p.b += at;
         }
     }
-    const int start = padded != 0 ? 0 : kStartTiles;
+    const int start = padded != 0 ? 0 : kStart;
     int count, tiles, row_tiles;  // the sequence's: tiles looked at, counted, row tiles
     const auto enter = [&] {
         p.len = t.length(p.b);
@@ -1359,7 +1338,7 @@ __global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_atten
                 reinterpret_cast<int2*>(a.pieces)[id * t.kv_heads + p.h] =
                     int2{p.slot, (at - counted + tiles - 1) / share - s};
             }
-            wide_rows<E, D, kReach>(a, lds, p);
+            work(p);
         }
         at += counted_end - counted;
         p.begin = 0;
@@ -1375,11 +1354,39 @@ __global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_atten
     }
 }
 
+// .. by 128 rows a workgroup,
+template <class E, int D, int kReach>
+__global__ __launch_bounds__(256, (WideLds<D, kReach>::kResident)) void kv_attention_shared_kernel(AttendArgs a)
+{
+    __shared__ WideLds<D, kReach> lds;
+    share_out<kReach, kWideRows, kStartTiles>(a, [&](const Piece& p) { wide_rows<E, D, kReach>(a, lds, p); });
+}
+
+// .. and by few rows.
+template <class E, int D, int kReach, int NT>
+__global__ __launch_bounds__(256, (FewLds<D, NT>::kResident)) void kv_attention_shared_few_kernel(AttendArgs a)
+{
+    constexpr int kRows = 16 * NT;
+    __shared__ FewLds<D, NT> lds;
+    share_out<kReach, kRows, kStartFew>(a, [&](const Piece& p) {
+        few_rows<E, D, kReach, NT>(a, lds, p, [&](int r, int ch, f32x4 acc, float top, float total) {
+            if (p.slot < 0) {
+                finish<E>(a, a.batch, p.q0, p.h, p.rows.begin + r, ch, acc, top, total);
+                return;
+            }
+            const int64_t at = static_cast<int64_t>(p.slot) * kRows + r;
+            *reinterpret_cast<f32x4*>(a.part_o + at * D + ch) = acc;
+            if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top, total};
+        });
+        __syncthreads();  // LDS is free again
+    });
+}
+
 // Joins the pieces of a row tile that several workgroups had a part of, D / 4
 // lanes a row and 1 << a.join_shift such groups of lanes, each with its part of
 // the pieces.  A lane looks up every D / 4-th piece's reference and sum, so that
 // all are under way at once.
-template <class E, int D, int kReach>
+template <class E, int D, int kReach, int kRows>
 __global__ __launch_bounds__(256) void kv_join_pieces_kernel(AttendArgs a)
 {
     constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
@@ -1391,18 +1398,18 @@ __global__ __launch_bounds__(256) void kv_join_pieces_kernel(AttendArgs a)
     const int ways = 1 << a.join_shift, way = group & (ways - 1);
     const int r = (blockIdx.x / t.kv_heads * kGroups + group) >> a.join_shift;
     Item it;
-    if (!item_of(a, kWideRows, it)) return;
+    if (!item_of(a, kRows, it)) return;
     const int2 entry = reinterpret_cast<const int2*>(a.pieces)[it.id * t.kv_heads + h];
     const int len = t.length(it.b);
     const int q0 = t.first_query(it.b);
     const int n = t.new_tokens(it.b, q0);
-    const RowTile rt = row_tile<kReach>(a, it.index, kWideRows, len, n);
+    const RowTile rt = row_tile<kReach>(a, it.index, kRows, len, n);
     const int slot = entry.x, pieces = entry.y + 1;
     if (rt.end <= rt.begin || slot < 0) return;  // no such tile, or written already
     const bool in = rt.begin + r < rt.end;
     // The parts after the first begin their shares: slots 2 (slot / 2 + i).
     const auto row_of = [&](int i) {
-        return static_cast<int64_t>(i == 0 ? slot : 2 * (slot / 2 + i)) * kWideRows + r;
+        return static_cast<int64_t>(i == 0 ? slot : 2 * (slot / 2 + i)) * kRows + r;
     };
     float top = -__builtin_inff(), total = 0.0f;
     f32x4 acc{0, 0, 0, 0};
@@ -1534,6 +1541,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a)
 struct AttendPlan {
     int nt;      // 16-row tiles a wave holds
     bool wide;   // four row tiles a workgroup over the same positions
+    bool shared; // drafts, cross attention: few rows, their tiles shared out
     dim3 grid, join;
 };
 
@@ -1549,8 +1557,19 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
     } else {
         if (p.wide) {
             kv_attention_shared_kernel<E, D, kReach><<<p.grid, 256, 0, stream>>>(a);
-            if (a.split_tiles != 0) kv_join_pieces_kernel<E, D, kReach><<<p.join, 256, 0, stream>>>(a);
+            if (a.split_tiles != 0) kv_join_pieces_kernel<E, D, kReach, kWideRows><<<p.join, 256, 0, stream>>>(a);
             return;
+        }
+        if (p.shared) {
+            const auto few = [&](auto nt) {
+                constexpr int kNt = decltype(nt)::value;
+                kv_attention_shared_few_kernel<E, D, kReach, kNt><<<p.grid, 256, 0, stream>>>(a);
+                kv_join_pieces_kernel<E, D, kReach, 16 * kNt><<<p.join, 256, 0, stream>>>(a);
+            };
+            if constexpr (D < 256) {
+                if (p.nt == 2) return few(std::integral_constant<int, 2>{});
+            }
+            return few(std::integral_constant<int, 1>{});
         }
     }
     const auto run = [&](auto nt) {

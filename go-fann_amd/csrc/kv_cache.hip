@@ -3,6 +3,69 @@
 #include "kv_attention.hpp"
 
 namespace gofann {
+namespace kv {
+namespace {
+
+// The tiles of a sequence that its filter leaves something of, in order: tile,
+// filter word and page, a place of four words each.  A workgroup lists 1,024
+// tiles and counts for itself what lies before them.
+constexpr int kLiveChunk = 1024;
+__global__ __launch_bounds__(256) void kv_live_kernel(AttendArgs a, u32x4* live, int32_t* count)
+{
+    __shared__ int part[4];
+    const Batch& t = a.batch;
+    const int b = blockIdx.y;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int len = t.length(b);
+    const int tiles = paged_tiles(t, len);
+    const int begin = blockIdx.x * kLiveChunk;
+    if (begin > 0 && begin >= tiles) return;
+    const auto word_of = [&](int tile) -> uint32_t {
+        if (tile >= tiles) return 0u;
+        const int left = (len < t.max_positions ? len : t.max_positions) - tile * kTile;
+        return t.word(b, tile) & (left < kTile ? (1u << left) - 1u : 0xFFFFFFFFu);
+    };
+    int before = 0;
+#pragma unroll 8
+    for (int tile = threadIdx.x; tile < begin; tile += 256) before += word_of(tile) != 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) before += __shfl_xor(before, d);
+    if (lane == 0) part[wave] = before;
+    __syncthreads();
+    before = part[0] + part[1] + part[2] + part[3];
+    __syncthreads();
+    // Four tiles a thread, next to each other.
+    uint32_t word[4];
+    int own = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        word[i] = word_of(begin + 4 * threadIdx.x + i);
+        own += word[i] != 0;
+    }
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(upto, d);
+        if (lane >= d) upto += x;
+    }
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    int at = before + upto - own;
+    for (int w = 0; w < wave; ++w) at += part[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (word[i] == 0) continue;
+        const int tile = begin + 4 * threadIdx.x + i;
+        const int page = t.page(b, tile >> (t.page_shift - 5));
+        live[static_cast<int64_t>(b) * a.live_stride + at++] =
+            u32x4{static_cast<uint32_t>(tile), word[i], static_cast<uint32_t>(page), 0};
+    }
+    if (begin + kLiveChunk >= tiles && threadIdx.x == 255) count[b] = at;
+}
+
+}  // namespace
+}  // namespace kv
+
 namespace {
 
 // Rows up to which a sequence of a long-chunk launch is left to the other kernel.
@@ -35,21 +98,36 @@ int split_tiles(const Context* ctx, uint64_t items, uint64_t most, bool ragged, 
     return static_cast<int>(n);
 }
 
-// Drafts and cross attention of more rows a sequence than this share their
-// tiles out, 128 rows a workgroup; fewer go to the kernel of few rows.  One
-// sequence of 40,000 positions, eight key/value heads, and 8 of 2,000 to 16,000,
-// us by the shared tiles / by few rows: 128 channels: 72 rows 47 / 40 and 51 / 48,
-// 128 rows 47 / 50 and 47 / 50, 256 rows 67 / 81 and 89 / 103; 64 channels: 128
-// rows 32 / 28 and 36 / 34, 256 rows 44 / 45 and 59 / 62; 256 channels: 72 rows
-// 86 / 72 and 95 / 98, 128 rows 95 / 120 and 98 / 104.
-bool shared_rows(uint64_t rows, uint32_t dim) { return rows > (dim == 64 ? 224u : 96u); }
-
 // Sequences whose tiles a workgroup counts for itself, 64 at a time.
 constexpr uint32_t kMostShared = 1024;
 
-// Tiles of a share at least: 25 tokens on 2,100 positions, 32 heads to 8, take
-// 17.8 us with 8, 21.5 with 16 and 27 with 32.
-constexpr int kLeastShare = 8;
+// Whether drafts and cross attention of `rows` rows a sequence share their tiles
+// out by 128 rows a workgroup, not by 16 or 32: past 256, where their row tiles
+// are nearly as full.  8 sequences of 2,000 to 16,000 positions, eight key/value
+// heads, us by few / by 128 rows: 128 channels: 128 rows 42 / 47, 256 rows 81 / 89,
+// 384 rows 123 / 117; 256 channels: 223 / 238 and 363 / 313 of 256 and 384 rows; 64
+// channels: 59 / 59 and 87 / 76; 19 drafts of 280 rows of 64 channels 27 / 33.
+bool many_rows(uint64_t rows)
+{
+    return rows > 256 && 10 * ((rows + 127) / 128 * 128) <= 11 * ((rows + 31) / 32 * 32);
+}
+
+// Whether few rows share their tiles out at all: up to 16 rows, whose kernels
+// have no registers left for it, and short calls, which a second launch would
+// lengthen, keep splits of one length, joined by the last of them.  One sequence
+// of 2,000 positions and 64 rows of 128 channels takes 18.7 us by splits, 15.7
+// shared out; of 1,000 13.9 and 15.2; 16 sequences of 250 to 1,000 18.5 and 22.2;
+// 16 of 1,000 to 16,000 and 72 rows 32.6 and 30.8; 32 of 500 to 16,000 under a
+// filter 80 and 63.
+bool share_few(uint64_t rows, uint32_t dim, uint64_t items, uint64_t most_tiles, int compute_units)
+{
+    return rows > 16 && (most_tiles > 64 || items * most_tiles * dim >= 4096ull * compute_units);
+}
+
+// Tiles of a share at least.  25 tokens on 2,100 positions, 32 heads to 8, by 128
+// rows: 17.8 us with 8, 21.5 with 16 and 27 with 32; few rows of one sequence of
+// 2,000 positions 15.7 with 8 and 16.8 with 16, of four 20.5 and 18.6.
+int least_share(bool wide, uint32_t sequences) { return wide || sequences == 1 ? 8 : 16; }
 
 // Bytes that the list of the tiles that a filter leaves may have.
 constexpr uint64_t kLiveBytes = 64ull << 20;
@@ -67,35 +145,37 @@ struct AttendShape {
 };
 
 AttendShape shared_shape(const Context* ctx, const gofann_kv_cache* cache, const gofann_kv_batch* batch,
-                         uint64_t group, uint64_t tokens, uint64_t most_tiles)
+                         uint64_t group, uint64_t tokens, uint64_t most_tiles, uint64_t per)
 {
     using namespace kv;
     AttendShape s{};
     const uint64_t heads = cache->kv_heads;
-    s.row_tiles = (tokens * group + kWideRows - 1) / kWideRows;
+    s.row_tiles = (tokens * group + per - 1) / per;
     uint64_t all = s.row_tiles * batch->sequences;
-    const uint64_t slots = batch->queries * group / kWideRows + batch->sequences;
+    const uint64_t slots = batch->queries * group / per + batch->sequences;
     s.where = dim3(static_cast<uint32_t>(heads), static_cast<uint32_t>(s.row_tiles), batch->sequences);
     if (batch->query_offsets != nullptr && 2 * slots <= all && slots <= 0x7FFFFFFFu) {
         s.slots = all = slots;
         s.where.y = slots < 65535 ? static_cast<uint32_t>(slots) : 65535u;
         s.where.z = static_cast<uint32_t>((slots + s.where.y - 1) / s.where.y);
     }
-    s.counted = (all + s.row_tiles) * heads * (most_tiles + kStartTiles);
-    // Two workgroups a CU are resident, at 256 channels one (LDS).
-    const uint64_t resident = static_cast<uint64_t>(ctx->compute_units) * (cache->dim == 256 ? 1 : 2);
-    const uint64_t workgroups = resident / kXcds * kXcds;
-    const uint64_t items = (batch->queries * group + kWideRows - 1) / kWideRows * heads;
+    s.counted = (all + s.row_tiles) * heads * (most_tiles + kStartFew);
+    // Workgroups that are resident: of 128 rows two a CU, at 256 channels one (LDS).
+    const bool wide = per == kWideRows;
+    const uint64_t each = wide ? (cache->dim == 256 ? 1 : 2)
+                               : per == 32 || cache->dim == 256 ? 2 : cache->dim == 128 ? 4 : 5;
+    const uint64_t workgroups = each * static_cast<uint64_t>(ctx->compute_units) / kXcds * kXcds;
+    const uint64_t items = (batch->queries * group + per - 1) / per * heads;
     // Enough row tiles to even out by themselves, the longest first, save the
     // parts' way through memory: 6 x 701 tokens on 900 to 7,000 positions take 233
     // us, 245 shared out; 4,096 on 5,000 345 and 364.  Not at 256 channels: 8 x 500
     // tokens on 8,000 take 866, and 697 shared out.
-    if (s.slots == 0 && cache->dim < 256 && 2 * items >= 3 * workgroups) return s;
+    if (wide && s.slots == 0 && cache->dim < 256 && 2 * items >= 3 * workgroups) return s;
     s.workgroups = static_cast<uint32_t>(workgroups);
     // Row tiles in so many parts that a lane group has about eight of them.
-    while (s.join_shift < 3 && (8ull << s.join_shift) * items < workgroups) ++s.join_shift;
-    if (cache->dim == 256 && s.join_shift > 2) s.join_shift = 2;  // four lane groups a workgroup
-    const uint64_t parts = 2 * workgroups * kWideRows;
+    const int most_shift = cache->dim == 256 ? 2 : 3;  // four lane groups a workgroup
+    while (s.join_shift < most_shift && (8ull << s.join_shift) * items < workgroups) ++s.join_shift;
+    const uint64_t parts = 2 * workgroups * per;
     s.o_bytes = parts * cache->dim * sizeof(float);
     s.ml_bytes = parts * 2 * sizeof(float);
     s.piece_bytes = (all * heads * 2 * sizeof(int32_t) + 15) / 16 * 16;
@@ -192,19 +272,27 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         }
     }
 
-    if (!own && blocks == nullptr && shared_rows(rows, dim) && batch->sequences <= kMostShared) {
-        const AttendShape shape = shared_shape(ctx, cache, batch, a.group, tokens, most_tiles);
+    // Drafts and cross attention: tiles shared out.
+    const bool many = many_rows(rows);
+    const uint64_t per_few = rows <= 16 || dim == 256 ? 16 : 32;
+    const uint64_t few_items = (static_cast<uint64_t>(batch->queries) * a.group + per_few - 1) / per_few * cache->kv_heads;
+    if (!own && blocks == nullptr && batch->sequences <= kMostShared &&
+        (many || share_few(rows, dim, few_items, most_tiles, ctx->compute_units))) {
+        AttendPlan p{};
+        p.wide = many;
+        p.shared = !many;
+        p.nt = static_cast<int>(per_few / 16);
+        const uint64_t per = many ? kWideRows : per_few;
+        const AttendShape shape = shared_shape(ctx, cache, batch, a.group, tokens, most_tiles, per);
         if (shape.row_tiles > 65535) return ctx->fail(GOFANN_ERR_UNSUPPORTED, too_many);
         // Tiles are counted in 32 bits.
         if (shape.counted < (1ull << 30)) {
-            AttendPlan p{};
-            p.wide = true;
             a.row_tiles = static_cast<int>(shape.row_tiles);
             a.slots = static_cast<int>(shape.slots);
             if (shape.workgroups == 0) {
                 p.grid = shape.where;
             } else {
-                a.split_tiles = kLeastShare;
+                a.split_tiles = least_share(many, batch->sequences);
                 a.join_shift = shape.join_shift;
                 a.live_stride = most_tiles;
                 char* const w = static_cast<char*>(ctx->workspace(Context::kScratchKv, shape.bytes()));
@@ -222,7 +310,7 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
                                                     reinterpret_cast<int32_t*>(count));
                 }
                 p.grid = dim3(shape.workgroups);
-                p.join = dim3((cache->kv_heads * kWideRows * dim / 1024) << shape.join_shift, shape.where.y,
+                p.join = dim3((cache->kv_heads * static_cast<uint32_t>(per) * dim / 1024) << shape.join_shift, shape.where.y,
                               shape.where.z);
             }
             launch(a, p);
