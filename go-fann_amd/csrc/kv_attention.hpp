@@ -344,7 +344,7 @@ struct Piece {
 // Where the four waves of a workgroup of few rows join what they have.
 template <int D, int NT>
 struct FewLds {
-    static constexpr int kResident = NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5;
+    static constexpr int kResident = NT == 2 && D == 256 ? 1 : NT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5;
     float m[4][16 * NT], sum[4][16 * NT];
     __attribute__((aligned(16))) float o[4][16][D + 4];  // rows start on other banks
 };
@@ -1566,10 +1566,10 @@ void attend_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t stream)
                 kv_attention_shared_few_kernel<E, D, kReach, kNt><<<p.grid, 256, 0, stream>>>(a);
                 kv_join_pieces_kernel<E, D, kReach, 16 * kNt><<<p.join, 256, 0, stream>>>(a);
             };
-            if constexpr (D < 256) {
-                if (p.nt == 2) return few(std::integral_constant<int, 2>{});
+            if constexpr (D == 256) {
+                if (p.nt == 1) return few(std::integral_constant<int, 1>{});
             }
-            return few(std::integral_constant<int, 1>{});
+            return few(std::integral_constant<int, 2>{});
         }
     }
     const auto run = [&](auto nt) {

@@ -105,11 +105,24 @@ constexpr uint32_t kMostShared = 1024;
 // out by 128 rows a workgroup, not by 16 or 32: past 256, where their row tiles
 // are nearly as full.  8 sequences of 2,000 to 16,000 positions, eight key/value
 // heads, us by few / by 128 rows: 128 channels: 128 rows 42 / 47, 256 rows 81 / 89,
-// 384 rows 123 / 117; 256 channels: 223 / 238 and 363 / 313 of 256 and 384 rows; 64
-// channels: 59 / 59 and 87 / 76; 19 drafts of 280 rows of 64 channels 27 / 33.
-bool many_rows(uint64_t rows)
+// 384 rows 123 / 117; 256 channels, four heads: 102 / 104, 160 / 169 and 387 / 403
+// of 256, 384 and 1,024 rows; 64 channels: 59 / 59 and 87 / 76 of 256 and 384; 19
+// drafts of 280 rows of 64 channels 27 / 33.  One sequence of 256 channels stays
+// with few rows further: 1,024 rows on 40,000 positions 239 / 284, on 10,000 76 / 97.
+bool many_rows(uint64_t rows, uint32_t dim, uint32_t sequences)
 {
-    return rows > 256 && 10 * ((rows + 127) / 128 * 128) <= 11 * ((rows + 31) / 32 * 32);
+    return rows > (dim == 256 && sequences == 1 ? 2048u : 256u) &&
+           10 * ((rows + 127) / 128 * 128) <= 11 * ((rows + 31) / 32 * 32);
+}
+
+// Tiles of 16 rows a wave that has few of them.  Two have no room for a second
+// wave a SIMD at 256 channels and pay there where there is much to read: 128 rows
+// on 40,000 positions 78 us, 90 with one; on 4,000 24.7 and 24.2; 72 rows on 40,000
+// 66 and 65.5.
+uint64_t few_tiles(uint64_t rows, uint32_t dim, uint64_t most_tiles)
+{
+    if (rows <= 16) return 1;
+    return dim < 256 || (rows >= 128 && most_tiles > 256) ? 2 : 1;
 }
 
 // Whether few rows share their tiles out at all: up to 16 rows, whose kernels
@@ -163,7 +176,7 @@ AttendShape shared_shape(const Context* ctx, const gofann_kv_cache* cache, const
     // Workgroups that are resident: of 128 rows two a CU, at 256 channels one (LDS).
     const bool wide = per == kWideRows;
     const uint64_t each = wide ? (cache->dim == 256 ? 1 : 2)
-                               : per == 32 || cache->dim == 256 ? 2 : cache->dim == 128 ? 4 : 5;
+                               : per == 32 && cache->dim == 256 ? 1 : per == 32 || cache->dim == 256 ? 2 : cache->dim == 128 ? 4 : 5;
     const uint64_t workgroups = each * static_cast<uint64_t>(ctx->compute_units) / kXcds * kXcds;
     const uint64_t items = (batch->queries * group + per - 1) / per * heads;
     // Enough row tiles to even out by themselves, the longest first, save the
@@ -273,8 +286,8 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
     }
 
     // Drafts and cross attention: tiles shared out.
-    const bool many = many_rows(rows);
-    const uint64_t per_few = rows <= 16 || dim == 256 ? 16 : 32;
+    const bool many = many_rows(rows, dim, batch->sequences);
+    const uint64_t per_few = 16 * few_tiles(rows, dim, most_tiles);
     const uint64_t few_items = (static_cast<uint64_t>(batch->queries) * a.group + per_few - 1) / per_few * cache->kv_heads;
     if (!own && blocks == nullptr && batch->sequences <= kMostShared &&
         (many || share_few(rows, dim, few_items, most_tiles, ctx->compute_units))) {

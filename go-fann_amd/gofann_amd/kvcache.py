@@ -332,11 +332,14 @@ class KvCache:
         the batch's tokens, exactly; with k or v given, only what is given, into
         it.  Rows of tokens without a page are zero."""
         self._ready(batch)
-        n, h = batch.queries, self.kv_heads
+        n, h, d = batch.queries, self.kv_heads, self.dim
         if k is None and v is None:
-            k, v = torch.empty((2, n, h, self.dim), dtype=self.dtype, device=self.device)
-        rk = None if k is None else self._rows("k", k, n, h, True)
-        rv = None if v is None else self._rows("v", v, n, h, True)
+            k = torch.empty((n, h, d), dtype=self.dtype, device=self.device)
+            v = torch.empty_like(k)
+            rk, rv = _lib.KvRows(k.data_ptr(), h * d, d), _lib.KvRows(v.data_ptr(), h * d, d)
+        else:
+            rk = None if k is None else self._rows("k", k, n, h, True)
+            rv = None if v is None else self._rows("v", v, n, h, True)
         self.ctx.check(self.lib.gofann_kv_read(self.ctx.handle, self.view, batch.view, rk, rv))
         return k, v
 
@@ -355,10 +358,11 @@ class KvCache:
 
 
 def _draft(ctx: _lib.Context, batch: KvBatch, **rows: torch.Tensor) -> None:
-    if batch.device.type != "cuda" or batch.device.index != ctx.device:
+    device, shape = batch.device, (batch.queries,)
+    if device.type != "cuda" or device.index != ctx.device:
         raise ValueError("the batch is not on the context's device")
     for name, t in rows.items():
-        _ints(name, t, (batch.queries,), batch.device)
+        _ints(name, t, shape, device)
     _current(ctx)
 
 
@@ -372,8 +376,7 @@ def draft_tree(ctx: _lib.Context, batch: KvBatch,
     a root.  At most 8192 tokens a sequence."""
     _draft(ctx, batch, parents=parents)
     words = (batch.max_queries + 31) // 32
-    sees = torch.empty((batch.queries, words), dtype=torch.int32, device=batch.device)
-    depths = torch.empty_like(parents)
+    sees, depths = parents.new_empty(batch.queries, words), torch.empty_like(parents)
     ctx.check(ctx.lib.gofann_kv_draft_tree(ctx.handle, batch.view, parents.data_ptr(), words,
                                            sees.data_ptr(), depths.data_ptr()))
     return sees, depths
@@ -391,8 +394,7 @@ def draft_accept(ctx: _lib.Context, batch: KvBatch, parents: torch.Tensor, draft
     _draft(ctx, batch, parents=parents, drafted=drafted, chosen=chosen)
     _counts(width=width)
     n = batch.sequences
-    path = torch.empty((n, width), dtype=torch.int32, device=batch.device)
-    lengths, answer = torch.empty((2, n), dtype=torch.int32, device=batch.device)
+    path, lengths, answer = parents.new_empty(n, width), parents.new_empty(n), parents.new_empty(n)
     ctx.check(ctx.lib.gofann_kv_draft_accept(
         ctx.handle, batch.view, parents.data_ptr(), drafted.data_ptr(), chosen.data_ptr(), width,
         path.data_ptr(), lengths.data_ptr(), answer.data_ptr()))
