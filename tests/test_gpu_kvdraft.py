@@ -643,3 +643,58 @@ def test_drafts_in_a_cache_past_four_gigabytes(ctx):
     torch.cuda.synchronize()
     for name in c.NAMES:
         assert np.array_equal(getattr(d, name)[150_000 - 4:].cpu().numpy(), getattr(c, name)), name
+
+
+def test_session_with_drafts(ctx, capsys):
+    """Drafts and steps of one token by turns, against what the cache then holds; refusals
+    leave the sequences as they were."""
+    from gofann_amd import longcontext
+    r = np.random.default_rng(6)
+    s = longcontext.Session(ctx, sequences=2, capacity=200, kv_heads=2, dim=64, page=32)
+    c = ref.Cache(14, 2, 32, 64, "bf16")
+    have = [40, 40]
+    p0 = [rows(r, 80, h, 64, "bf16") for h in (8, 2, 2)]
+    s.step(*(t for t, _ in p0))
+    put = lambda b, pos, k, v: c.write(7 * b + pos // 32, pos % 32, k, v)  # noqa: E731
+    for b in range(2):
+        for i in range(40):
+            put(b, i, p0[1][1][40 * b + i], p0[2][1][40 * b + i])
+    for turn, n in enumerate((11, 1, 20, 7)):
+        (q, q64), (k, k64), (v, v64) = (rows(r, 2 * n, h, 64, "bf16") for h in (8, 2, 2))
+        p = draft.trees([n, n], seed=turn)
+        tok, ans = (r.integers(0, 2, 2 * n).astype(np.int32) for _ in range(2))
+        sees, _ = draft.tree([n, n], p)
+        out = s.draft(q, k, v, dev(p))
+        for b in range(2):
+            for i in range(n):
+                put(b, have[b] + i, k64[b * n + i], v64[b * n + i])
+        b_ = ref.Batch(32, [h + n for h in have], [n, n], pages=14)
+        b_.table, b_.width = np.arange(14, dtype=np.int32).reshape(2, 7), 7
+        want = draft.attend(c, b_, q64, 64 ** -0.5, sees)
+        check_attend(out, None, want[0], None, want[2])
+        for bad in (lambda: s.draft(q, k, v, dev(p)), lambda: s.step(q, k, v), lambda: s.grow(1)):
+            with pytest.raises(ValueError, match="settled"):
+                bad()
+        path, answer = s.settle(dev(tok), dev(ans), 4)
+        want = draft.accept(b_.lens, [n, n], p, tok, ans, 4)
+        assert np.array_equal(path.cpu().numpy(), want[0]) and np.array_equal(answer.cpu().numpy(), want[2])
+        draft.keep(c, b_, want[0])
+        have = list(want[1])
+        assert s.lengths.tolist() == have and s.filled >= max(have)
+        (q, q64), (k, k64), (v, v64) = (rows(r, 2, h, 64, "bf16") for h in (8, 2, 2))
+        out = s.step(q, k, v)
+        for b in range(2):
+            put(b, have[b], k64[b], v64[b])
+        have = [h + 1 for h in have]
+        b_ = ref.Batch(32, have, [1, 1], pages=14)
+        b_.table, b_.width = np.arange(14, dtype=np.int32).reshape(2, 7), 7
+        want = ref.attend(c, b_, q64, 64 ** -0.5)
+        check_attend(out, None, want[0], None, want[2])
+    with pytest.raises(ValueError, match="no draft"):
+        s.settle(dev(tok), dev(ans), 4)
+    bound, lens = s.filled, s.lengths.tolist()
+    with pytest.raises(ValueError):
+        s.draft(q, k, v[:1], torch.full((2,), -1, dtype=torch.int32, device="cuda"))
+    assert s.filled == bound and s.lengths.tolist() == lens and s.pending is None
+    longcontext.main(["--context", "1500", "--steps", "2", "--sequences", "2", "--width", "8", "--draft", "13"])
+    assert "13 drafted tokens" in capsys.readouterr().out

@@ -281,9 +281,51 @@ def case_nothing_to_do(f: Drafts):
     assert len(f.launched()) == 1
 
 
-def case_workspace_under_capture(f: Drafts):
+def case_launches(f: Drafts):
+    """Which kernels a call takes, by its rows, what there is to read, and its sequences."""
+    h = f.context()
+
+    def names(call, heads=32, dim=128, **kw):
+        assert call(h, heads=heads, cache=f.cache(dim=dim), batch=f.batch(**kw)) == f.L.OK
+        return [n.split("kernel")[0].split("kv_")[-1] for n, _ in f.launched()]
+
+    shared, few = ["attention_shared_", "join_pieces_"], ["attention_shared_few_", "join_pieces_"]
     for call in (f.draft, f.cross):
+        one = dict(sequences=1, queries=1)
+        assert names(call, **one, max_length=2000) == ["attention_"]
+        assert names(call, **one, max_length=32768) == ["attention_", "join_"]
+        # more than 16 rows: shared out where there is something to share
+        some = dict(sequences=1, queries=16, max_queries=16)
+        assert names(call, **some, max_length=1000) == ["attention_"]
+        assert names(call, **some, max_length=4000) == few
+        assert names(call, **some, max_length=4000, dim=256) == few
+        assert names(call, sequences=64, queries=1024, max_queries=16, max_length=1000) == few
+        # 128 rows a workgroup, and enough of them
+        many = dict(sequences=1, queries=128, max_queries=128)
+        assert names(call, **many, max_length=4000) == shared
+        assert names(call, **many, max_length=4000, dim=256) == few
+        assert names(call, sequences=2, queries=256, max_queries=128, max_length=4000, dim=256) == shared
+        # 288 rows: a third tile of 128 would be mostly empty
+        assert names(call, sequences=1, queries=72, max_queries=72, max_length=4000) == few
+        assert names(call, sequences=4, queries=4096, max_queries=1024) == ["attention_shared_"]
+        # a filter's tiles are listed first, unless the list would be too long
+        p = dict(visible=f.p, visible_stride=1024, visible_width=1024)
+        assert names(call, **some, max_length=4000, **p) == ["live_", *few]
+        assert names(call, sequences=1000, queries=16000, max_queries=16, max_length=2 ** 18,
+                     table_width=4096, table_stride=4096, **p) == few
+        # sequences past those that tiles are shared out over
+        assert "attention_shared_few_" not in names(call, sequences=1025, queries=1025 * 16, max_queries=16)
+    assert names(f.draft, **some, max_length=4000) == few
+    assert f.draft(h, blocks=f.p, width=64, batch=f.batch(**some)) == f.L.OK
+    assert [n for n, _ in f.launched() if "shared" in n] == []
+
+
+def case_workspace_under_capture(f: Drafts):
+    few, many = dict(queries=64, max_queries=16), dict(queries=512, max_queries=128)
+    for call, kw in ((f.draft, {}), (f.cross, {}), (f.draft, few), (f.cross, few), (f.draft, many), (f.cross, many)):
         h = f.context(host.SIDE)
+        big = f.batch(**kw)
+        call = lambda h, to=call: to(h, batch=big)  # noqa: E731
         f.hip.fake_capture(host.SIDE)
         assert call(h) == f.L.ERR_NOMEM
         assert b"before capturing" in f.lib.gofann_last_error(h)
