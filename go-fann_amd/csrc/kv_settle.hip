@@ -22,7 +22,7 @@ struct TreeArgs {
 // A thread a token: the walk from it to its root goes to ever lower tokens, so
 // its words are finished from the highest down and each is written once.  The
 // parents up to the workgroup's last token are in LDS; a step of the walk is
-// one read of it.  40 tokens for each of 64 sequences take 3.9 us, mostly the
+// one read of it.  40 tokens for each of 64 sequences take 3.4 us, mostly the
 // launch and the chain of offsets and parents.
 __global__ __launch_bounds__(256) void kv_tree_kernel(TreeArgs a)
 {
@@ -79,7 +79,8 @@ struct AcceptArgs {
 // A wave a sequence.  A child's index is above its parent's, so one pass over
 // the tokens, 64 at a time, finds the whole path: of those past the path's last
 // token, the lowest that is its child and drafted its answer, again and again
-// until the 64 hold none.  A step is a comparison a lane and a ballot.
+// until the 64 hold none.  A step is a comparison a lane and a ballot; 64
+// sequences of up to 40 tokens take 3.2 us.
 __global__ __launch_bounds__(64) void kv_accept_kernel(AcceptArgs a)
 {
     const Batch& t = a.batch;
@@ -136,9 +137,9 @@ struct KeepArgs {
 // turns lie past everything that an earlier turn wrote, and a turn's rows are
 // all in registers before any is written.  D / 8 threads a row, as append has.
 //
-// Latency bounds it: 64 sequences of 8 heads, up to 10 rows moved and a page's
-// keys read for its box, take 8.8 us: offsets and path, page ids, rows, then
-// keys, one after another.
+// Latency bounds it: 64 sequences of 8 heads of 128 channels, up to 10 rows moved
+// and a page's keys read for its box, take 6.9 us: offsets and path, page ids,
+// rows, then keys, one after another.
 template <class E, int D>
 __global__ __launch_bounds__(256) void kv_keep_kernel(KeepArgs a)
 {
