@@ -210,3 +210,92 @@ def test_bounds_below_what_the_device_says_write_nothing_out_of_place(ctx):
     w.cache.cross(short, w.q, out=out)
     same = (out == 99.0).flatten(1).all(1) | ((out.float() - full.float()).abs() < 0.2).flatten(1).all(1)
     assert same.all()
+
+
+@pytest.mark.parametrize("how", ["cross", "draft"])
+@pytest.mark.parametrize("elem,dim,heads,group,length", [("bf16", 128, 2, 40, 3000), ("f16", 64, 1, 300, 2500),
+                                                         ("bf16", 256, 1, 24, 2300), ("f16", 128, 1, 1024, 400)])
+def test_one_token_each_under_many_heads(ctx, elem, dim, heads, group, length, how):
+    """Rows of one token alone, without offsets, in every kind of row tile."""
+    from gofann_amd import kvcache
+    w = World(ctx, elem, dim, 64, heads, group, [length, 7, length // 2], [1, 1, 1], 0.6, seed=group)
+    w.batch = kvcache.KvBatch(w.table, w.batch._keep[1], max_length=length, visible=w.batch._keep[3])
+    w.run(how)
+
+
+@pytest.mark.parametrize("how", ["cross", "draft"])
+@pytest.mark.parametrize("dim,new,group", [(128, 40, 4), (128, 128, 4), (64, 130, 3), (256, 30, 2), (256, 200, 2)])
+def test_far_scores_and_strange_queries_in_shared_tiles(ctx, how, dim, new, group):
+    """Scaled scores past 2^22, and queries that hold an infinity or NaN, whose rows alone are lost."""
+    w = World(ctx, "bf16", dim, 64, 2, group, [2600, 2500], [new, 3], seed=dim)
+    call = (lambda q, **kw: w.cache.cross(w.batch, q, **kw)) if how == "cross" else \
+        (lambda q, **kw: w.cache.attend(w.batch, q, sees=w.words, **kw))
+    clean = call(w.q)
+    q = w.q.clone()
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    for at, x in (((0, 1), float("nan")), ((1, 0), float("inf")), ((new, 2 * group - 1), float("-inf"))):
+        q[(*at, 5)] = x
+        bad[at] = True
+    out = call(q)
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad])
+    # one channel alone, of scores that are multiples of a large power of two: only the highest has weight
+    q = torch.zeros_like(w.q)
+    q[:, :, 0] = 1.0
+    out = call(q, scale=2.0 ** 26)
+    for b, n in enumerate(w.lens):
+        k, v = w.k[w.starts[b]:w.starts[b] + n], w.v[w.starts[b]:w.starts[b] + n]
+        for i in range(w.new[b]):
+            ok = torch.ones(n, dtype=torch.bool, device="cuda")
+            if how == "draft":
+                ok[n - w.new[b]:] = torch.from_numpy(w.sees[w.off[b] + i][:w.new[b]]).cuda()
+            for h in range(2):
+                best = ok & (k[:, h, 0] == k[ok, h, 0].max())
+                want = v[best, h].mean(0)
+                off = (out[w.off[b] + i, h * group].double() - want).abs()
+                # weights of one, an output's rounding, and sums of at most n values in 32 bits
+                assert (off <= want.abs() * 2.0 ** -8 + v[best, h].abs().max() * n * 2.0 ** -23).all()
+
+
+@pytest.mark.parametrize("dim,new", [(128, 30), (128, 128), (64, 1)])
+def test_a_filter_without_words_hides_everything(ctx, dim, new):
+    from gofann_amd import kvcache
+    w = World(ctx, "f16", dim, 64, 2, 4, [2600, 200], [new, 1], seed=1)
+    none = kvcache.KvBatch(w.table, w.batch._keep[1], w.batch._keep[2], queries=w.n, max_queries=new,
+                           max_length=2600, visible=torch.empty((2, 0), dtype=torch.int32, device="cuda"))
+    lse = torch.zeros((w.n, 8), device="cuda")
+    assert (w.cache.cross(none, w.q, lse=lse) == 0).all() and torch.isneginf(lse).all()
+    lse.zero_()
+    assert (w.cache.attend(none, w.q, sees=w.words, lse=lse) == 0).all() and torch.isneginf(lse).all()
+
+
+def test_graphs_of_shared_tiles_replay_after_larger_calls(gpu_ctx):
+    """A captured call of shared tiles under a filter keeps its workspace while eager calls of other
+    sizes, and a second graph, use the context between its replays."""
+    from gofann_amd import _lib
+    own = _lib.Context(0)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        own.bind_stream(side)
+        some = World(own, "bf16", 128, 64, 2, 4, [3000, 500], [20, 9], 0.5, seed=1)
+        more = World(own, "bf16", 128, 64, 2, 4, [2600, 2500, 900], [128, 100, 7], 0.5, seed=2)
+        outs = [torch.empty_like(w.q) for w in (some, more)]
+        call = lambda w, out: w.cache.attend(w.batch, w.q, sees=w.words, out=out)  # noqa: E731
+        graphs = []
+        for w, out in zip((some, more), outs):
+            call(w, out)
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                call(w, out)
+            graphs.append(g)
+        for i in range(4):
+            for w, out, g in zip((some, more), outs, graphs):
+                w.q.normal_()
+                out.fill_(9.0)
+                g.replay()
+                side.synchronize()
+                seen = out.clone()
+                assert torch.equal(seen, call(w, out))
+                more.cache.cross(more.batch, more.q)
+            side.synchronize()
+    own.close()
