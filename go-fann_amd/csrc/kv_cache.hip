@@ -173,11 +173,12 @@ AttendShape shared_shape(const Context* ctx, const gofann_kv_cache* cache, const
         s.where.z = static_cast<uint32_t>((slots + s.where.y - 1) / s.where.y);
     }
     s.counted = (all + s.row_tiles) * heads * (most_tiles + kStartFew);
-    // Workgroups that are resident: of 128 rows two a CU, at 256 channels one (LDS).
+    // Workgroups that are resident: two a CU; of 128 or 32 rows of 256 channels one
+    // (LDS, registers).  A third of 32 rows of 64 channels gave 1% on average.
     const bool wide = per == kWideRows;
-    const uint64_t each = wide ? (cache->dim == 256 ? 1 : 2)
-                               : per == 32 && cache->dim == 256 ? 1 : per == 32 || cache->dim == 256 ? 2 : cache->dim == 128 ? 4 : 5;
-    const uint64_t workgroups = each * static_cast<uint64_t>(ctx->compute_units) / kXcds * kXcds;
+    const uint64_t each = cache->dim == 256 && per > 16 ? 1 : 2;
+    uint64_t workgroups = each * static_cast<uint64_t>(ctx->compute_units) / kXcds * kXcds;
+    if (workgroups == 0) workgroups = kXcds;
     const uint64_t items = (batch->queries * group + per - 1) / per * heads;
     // Enough row tiles to even out by themselves, the longest first, save the
     // parts' way through memory: 6 x 701 tokens on 900 to 7,000 positions take 233
@@ -248,7 +249,12 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         else
             of_reach(std::integral_constant<int, kOwn>{});
     };
-    const char* const too_many = "kv_attention: too many tokens a sequence for one call";
+    const bool own = !reach.cross && reach.sees == nullptr;
+    const auto fail = [&](int code, const char* what) {
+        const char* const call = own ? "kv_attention: " : reach.cross ? "kv_cross_attention: " : "kv_draft_attention: ";
+        return ctx->fail(code, std::string(call) + what);
+    };
+    const char* const too_many = "too many tokens a sequence for one call";
     uint64_t rows = blocks != nullptr ? static_cast<uint64_t>(a.group)
                                       : static_cast<uint64_t>(tokens) * a.group;
     a.rows_upto = 0x7FFFFFFF;
@@ -260,13 +266,12 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
     // the decoding ones of a mixed batch, would each keep a workgroup busy with
     // all of their positions; they are left to the other kernel.
     const uint64_t all_rows = static_cast<uint64_t>(batch->queries) * a.group;
-    const bool own = !reach.cross && reach.sees == nullptr;
     if (own && blocks == nullptr && rows > kFewRows &&
         all_rows / kWideRows * cache->kv_heads >= static_cast<uint64_t>(ctx->compute_units)) {
         AttendPlan p{};
         p.wide = true;
         const uint64_t row_tiles = (rows + kWideRows - 1) / kWideRows;
-        if (row_tiles > 65535) return ctx->fail(GOFANN_ERR_UNSUPPORTED, too_many);
+        if (row_tiles > 65535) return fail(GOFANN_ERR_UNSUPPORTED, too_many);
         a.splits = 1;
         a.split_tiles = static_cast<int>(most_tiles);
         a.row_tiles = static_cast<int>(row_tiles);
@@ -274,7 +279,7 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         a.rows_over = mixed ? kFewRows : 0;
         p.grid = dim3(cache->kv_heads, static_cast<uint32_t>(row_tiles), batch->sequences);
         launch(a, p);
-        if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_attention: launch");
+        if (hipGetLastError() != hipSuccess) return fail(GOFANN_ERR_HIP, "launch");
         if (!mixed) return GOFANN_OK;
         a.rows_over = 0;
         a.rows_upto = kFewRows;
@@ -288,7 +293,7 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
     // Drafts and cross attention: tiles shared out.
     const bool many = many_rows(rows, dim, batch->sequences);
     const uint64_t per_few = 16 * few_tiles(rows, dim, most_tiles);
-    const uint64_t few_items = (static_cast<uint64_t>(batch->queries) * a.group + per_few - 1) / per_few * cache->kv_heads;
+    const uint64_t few_items = (all_rows + per_few - 1) / per_few * cache->kv_heads;
     if (!own && blocks == nullptr && batch->sequences <= kMostShared &&
         (many || share_few(rows, dim, few_items, most_tiles, ctx->compute_units))) {
         AttendPlan p{};
@@ -297,7 +302,7 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         p.nt = static_cast<int>(per_few / 16);
         const uint64_t per = many ? kWideRows : per_few;
         const AttendShape shape = shared_shape(ctx, cache, batch, a.group, tokens, most_tiles, per);
-        if (shape.row_tiles > 65535) return ctx->fail(GOFANN_ERR_UNSUPPORTED, too_many);
+        if (shape.row_tiles > 65535) return fail(GOFANN_ERR_UNSUPPORTED, too_many);
         // Tiles are counted in 32 bits.
         if (shape.counted < (1ull << 30)) {
             a.row_tiles = static_cast<int>(shape.row_tiles);
@@ -323,11 +328,11 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
                                                     reinterpret_cast<int32_t*>(count));
                 }
                 p.grid = dim3(shape.workgroups);
-                p.join = dim3((cache->kv_heads * static_cast<uint32_t>(per) * dim / 1024) << shape.join_shift, shape.where.y,
-                              shape.where.z);
+                const uint32_t lanes = static_cast<uint32_t>(per) * dim / 4 << shape.join_shift;
+                p.join = dim3(cache->kv_heads * lanes / 256, shape.where.y, shape.where.z);
             }
             launch(a, p);
-            if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_attention: launch");
+            if (hipGetLastError() != hipSuccess) return fail(GOFANN_ERR_HIP, "launch");
             return GOFANN_OK;
         }
     }
@@ -342,7 +347,7 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
     a.token_tiles = static_cast<int>((a.group + per - 1) / per);
     const uint64_t row_tiles =
         blocks != nullptr ? static_cast<uint64_t>(tokens) * a.token_tiles : (rows + per - 1) / per;
-    if (row_tiles > 65535) return ctx->fail(GOFANN_ERR_UNSUPPORTED, too_many);
+    if (row_tiles > 65535) return fail(GOFANN_ERR_UNSUPPORTED, too_many);
     a.row_tiles = static_cast<int>(row_tiles);
     // Tiles counted through the sequences where a grid of them is twice as many:
     // 63 sequences of one token and one of 128, 32 heads to 8, up to 8,192
@@ -382,7 +387,7 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
     p.grid = dim3(cache->kv_heads * static_cast<uint32_t>(a.splits), where.y, where.z);
     p.join = dim3(cache->kv_heads * per, where.y, where.z);
     launch(a, p);
-    if (hipGetLastError() != hipSuccess) return ctx->fail(GOFANN_ERR_HIP, "kv_attention: launch");
+    if (hipGetLastError() != hipSuccess) return fail(GOFANN_ERR_HIP, "launch");
     return GOFANN_OK;
 }
 
