@@ -292,6 +292,8 @@ class KvCache:
         if sees.numel() and (sees.stride(1) != 1 or (sees.shape[0] > 1 and sees.stride(0) < words)):
             raise ValueError("sees must be contiguous along its last axis, its rows apart")
         stride = sees.stride(0) if sees.shape[0] > 1 else words
+        if stride >= 1 << 32:
+            raise ValueError("rows of sees must be less than 2^32 words apart")
         # Without words there is no address, and none is read.
         at = sees.data_ptr() if words else out.data_ptr() & ~3
         self.ctx.check(self.lib.gofann_kv_draft_attention(

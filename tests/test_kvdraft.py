@@ -132,6 +132,19 @@ def test_bits_that_are_refused(cache):
     assert len(cache.calls) == n
 
 
+def test_rows_of_bits_too_far_apart_are_refused(cache):
+    import torch
+
+    class Far(torch.Tensor):  # a view into more words than a 32-bit stride spans
+        def stride(self, *axis):
+            return 1 if axis == (1,) else 1 << 32
+
+    b, q = _batch(), torch.zeros(5, 4, 128, dtype=cache.dtype)
+    far = torch.zeros(5, 2, dtype=torch.int32).as_subclass(Far)
+    with pytest.raises(ValueError, match="sees"):
+        cache.attend(b, q, sees=far)
+
+
 def test_rows_and_paths_that_are_refused(cache):
     import torch
     b = _batch()
