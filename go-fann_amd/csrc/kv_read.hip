@@ -36,8 +36,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a)
     // first have no page, as blocks past the table have none.
     const int start = len - n;
     const int block = (start >> t.page_shift) + static_cast<int>(blockIdx.y);
+    // Compared as blocks: behind a length near 2^31 the position would wrap.
+    if (block > (len - 1) >> t.page_shift) return;
     const int page_begin = block * P;
-    if (page_begin >= len) return;
     const int page = t.page(b, block);
     const int from = start > page_begin ? start - page_begin : 0;
     const int there = len - page_begin < P ? len - page_begin : P;
