@@ -1405,6 +1405,8 @@ __global__ __launch_bounds__(256) void kv_join_pieces_kernel(AttendArgs a)
     const int r = (blockIdx.x / t.kv_heads * kGroups + group) >> a.join_shift;
     Item it;
     if (!item_of(a, kRows, it)) return;
+    // Tokens beyond the host's bound: no share had them, and nothing was noted of them.
+    if (it.index >= a.row_tiles) return;
     const int2 entry = reinterpret_cast<const int2*>(a.pieces)[it.id * t.kv_heads + h];
     const int len = t.length(it.b);
     const int q0 = t.first_query(it.b);

@@ -6,6 +6,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_kvdraft_shapes import World
+
 pytestmark = pytest.mark.gpu
 
 
@@ -38,3 +40,37 @@ def test_reading_behind_a_length_next_to_2_to_the_31(ctx, page, dim):
         for got, held in zip(rows, want):
             assert torch.equal(got[1:1 + many], held)
             assert (got[:1] == 0).all() and (got[1 + many:] == 0).all()
+
+
+@pytest.mark.parametrize("how", ["cross", "draft"])
+@pytest.mark.parametrize("dim,lens,new,group,most,per", [
+    (128, [2500, 2300], [128, 100], 4, 96, 128),             # a grid of row tiles
+    (128, [2400] * 60, [2] * 37 + [600] + [2] * 22, 4, 96, 128),  # counted through the sequences
+    (128, [2400] * 60, [2] * 37 + [600] + [2] * 22, 4, 64, 32),
+    (64, [2200] * 70, [1] * 5 + [300, 150] + [3] * 63, 2, 30, 32),
+    (256, [2200] * 60, [3] * 59 + [200], 2, 60, 16),
+])
+def test_tokens_beyond_max_queries_are_left_out(ctx, dim, lens, new, group, most, per, how):
+    """Offsets that give sequences more tokens than the call's bound: the row tiles that there is room
+    for are right, and every other row is left as it is."""
+    from gofann_amd import kvcache
+    w = World(ctx, "bf16", dim, 64, 2, group, lens, new, seed=most)
+    scale = 0.7 * dim ** -0.5
+    call = (lambda b, **kw: w.cache.cross(b, w.q, scale=scale, **kw)) if how == "cross" else \
+        (lambda b, **kw: w.cache.attend(b, w.q, scale=scale, sees=w.words, **kw))
+    full_lse = torch.empty(w.n, 2 * group, device="cuda")
+    full = call(w.batch, lse=full_lse)
+    short = kvcache.KvBatch(w.table, w.batch._keep[1], w.batch._keep[2], queries=w.n, max_queries=most,
+                            max_length=max(lens))
+    room = -(-most * group // per) * per  # rows of a sequence
+    nth = np.concatenate([np.arange(m) for m in new])
+    row = torch.from_numpy(nth).cuda()[:, None, None] * group + torch.arange(group, device="cuda")
+    there = (row < room).expand(w.n, 2, group).reshape(w.n, 2 * group)
+    assert there.any() and not there.all()
+    for _ in range(2):  # the second call finds the first one's notes in its scratch
+        out, lse = torch.full_like(w.q, 99.0), torch.full_like(full_lse, 77.0)
+        call(short, out=out, lse=lse)
+        assert (out[~there] == 99.0).all() and (lse[~there] == 77.0).all()
+        w.check(torch.where(there[..., None], out, full), torch.where(there, lse, full_lse), scale,
+                None if how == "cross" else w.sees)
+        call(w.batch)
