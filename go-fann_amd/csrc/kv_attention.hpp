@@ -1201,6 +1201,9 @@ constexpr int kStartTiles = 6;
 // to 16,000 positions take 81 us with 6, 73 with 10, 67 with 16 and 24, 74 with 48.
 constexpr int kStartFew = 16;
 
+// More tiles than a call counts: the host takes other ways from here on.
+constexpr int kMostCounted = (1 << 30) - 1;
+
 // Row tiles of a sequence of n tokens, at most as many as there is room for.
 __device__ __forceinline__ int shared_row_tiles(const AttendArgs& a, int rows, int n)
 {
@@ -1246,7 +1249,8 @@ __device__ __forceinline__ void share_out(const AttendArgs& a, F&& work)
         p.begin = 0;
     } else {
         // Tiles of 64 sequences from b on, a sequence a lane: those of the lanes up
-        // to this one, and this one's.
+        // to this one, and this one's.  A sequence's own are below kMostCounted.
+        const auto capped = [](int x) { return x < kMostCounted ? x : kMostCounted; };
         const auto tiles_from = [&](int b, int& own) {
             own = 0;
             if (b + lane < a.sequences) {
@@ -1258,16 +1262,24 @@ __device__ __forceinline__ void share_out(const AttendArgs& a, F&& work)
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const int x = __shfl_up(upto, d);
-                if (lane >= d) upto += x;
+                if (lane >= d) upto = capped(upto + x);
             }
             return upto;
         };
         int total = 0, own, upto;
         for (int b = 0; b < a.sequences; b += 64) {
             upto = tiles_from(b, own);
-            total += __builtin_amdgcn_readlane(upto, 63);
+            total = capped(total + __builtin_amdgcn_readlane(upto, 63));
         }
         if (total == 0) return;
+        if (total == kMostCounted) {
+            // Row offsets that overlap give more than the host bounds: no row tile
+            // is worked on, and all are noted as written.
+            const int64_t all = static_cast<int64_t>(a.slots) * t.kv_heads;
+            for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256)
+                reinterpret_cast<int2*>(a.pieces)[i] = int2{-1, 0};
+            return;
+        }
         const int workgroups = gridDim.x;
         share = (total + workgroups - 1) / workgroups;
         if (share < a.split_tiles) share = a.split_tiles;

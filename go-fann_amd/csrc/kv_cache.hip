@@ -304,7 +304,7 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         const AttendShape shape = shared_shape(ctx, cache, batch, a.group, tokens, most_tiles, per);
         if (shape.row_tiles > 65535) return fail(GOFANN_ERR_UNSUPPORTED, too_many);
         // Tiles are counted in 32 bits.
-        if (shape.counted < (1ull << 30)) {
+        if (shape.counted < kMostCounted) {
             a.row_tiles = static_cast<int>(shape.row_tiles);
             a.slots = static_cast<int>(shape.slots);
             if (shape.workgroups == 0) {

@@ -74,3 +74,37 @@ def test_tokens_beyond_max_queries_are_left_out(ctx, dim, lens, new, group, most
         w.check(torch.where(there[..., None], out, full), torch.where(there, lse, full_lse), scale,
                 None if how == "cross" else w.sees)
         call(w.batch)
+
+
+@pytest.mark.parametrize("how", ["cross", "draft"])
+@pytest.mark.parametrize("length,sequences", [(480_000, 1024), (470_000, 1000), (2000, 1024), (30_000, 200)])
+def test_offsets_that_overlap_compute_nothing_out_of_place(ctx, how, length, sequences):
+    """Every second sequence has all of the call's rows.  The longest count more tiles than 32 bits
+    hold, where the bounds that the host goes by (rows in all) count a quarter of 2^30."""
+    from gofann_amd import kvcache
+    dim, heads, tokens, group, page = 64, 64, 64, 4, 256
+    g = torch.Generator(device="cuda").manual_seed(length)
+    rnd = lambda lo, hi, *s: torch.randint(lo, hi, s, device="cuda", generator=g).to(torch.uint8)  # noqa: E731
+    cache = kvcache.KvCache(ctx, rnd(0, 256, 8, heads, page, dim // 2), rnd(123, 127, 8, heads, page, dim // 32),
+                            rnd(0, 256, 8, heads, page // 8, 16, 8, dim // 32),
+                            rnd(123, 127, 8, heads, page // 8, dim // 32, 8))
+    dev = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.full((sequences, -(-length // page)), -1, dtype=torch.int32, device="cuda")
+    table[:, :8] = torch.arange(8, dtype=torch.int32, device="cuda")[:table.shape[1]]
+    offsets = dev(([0, tokens] * sequences)[:sequences + 1])
+    lengths = dev([length] * sequences)
+    q = torch.randn(tokens, heads * group, dim, device="cuda", generator=g).to(cache.dtype)
+    words = torch.full((tokens, tokens // 32), -1, dtype=torch.int32, device="cuda")
+    call = (lambda b, **kw: cache.cross(b, q, **kw)) if how == "cross" else \
+        (lambda b, **kw: cache.attend(b, q, sees=words, **kw))
+    one = kvcache.KvBatch(table[:1], lengths[:1], dev([0, tokens]), queries=tokens, max_queries=tokens, max_length=length)
+    want = call(one)
+    around = torch.full((3, *q.shape), 99.0, dtype=q.dtype, device="cuda")
+    lse = torch.full((3, tokens, heads * group), 77.0, device="cuda")
+    for _ in range(2):
+        bad = kvcache.KvBatch(table, lengths, offsets, queries=tokens, max_queries=tokens, max_length=length)
+        call(bad, out=around[1], lse=lse[1])
+        assert (around[::2] == 99.0).all() and (lse[::2] == 77.0).all()
+        if length > 400_000:
+            assert (around[1] == 99.0).all() and (lse[1] == 77.0).all()
+        assert torch.equal(call(one), want)
