@@ -166,7 +166,8 @@ AttendShape shared_shape(const Context* ctx, const gofann_kv_cache* cache, const
     s.row_tiles = (tokens * group + per - 1) / per;
     uint64_t all = s.row_tiles * batch->sequences;
     const uint64_t slots = batch->queries * group / per + batch->sequences;
-    s.where = dim3(static_cast<uint32_t>(heads), static_cast<uint32_t>(s.row_tiles), batch->sequences);
+    const dim3 grid(static_cast<uint32_t>(heads), static_cast<uint32_t>(s.row_tiles), batch->sequences);
+    s.where = grid;
     if (batch->query_offsets != nullptr && 2 * slots <= all && slots <= 0x7FFFFFFFu) {
         s.slots = all = slots;
         s.where.y = slots < 65535 ? static_cast<uint32_t>(slots) : 65535u;
@@ -184,7 +185,12 @@ AttendShape shared_shape(const Context* ctx, const gofann_kv_cache* cache, const
     // parts' way through memory: 6 x 701 tokens on 900 to 7,000 positions take 233
     // us, 245 shared out; 4,096 on 5,000 345 and 364.  Not at 256 channels: 8 x 500
     // tokens on 8,000 take 866, and 697 shared out.
-    if (wide && s.slots == 0 && cache->dim < 256 && 2 * items >= 3 * workgroups) return s;
+    // Nor are those of a call counted that may have too many tiles for it.
+    if (wide && (s.counted >= kMostCounted || (s.slots == 0 && cache->dim < 256 && 2 * items >= 3 * workgroups))) {
+        s.slots = 0;
+        s.where = grid;
+        return s;
+    }
     s.workgroups = static_cast<uint32_t>(workgroups);
     // Row tiles in so many parts that a lane group has about eight of them.
     const int most_shift = cache->dim == 256 ? 2 : 3;  // four lane groups a workgroup
@@ -303,8 +309,9 @@ int kv_attention(Context* ctx, const gofann_kv_cache* cache, const gofann_kv_bat
         const uint64_t per = many ? kWideRows : per_few;
         const AttendShape shape = shared_shape(ctx, cache, batch, a.group, tokens, most_tiles, per);
         if (shape.row_tiles > 65535) return fail(GOFANN_ERR_UNSUPPORTED, too_many);
-        // Tiles are counted in 32 bits.
-        if (shape.counted < kMostCounted) {
+        // Tiles are counted in 32 bits.  Few rows that may have too many go by splits:
+        // 1,024 sequences of 64 rows, eight heads, from 2,100,000 positions on.
+        if (shape.workgroups == 0 || shape.counted < kMostCounted) {
             a.row_tiles = static_cast<int>(shape.row_tiles);
             a.slots = static_cast<int>(shape.slots);
             if (shape.workgroups == 0) {

@@ -108,3 +108,24 @@ def test_offsets_that_overlap_compute_nothing_out_of_place(ctx, how, length, seq
         if length > 400_000:
             assert (around[1] == 99.0).all() and (lse[1] == 77.0).all()
         assert torch.equal(call(one), want)
+
+
+@pytest.mark.parametrize("how", ["cross", "draft"])
+@pytest.mark.parametrize("filt", [0.0, 0.5])
+@pytest.mark.parametrize("dim,group,lens,new,tiles", [
+    (256, 2, [700, 300, 500, 301, 640, 333, 450, 600], [300, 200, 300, 1, 17, 300, 0, 260], 380_000),
+    (128, 4, [650] * 100, [1] * 50 + [600] + [3] * 49, 120_000),  # more sequences than are ordered by length
+])
+def test_bounds_past_a_count_of_tiles(ctx, dim, group, lens, new, tiles, filt, how):
+    """A length's bound so loose that tiles are not counted: a row tile a workgroup."""
+    from gofann_amd import kvcache
+    w = World(ctx, "bf16", dim, 256, 64, group, lens, new, filt, seed=dim)
+    pages = tiles // 8
+    table = torch.full((len(lens), pages), -1, dtype=torch.int32, device="cuda")
+    table[:, :w.table.shape[1]] = w.table
+    row_tiles = -(-max(new) * group // 128)
+    grid, slots = row_tiles * len(lens), sum(new) * group // 128 + len(lens)
+    assert ((slots if 2 * slots <= grid else grid) + row_tiles) * 64 * tiles > 1 << 30
+    w.batch = kvcache.KvBatch(table, w.batch._keep[1], w.batch._keep[2], queries=w.n, max_queries=max(new),
+                              max_length=tiles * 32, visible=w.batch._keep[3])
+    w.run(how, set(range(8)) | set(range(48, 53)))
