@@ -29,6 +29,7 @@ class Session:
     """Sequences of equal capacity whose pages are handed out in order."""
 
     pending = None  # a draft that is not settled: its batch, its parents, `filled` before it
+    loose = False   # drafts were settled: the sequences may be shorter than `filled`
 
     def __init__(self, ctx: _lib.Context, *, sequences: int, capacity: int, kv_heads: int = 8,
                  dim: int = 128, page: int = 64, dtype: torch.dtype = torch.bfloat16):
@@ -46,6 +47,10 @@ class Session:
         """The batch of `tokens` further tokens of every sequence."""
         if self.pending is not None:
             raise ValueError("a draft is not settled")
+        if self.filled + tokens > self.capacity and self.loose:
+            # Only the device knows how many tokens of the drafts were kept: it is
+            # asked, and waited for, where the bound would refuse.
+            self.filled, self.loose = int(self.lengths.max()), False
         if self.filled + tokens > self.capacity:
             raise ValueError("the sequences are full")
         self.filled += tokens
@@ -95,8 +100,8 @@ class Session:
         them: each over what came before the draft, its ancestors and itself.  The
         sequences hold the whole draft until `settle`."""
         tokens = self._tokens(q)
-        before = self.filled
         batch = self.grow(tokens)
+        before = self.filled - tokens
         try:
             sees, _ = draft_tree(self.cache.ctx, batch, parents)
             self.cache.append(batch, k, v)
@@ -118,7 +123,7 @@ class Session:
         self.cache.keep(batch, path)
         self.lengths.copy_(lengths)
         self.filled = before + min(width, batch.max_queries)
-        self.pending = None
+        self.pending, self.loose = None, True
         return path, answer
 
 

@@ -1,16 +1,75 @@
-"""Edges of drafts and cross attention without a GPU: plans of calls with large
-bounds, over the stand-in HIP runtime."""
+"""Edges of drafts and cross attention without a GPU: the example's bounds, and plans
+of calls with large ones over the stand-in HIP runtime."""
 from __future__ import annotations
 
 import subprocess
 import sys
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 
 sys.path.insert(0, str(Path(__file__).resolve().parent))
 import test_host_dispatch as host  # noqa: E402
 from test_kvdraft import Drafts  # noqa: E402
+
+
+# ---- the example ------------------------------------------------------------------
+
+def test_settled_drafts_leave_the_room_that_they_did_not_take(monkeypatch):
+    """A session is full when its longest sequence is, not when its drafts could have made it so."""
+    import torch
+    from gofann_amd import longcontext
+    s = longcontext.Session.__new__(longcontext.Session)
+    s.sequences, s.capacity, s.filled = 2, 40, 0
+    s.table = torch.zeros((2, 2), dtype=torch.int32)
+    s.lengths = torch.zeros(2, dtype=torch.int32)
+    s.visible = torch.full((2, 2), -1, dtype=torch.int32)
+    kept = [1, 2]  # tokens of each draft
+
+    def accept(ctx, batch, parents, drafted, chosen, width):
+        return None, s.lengths - batch.max_queries + torch.tensor(kept, dtype=torch.int32), None
+
+    monkeypatch.setattr(longcontext, "draft_tree", lambda ctx, batch, parents: (None, None))
+    monkeypatch.setattr(longcontext, "draft_accept", accept)
+    bounds = []
+
+    def attend(batch, q, **kw):
+        bounds.append(batch.max_length)
+        assert batch.max_length >= int(s.lengths.max())
+
+    s.cache = SimpleNamespace(ctx=None, append=lambda *a: None, attend=attend, keep=lambda *a: None)
+    q = torch.zeros((16, 4, 64))
+    for i in range(17):  # 8 tokens of 40, two of them kept: 17 drafts, not 5
+        s.draft(q, q, q, None)
+        s.settle(None, None, 8)
+        assert s.lengths.tolist() == [i + 1, 2 * i + 2]
+    with pytest.raises(ValueError, match="full"):
+        s.draft(q, q, q, None)
+    assert s.lengths.tolist() == [17, 34] and s.filled == 34 and s.pending is None
+    s.grow(6)
+    assert s.lengths.tolist() == [23, 40] and max(bounds) <= 40
+    with pytest.raises(ValueError, match="full"):
+        s.grow(1)
+
+
+def test_a_refused_draft_keeps_the_renewed_bound(monkeypatch):
+    import torch
+    from gofann_amd import longcontext
+    s = longcontext.Session.__new__(longcontext.Session)
+    s.sequences, s.capacity, s.filled, s.loose = 1, 40, 38, True
+    s.table, s.visible = torch.zeros((1, 2), dtype=torch.int32), torch.zeros((1, 2), dtype=torch.int32)
+    s.lengths = torch.full((1,), 9, dtype=torch.int32)
+
+    def refuse(*a):
+        raise ValueError("refused")
+
+    monkeypatch.setattr(longcontext, "draft_tree", refuse)
+    s.cache = SimpleNamespace(ctx=None)
+    q = torch.zeros((8, 4, 64))
+    with pytest.raises(ValueError, match="refused"):
+        s.draft(q, q, q, None)
+    assert s.filled == 9 and s.lengths.tolist() == [9] and s.pending is None
 
 
 # ---- C entries over the stand-in runtime ------------------------------------------
