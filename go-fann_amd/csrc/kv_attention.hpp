@@ -1220,10 +1220,11 @@ __device__ __forceinline__ int shared_row_tiles(const AttendArgs& a, int rows, i
 // kv_join_pieces_kernel joins.  Row tiles of one sequence and head stand next to
 // each other and a piece goes to the XCD that has its neighbours, so that they
 // find their positions in its L2.  32 drafts of 16 tokens, 32 heads to 8, on 500 to
-// 16,000 positions under a filter (109 MB) take 66 us with the list and the join,
-// 80 by splits of one length, whose 5,600 workgroups each had a beginning; 8 of 63
-// tokens, 64 heads, on 4,000 to 30,000 (186 GFLOP) 233 to 250 us, 745 to 800 TFLOP/s;
-// 60 on 200,001 (393 GFLOP) 433 to 452, 870 to 907, what the causal kernel reaches.
+// 16,000 positions under a filter (109 MB) take 65 to 69 us with the list and the
+// join, 80 by splits of one length, whose 5,600 workgroups each had a beginning; 8
+// of 63 tokens, 64 heads, on 4,000 to 30,000 (186 GFLOP) 232 to 250 us, 745 to 800
+// TFLOP/s; 60 on 200,001 (393 GFLOP) 430 to 460, 855 to 915, within what the causal
+// kernel reaches.
 template <int kReach, int kRows, int kStart, class F>
 __device__ __forceinline__ void share_out(const AttendArgs& a, F&& work)
 {

@@ -98,17 +98,28 @@ int split_tiles(const Context* ctx, uint64_t items, uint64_t most, bool ragged, 
     return static_cast<int>(n);
 }
 
-// Sequences whose tiles a workgroup counts for itself, 64 at a time.
+// Sequences whose tiles a workgroup counts for itself, 64 at a time.  Past it
+// nothing is lost: 1,100 of 16 tokens, 32 heads to 8, on 100 to 2,000 positions take
+// 620 us by splits, 730 shared out; of 80 tokens 2,720 and 3,430.
 constexpr uint32_t kMostShared = 1024;
 
 // Whether drafts and cross attention of `rows` rows a sequence share their tiles
 // out by 128 rows a workgroup, not by 16 or 32: past 256, where their row tiles
 // are nearly as full.  8 sequences of 2,000 to 16,000 positions, eight key/value
 // heads, us by few / by 128 rows: 128 channels: 128 rows 42 / 47, 256 rows 81 / 89,
-// 384 rows 123 / 117; 256 channels, four heads: 102 / 104, 160 / 169 and 387 / 403
-// of 256, 384 and 1,024 rows; 64 channels: 59 / 59 and 87 / 76 of 256 and 384; 19
-// drafts of 280 rows of 64 channels 27 / 33.  One sequence of 256 channels stays
-// with few rows further: 1,024 rows on 40,000 positions 239 / 284, on 10,000 76 / 97.
+// 384 rows 123 / 117; 64 channels: 59 / 59 and 87 / 76 of 256 and 384; 19 drafts of
+// 280 rows of 64 channels 27 / 33.  One sequence of 2,800 rows, which goes by 128, would
+// be faster by few: of 128 channels on 3,055 positions 63 / 70, of 64 on 6,502 77 / 83.
+//
+// 256 channels, four heads: 384, 1,024 and 2,000 rows of 16 sequences of 1,000 to 4,000
+// positions 111 / 115, 292 / 279 and 538 / 480; of 8 of 2,000 to 16,000 161 / 168,
+// 387 / 403 and 673 / 700; of 2 of 10,000 65 / 80, 140 / 160 and 219 / 244.  They go by
+// 128 rows for the first; the others lose 4 to 22% by it.  One sequence stays with few
+// rows further: 1,024 rows on 40,000 positions 239 / 284, on 10,000 76 / 97.
+//
+// The longest sequence decides for all.  One of 700 tokens among 63 of one token on 700
+// to 8,000 positions, 32 heads to 8, which goes by 128 rows: 64 channels 137 / 177, 128
+// 125 / 201, 256 411 / 783; a single token's row tile is as long as a full one's.
 bool many_rows(uint64_t rows, uint32_t dim, uint32_t sequences)
 {
     return rows > (dim == 256 && sequences == 1 ? 2048u : 256u) &&
@@ -127,19 +138,23 @@ uint64_t few_tiles(uint64_t rows, uint32_t dim, uint64_t most_tiles)
 
 // Whether few rows share their tiles out at all: up to 16 rows, whose kernels
 // have no registers left for it, and short calls, which a second launch would
-// lengthen, keep splits of one length, joined by the last of them.  One sequence
-// of 2,000 positions and 64 rows of 128 channels takes 18.7 us by splits, 15.7
-// shared out; of 1,000 13.9 and 15.2; 16 sequences of 250 to 1,000 18.5 and 22.2;
-// 16 of 1,000 to 16,000 and 72 rows 32.6 and 30.8; 32 of 500 to 16,000 under a
-// filter 80 and 63.
+// lengthen, keep splits of one length, joined by the last of them.  64 rows of 128
+// channels, eight key/value heads, us by splits / shared out: 16 sequences of 250 to
+// 1,000 positions 17.9 / 21.5, four of 2,000 18.2 / 20.0, four of 1,000 to 4,000
+// 21.6 / 21.5, 16 of 500 to 2,000 25.1 / 25.8, 16 of 1,000 to 16,000 58 / 48, 32 of 500
+// to 16,000 under a filter 80 / 63.  One of 1,000 13.8 / 14.3, of 2,100 20.2 / 14.4; from
+// some 1,200 to 2,048 a single one, which stays with splits, loses by it: of 1,500
+// 17.0 / 14.4, of 2,000 18.8 / 14.6 (64 channels 14.3 / 12.4, 256 23.6 / 15.5).
 bool share_few(uint64_t rows, uint32_t dim, uint64_t items, uint64_t most_tiles, int compute_units)
 {
     return rows > 16 && (most_tiles > 64 || items * most_tiles * dim >= 4096ull * compute_units);
 }
 
-// Tiles of a share at least.  25 tokens on 2,100 positions, 32 heads to 8, by 128
-// rows: 17.8 us with 8, 21.5 with 16 and 27 with 32; few rows of one sequence of
-// 2,000 positions 15.7 with 8 and 16.8 with 16, of four 20.5 and 18.6.
+// Tiles of a share at least, us with 8 / 16 / 32.  64 rows of 128 channels: one
+// sequence of 2,500 positions 14.5 / 15.7 / 17.7, of 8,000 18.8 / 16.4 / 18.8; four of
+// 2,500 21.0 / 21.6 / 21.5, of 4,000 23.8 / 23.7 / 25.5; with more the shares are
+// longer anyway.  512 rows, by 128: one sequence of 2,100 26.1 / 25.0 / 29.3, of 4,000
+// 30.7 / 29.1 / 36.1; four of 1,000 to 2,000 41.2 / 41.7 / 42.3.
 int least_share(bool wide, uint32_t sequences) { return wide || sequences == 1 ? 8 : 16; }
 
 // Bytes that the list of the tiles that a filter leaves may have.
